@@ -321,6 +321,118 @@ int leo_b200_sparse_mean_apply_static(int device, float* target, uint32_t length
    (0 before its first call there; the static variant never adds to it). */
 size_t leo_b200_sparse_apply_scratch_bytes(int device);
 
+/* ---- Operators on caller-owned device tensors: no counterpart in the reference ----
+   All pointers are device memory on `device` unless said otherwise, `dtype`
+   and `decay_dtype` are LeoB200Dtype values, strides count elements between
+   rows (the elements of a row are adjacent), `stream` is a cudaStream_t.  The
+   calls only enqueue: they neither wait nor allocate, the caller's current
+   device is restored, and they can be captured into a CUDA graph.  Outputs
+   must not overlap inputs unless said otherwise. */
+
+/* The story table of a packed batch, on the host: story s owns tokens
+   offsets[s] .. offsets[s + 1] (offsets[0] == 0, fewer than 2^31 tokens).
+   `words` receives ceil(tokens / 32) entries, `order` one per story, `full`
+   the number of stories with a token; the caller copies both arrays to the
+   device and fills a LeoB200StoryTables.  The device calls trust its contents. */
+int leo_b200_story_table(const uint64_t* offsets, uint32_t stories, LeoB200StoryWord* words, uint32_t* order,
+                         uint32_t* full);
+
+/* Bytes of device scratch (any contents) that one call of
+   leo_b200_gated_scan or leo_b200_gated_scan_backward needs for `tokens`
+   tokens of `channels` channels; calls that may overlap in time, or that are
+   captured into different graphs, need scratch of their own. */
+size_t leo_b200_gated_scan_workspace(uint32_t tokens, uint32_t channels);
+/* Floats that leo_b200_gated_scan keeps for its backward pass. */
+size_t leo_b200_gated_scan_carry_count(uint32_t tokens, uint32_t channels);
+
+/* The gated linear recurrence of every story and channel, as the decaying
+   states of the per-byte step are, over whole stories:
+       h[t] = decay[t] * h[t - 1] + drive[t],
+   h before a story's first token being initial[story] (NULL: 0).  States are
+   carried in 32 bits or more; states[t] (dtype, rows adjacent) is rounded
+   once.  `decay` is one row per token (decay_shared 0; of `dtype` or float)
+   or one row for all tokens (decay_shared 1).  Gates are meant to lie in
+   [-1, 1]; a larger one is taken as it is, as long as the product of the
+   gates of any span of a story stays finite.  final_states[story] (float,
+   [stories][channels]) receives the state after the last token, initial[story]
+   for a story without one.  `carries` (NULL: not kept) receives
+   leo_b200_gated_scan_carry_count floats for the backward pass. */
+int leo_b200_gated_scan(int device, const LeoB200StoryTables* tables, uint32_t channels, int dtype,
+                        const void* drive, int64_t drive_stride, int decay_dtype, const void* decay,
+                        int64_t decay_stride, int decay_shared, const float* initial, void* states,
+                        float* final_states, float* carries, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The gradients of leo_b200_gated_scan, given those of its states (dtype)
+   and final states (float; NULL: 0):
+       slope[t] = grad_states[t] + decay[t + 1] * slope[t + 1]  (grad_final after the last token)
+       grad_drive[t] = slope[t],  grad_decay[t] = slope[t] * h[t - 1],
+       grad_initial[story] = decay[first] * slope[first]  (grad_final for a story without a token).
+   h is formed anew in 32 bits from `carries` of the forward call with the
+   same inputs.  grad_drive is of `dtype` and grad_decay of `decay_dtype`,
+   one row per token, rows adjacent; with decay_shared 1 grad_decay is one
+   row, the sum over all tokens in a fixed order.  grad_initial (NULL: not
+   wanted) is float. */
+int leo_b200_gated_scan_backward(int device, const LeoB200StoryTables* tables, uint32_t channels, int dtype,
+                                 const void* grad_states, int64_t grad_states_stride, const void* drive,
+                                 int64_t drive_stride, int decay_dtype, const void* decay, int64_t decay_stride,
+                                 int decay_shared, const float* initial, const float* grad_final,
+                                 const float* carries, void* grad_drive, void* grad_decay, float* grad_initial,
+                                 void* workspace, size_t workspace_bytes, void* stream);
+
+/* A wait between the thread blocks of one scan gave up (it never should: a
+   block only waits for blocks that started before it): the states after it
+   are NaN.  Stores whether that happened on `device` since the library was
+   loaded; waits for the device. */
+int leo_b200_gated_scan_status(int device, uint32_t* gave_up);
+
+/* One token for each of `lanes` lanes: state = decay * state + drive in place
+   (float, [lanes] rows), output = the state in `dtype` (rows adjacent). */
+int leo_b200_gated_step(int device, uint32_t lanes, uint32_t channels, int dtype, const void* drive,
+                        int64_t drive_stride, int decay_dtype, const void* decay, int64_t decay_stride,
+                        int decay_shared, float* state, int64_t state_stride, void* output, void* stream);
+
+/* A row of logits under its rules, symbol v having occurred c times in the
+   row's history:
+       c > 0:  l = l > 0 ? l / repetition : l * repetition;  l -= presence + frequency * c
+       l += bias[v]
+       l = -inf where the mask forbids v, whatever it was before (NaN too).
+   Computed in float, rounded once to `dtype`. */
+int leo_b200_adjust_logits(int device, int dtype, const void* logits, int64_t logits_stride, uint32_t rows,
+                           uint32_t vocabulary, const LeoB200LogitRules* rules, void* out, int64_t out_stride,
+                           void* stream);
+
+/* The next symbol of each row under its rules, computed in double from the
+   inputs as they are.  Temperature 0: the largest adjusted logit, the lowest
+   symbol of equal ones.  Above 0: the first symbol v with
+   sum of p[0..v] > u, p the softmax of the adjusted logits over the
+   temperature and u = uniforms[row] in [0, 1).  log_probability (float; NULL:
+   not wanted) receives log p[v], at temperature 1 for a greedy row.  A row
+   in which nothing is left (everything masked or -inf) gives symbol -1 and
+   -inf; a row with a NaN logit that is not masked, or whose temperature is
+   negative or NaN, gives -1 and NaN.  `temperature` is [rows] or NULL
+   (temperature_value in every row); `uniforms` may be NULL only if that is 0. */
+int leo_b200_pick_symbols(int device, int dtype, const void* logits, int64_t logits_stride, uint32_t rows,
+                          uint32_t vocabulary, const LeoB200LogitRules* rules, const float* temperature,
+                          float temperature_value, const double* uniforms, int32_t* symbols, float* log_probability,
+                          void* stream);
+
+/* Loss and gradient of each row's target under its mask, as the per-byte
+   step forms its loss and errors:
+       losses[r] = log(sum over allowed v of exp l[v]) - l[target]
+       gradient[r][v] = weights[r] * (p[v] - (v == target)),  0 where masked,
+   p the softmax over the allowed symbols (weights NULL: 1; losses are not
+   weighted).  A negative target marks a row without one: loss 0, gradient 0.
+   A target that the mask forbids, or a row in which nothing is left, has loss
+   +inf; the gradient keeps its formula without the target's term in the first
+   case and is 0 in the second.  A target of `vocabulary` or more has loss NaN
+   and gradient 0.  Sums are held in float; the gradient is rounded once to
+   `dtype`. */
+int leo_b200_masked_cross_entropy(int device, int dtype, const void* logits, int64_t logits_stride, uint32_t rows,
+                                  uint32_t vocabulary, const int32_t* targets, const uint32_t* allowed,
+                                  int64_t allowed_stride, uint32_t states, const int32_t* state,
+                                  const float* weights, float* losses, void* gradient, int64_t gradient_stride,
+                                  void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -350,6 +350,59 @@ typedef struct LeoB200PerfStats {
     uint64_t work_winners;  /* block winners (selection records) assembled */
 } LeoB200PerfStats;
 
+/* ---- Operators on caller-owned device tensors ---- */
+
+/* Element types. */
+enum LeoB200Dtype {
+    LEO_B200_F32 = 0,
+    LEO_B200_BF16 = 1,
+    LEO_B200_F16 = 2
+};
+
+#define LEO_B200_STORY_WORD_TOKENS 32u
+
+/* Where stories begin and end in a word of 32 consecutive tokens of a packed
+   batch (leo_b200_story_table).  "A story of the word" has a token in it. */
+typedef struct LeoB200StoryWord {
+    uint32_t starts; /* bit i: token 32 w + i is the first of its story */
+    uint32_t rank;   /* stories with a token that start before token 32 w */
+    uint32_t begin;  /* first token of the story that token 32 w belongs to */
+    uint32_t end;    /* one past the last token of the story that the word's last token belongs to */
+} LeoB200StoryWord;
+
+/* The device copy of a story table. */
+typedef struct LeoB200StoryTables {
+    const LeoB200StoryWord* words; /* device, [ceil(tokens / 32)] */
+    const uint32_t* order;         /* device, [stories]: the stories with a token in order, then those without */
+    uint32_t tokens;
+    uint32_t stories;
+    uint32_t full;                 /* stories with a token */
+} LeoB200StoryTables;
+
+/* What acts on a row of logits before it is used, in this order: penalties
+   for the symbols of the row's history, the bias, the grammar mask.  All
+   pointers are device memory; a NULL `history`, `bias` or `allowed` leaves
+   that part out. */
+typedef struct LeoB200LogitRules {
+    const int32_t* history;     /* [rows] rows of symbols; those outside [0, vocabulary) are passed over */
+    int64_t history_stride;     /* elements between rows */
+    uint32_t history_capacity;  /* columns of `history` */
+    const int32_t* lengths;     /* [rows] symbols in use, clamped to [0, capacity]; NULL: all of them */
+    const float* repetition;    /* [rows], or NULL: repetition_value in every row; > 0 */
+    const float* presence;      /* [rows], or NULL: presence_value */
+    const float* frequency;     /* [rows], or NULL: frequency_value */
+    float repetition_value;
+    float presence_value;
+    float frequency_value;
+    const float* bias;          /* [vocabulary], or [rows] rows of it */
+    int64_t bias_stride;        /* elements between rows; 0: one row for all */
+    const uint32_t* allowed;    /* [states] rows of mask words: bit v % 32 of word v / 32 allows symbol v */
+    int64_t allowed_stride;     /* words between rows */
+    uint32_t states;
+    const int32_t* state;       /* [rows] mask row; -1: nothing is masked; another one outside [0, states): everything.
+                                   NULL: row 0 for all (states == 1) or row r for row r (states == rows) */
+} LeoB200LogitRules;
+
 #ifdef __cplusplus
 }
 #endif

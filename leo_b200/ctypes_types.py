@@ -277,3 +277,41 @@ class LeoB200PerfStats(C.Structure):
         ("work_inhibit", C.c_uint64),
         ("work_winners", C.c_uint64),
     ]
+
+
+F32, BF16, F16 = 0, 1, 2
+
+
+class LeoB200StoryWord(C.Structure):
+    _fields_ = [("starts", C.c_uint32), ("rank", C.c_uint32), ("begin", C.c_uint32), ("end", C.c_uint32)]
+
+
+class LeoB200StoryTables(C.Structure):
+    _fields_ = [
+        ("words", C.c_void_p),
+        ("order", C.c_void_p),
+        ("tokens", C.c_uint32),
+        ("stories", C.c_uint32),
+        ("full", C.c_uint32),
+    ]
+
+
+class LeoB200LogitRules(C.Structure):
+    _fields_ = [
+        ("history", C.c_void_p),
+        ("history_stride", C.c_int64),
+        ("history_capacity", C.c_uint32),
+        ("lengths", C.c_void_p),
+        ("repetition", C.c_void_p),
+        ("presence", C.c_void_p),
+        ("frequency", C.c_void_p),
+        ("repetition_value", C.c_float),
+        ("presence_value", C.c_float),
+        ("frequency_value", C.c_float),
+        ("bias", C.c_void_p),
+        ("bias_stride", C.c_int64),
+        ("allowed", C.c_void_p),
+        ("allowed_stride", C.c_int64),
+        ("states", C.c_uint32),
+        ("state", C.c_void_p),
+    ]

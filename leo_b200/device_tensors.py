@@ -1,0 +1,75 @@
+"""What the operators on CUDA tensors share: element types, argument checks
+and the stream that a call runs on."""
+
+from __future__ import annotations
+
+import contextlib
+
+import torch
+
+from .ctypes_types import BF16, F16, F32
+
+DTYPE_CODES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
+
+
+def dtype_code(name: str, tensor) -> int:
+    code = DTYPE_CODES.get(tensor.dtype)
+    if code is None:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16, not {tensor.dtype}")
+    return code
+
+
+def check_tensor(name: str, tensor, device, dtype=None, shape=None) -> None:
+    """A tensor of the call: a CUDA tensor on ``device`` that asks for no gradient."""
+    if not isinstance(tensor, torch.Tensor) or not tensor.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if tensor.device != device:
+        raise ValueError(f"{name} is on {tensor.device}, not on {device}")
+    if dtype is not None and tensor.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, not {tensor.dtype}")
+    if shape is not None and tensor.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(tensor.shape)}")
+    if tensor.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} asks for a gradient, which this call does not record: detach it and use the "
+                         "gradients that the operators return")
+
+
+def row_stride(name: str, tensor) -> int:
+    """Elements between the rows of a 2-D tensor whose rows are adjacent elements."""
+    if tensor.dim() != 2:
+        raise ValueError(f"{name} must have two dimensions, not {tensor.dim()}")
+    if tensor.shape[1] > 1 and tensor.stride(1) != 1:
+        raise ValueError(f"the elements of a row of {name} must be adjacent")
+    return tensor.stride(0)
+
+
+def check_contiguous(name: str, tensor) -> None:
+    if not tensor.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def pointer(tensor) -> int | None:
+    return None if tensor is None else tensor.data_ptr()
+
+
+@contextlib.contextmanager
+def _other_stream(stream, tensors):
+    with torch.cuda.stream(stream):
+        yield stream.cuda_stream
+    for t in tensors:
+        if t is not None:
+            t.record_stream(stream)
+
+
+def on_stream(device, stream, tensors):
+    """The raw stream of a call: the current one of ``device``, or ``stream``.
+
+    Outputs and scratch are to be allocated inside the context, so that they
+    belong to the stream that writes them; with a ``stream`` other than the
+    current one, ``tensors`` (the call's inputs) are marked as used on it."""
+    current = torch.cuda.current_stream(device)
+    if stream is None or stream == current:
+        return contextlib.nullcontext(current.cuda_stream)
+    if stream.device != device:
+        raise ValueError(f"the stream is on {stream.device}, not on {device}")
+    return _other_stream(stream, tensors)

@@ -1,0 +1,216 @@
+"""The gated linear recurrence over whole stories (``leo_b200_gated_scan``).
+
+The per-byte step decays every neuron's state and every synapse's trace a tick
+at a time.  These operators advance such states over all the tokens of a packed
+story batch in one call,
+
+    h[t] = decay[t] * h[t - 1] + drive[t]     (per channel, from ``initial`` at a story's first token),
+
+with their gradients for training (:func:`gated_scan_backward`) and the
+one-token form for serving (:func:`gated_step`).  Packed tensors hold the
+stories' tokens back to back, ``[tokens, channels]``, as
+:func:`leo_b200.synthetic.pack_stories` packs their bytes; a
+:class:`StoryLayout` made once from the offsets says where they begin.
+
+Types: float32, bfloat16 or float16 drives; gates of the same type or float32
+(slow decays such as 0.999 are 1 in bfloat16); states between tokens, initial
+and final states are float32.  The calls run asynchronously on the current
+stream of the tensors' device, or on ``stream``, and can be captured into a
+CUDA graph.  PyTorch only owns the memory; no gradient is recorded for autograd.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple, Sequence
+
+import numpy as np
+import torch
+
+from . import native
+from .ctypes_types import LeoB200StoryTables, LeoB200StoryWord
+from .device_tensors import check_contiguous, check_tensor, dtype_code, on_stream, pointer, row_stride
+
+
+class StoryLayout:
+    """Where the stories of a packed batch begin, checked once on the host and
+    laid out on ``device`` for the scans.  ``story_offsets``: ``stories + 1``
+    host integers; empty stories are allowed.  The layout may be used by any
+    number of calls, streams and graphs, and must outlive the graphs that captured it."""
+
+    def __init__(self, story_offsets: Sequence[int], device: torch.device | str | int):
+        offsets = np.asarray(story_offsets)
+        if offsets.ndim != 1 or offsets.size < 2 or offsets.dtype.kind not in "iu":
+            raise ValueError("story_offsets must be stories + 1 integers, for one story or more")
+        if offsets.dtype.kind == "i" and int(offsets.min()) < 0:
+            raise ValueError("story_offsets must not be negative")
+        offsets = np.ascontiguousarray(offsets.astype(np.uint64))
+        device = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
+        if device.type != "cuda":
+            raise ValueError("a story layout lives on a CUDA device")
+        stories = offsets.size - 1
+        words = np.zeros((min(int(offsets[-1]), 2**31) + 31) // 32 * 4, dtype=np.uint32)
+        order = np.zeros(stories, dtype=np.uint32)
+        full = C.c_uint32()
+        native.check(native.lib().leo_b200_story_table(offsets.ctypes.data, stories, words.ctypes.data,
+                                                        order.ctypes.data, C.byref(full)))
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        self.device = device
+        self.stories = stories
+        self.tokens = int(offsets[-1])
+        tables = np.concatenate([words, order]).view(np.int32)
+        self._tables = torch.from_numpy(tables).to(device)  # waits for the copy
+        base = self._tables.data_ptr()
+        self._c = LeoB200StoryTables(base, base + words.nbytes, self.tokens, stories, full.value)
+        self._ref = C.byref(self._c)
+
+
+assert C.sizeof(LeoB200StoryWord) == 16
+
+
+class GatedScan(NamedTuple):
+    """``states`` [tokens, channels] of the drive's type, ``final`` [stories,
+    channels] float32, and what the backward pass needs (``None`` unless kept)."""
+
+    states: torch.Tensor
+    final: torch.Tensor
+    carries: torch.Tensor | None
+
+
+class GatedScanGradients(NamedTuple):
+    """Gradients in the types and shapes of ``drive`` and ``decay``;
+    ``initial`` is ``None`` where the scan had no initial state."""
+
+    drive: torch.Tensor
+    decay: torch.Tensor
+    initial: torch.Tensor | None
+
+
+def _check_decay(decay, drive) -> tuple[int, int, int]:
+    """(type code, row stride, one row for all tokens or lanes)."""
+    check_tensor("decay", decay, drive.device)
+    code = dtype_code("decay", decay)
+    if decay.dtype != drive.dtype and decay.dtype != torch.float32:
+        raise ValueError(f"decay must be of the drive's type or float32, not {decay.dtype}")
+    if decay.dim() == 1:
+        if decay.shape[0] != drive.shape[1] or (decay.shape[0] > 1 and decay.stride(0) != 1):
+            raise ValueError("a decay of one row must be one adjacent element a channel")
+        return code, 0, 1
+    if decay.shape != drive.shape:
+        raise ValueError(f"decay must have shape {tuple(drive.shape)} or {tuple(drive.shape[1:])}, "
+                         f"not {tuple(decay.shape)}")
+    return code, row_stride("decay", decay), 0
+
+
+def _check_scan(drive, decay, layout, initial):
+    if not isinstance(drive, torch.Tensor) or not drive.is_cuda:
+        raise ValueError("drive must be a CUDA tensor")
+    check_tensor("drive", drive, drive.device)
+    stride = row_stride("drive", drive)
+    if layout.device != drive.device:
+        raise ValueError(f"the layout is on {layout.device}, not on {drive.device}")
+    if drive.shape[0] != layout.tokens or drive.shape[1] == 0:
+        raise ValueError(f"drive must have {layout.tokens} tokens of at least one channel, not {tuple(drive.shape)}")
+    if initial is not None:
+        check_tensor("initial", initial, drive.device, torch.float32, (layout.stories, drive.shape[1]))
+        check_contiguous("initial", initial)
+    return dtype_code("drive", drive), stride, _check_decay(decay, drive)
+
+
+def gated_scan(drive, decay, layout: StoryLayout, initial=None, keep_carries: bool = False,
+               stream=None) -> GatedScan:
+    """The states of every token of a packed batch.
+
+    ``drive``: [tokens, channels]; ``decay``: the same shape, or [channels] for
+    one fixed decay a channel (the elements of a row adjacent, rows at any
+    distance, so a slice of a wider projection will do).  ``initial``: float32
+    [stories, channels], zero if ``None``.  ``keep_carries``: keep what
+    :func:`gated_scan_backward` needs."""
+    code, stride, (decay_code, decay_stride, shared) = _check_scan(drive, decay, layout, initial)
+    tokens, channels = drive.shape
+    L = native.lib()
+    with on_stream(drive.device, stream, (drive, decay, initial)) as raw:
+        states = torch.empty((tokens, channels), dtype=drive.dtype, device=drive.device)
+        final = torch.empty((layout.stories, channels), dtype=torch.float32, device=drive.device)
+        carries = None
+        if keep_carries:
+            carries = torch.empty(L.leo_b200_gated_scan_carry_count(tokens, channels), dtype=torch.float32,
+                                  device=drive.device)
+        size = L.leo_b200_gated_scan_workspace(tokens, channels)
+        scratch = torch.empty(size, dtype=torch.uint8, device=drive.device) if size else None
+        native.check(L.leo_b200_gated_scan(
+            drive.device.index, layout._ref, channels, code, drive.data_ptr(), stride, decay_code, decay.data_ptr(),
+            decay_stride, shared, pointer(initial), states.data_ptr(), final.data_ptr(), pointer(carries),
+            pointer(scratch), size, raw))
+    return GatedScan(states, final, carries)
+
+
+def gated_scan_backward(grad_states, drive, decay, layout: StoryLayout, carries, initial=None, grad_final=None,
+                        stream=None) -> GatedScanGradients:
+    """The gradients of :func:`gated_scan` for the same ``drive``, ``decay``,
+    ``layout`` and ``initial``, with the ``carries`` that it kept.
+    ``grad_states``: of the drive's shape and type; ``grad_final``: float32
+    [stories, channels], zero if ``None``.  The gradient of a [channels] decay
+    is summed over all tokens in a fixed order."""
+    code, stride, (decay_code, decay_stride, shared) = _check_scan(drive, decay, layout, initial)
+    tokens, channels = drive.shape
+    device = drive.device
+    check_tensor("grad_states", grad_states, device, drive.dtype, drive.shape)
+    grad_stride = row_stride("grad_states", grad_states)
+    if grad_final is not None:
+        check_tensor("grad_final", grad_final, device, torch.float32, (layout.stories, channels))
+        check_contiguous("grad_final", grad_final)
+    L = native.lib()
+    if carries is None:
+        raise ValueError("the backward pass needs the carries of gated_scan(..., keep_carries=True)")
+    check_tensor("carries", carries, device, torch.float32, (L.leo_b200_gated_scan_carry_count(tokens, channels),))
+    check_contiguous("carries", carries)
+    with on_stream(device, stream, (grad_states, drive, decay, carries, initial, grad_final)) as raw:
+        grad_drive = torch.empty((tokens, channels), dtype=drive.dtype, device=device)
+        grad_decay = torch.empty(decay.shape, dtype=decay.dtype, device=device)
+        grad_initial = None
+        if initial is not None:
+            grad_initial = torch.empty((layout.stories, channels), dtype=torch.float32, device=device)
+        size = L.leo_b200_gated_scan_workspace(tokens, channels)
+        scratch = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+        native.check(L.leo_b200_gated_scan_backward(
+            device.index, layout._ref, channels, code, grad_states.data_ptr(), grad_stride, drive.data_ptr(), stride,
+            decay_code, decay.data_ptr(), decay_stride, shared, pointer(initial), pointer(grad_final),
+            carries.data_ptr(), grad_drive.data_ptr(), grad_decay.data_ptr(), pointer(grad_initial),
+            pointer(scratch), size, raw))
+    return GatedScanGradients(grad_drive, grad_decay, grad_initial)
+
+
+def gated_scan_gave_up(device: int = 0) -> bool:
+    """Whether a wait inside a scan on ``device`` ever gave up (its states are
+    then NaN from there on).  Waits for the device."""
+    flag = C.c_uint32()
+    native.check(native.lib().leo_b200_gated_scan_status(device, C.byref(flag)))
+    return bool(flag.value)
+
+
+def gated_step(drive, decay, state, stream=None):
+    """One token for each lane: ``state`` (float32 [lanes, channels]) becomes
+    ``decay * state + drive`` in place; returns it in the drive's type.
+    ``drive``: [lanes, channels]; ``decay``: the same shape, or [channels]."""
+    if not isinstance(drive, torch.Tensor) or not drive.is_cuda:
+        raise ValueError("drive must be a CUDA tensor")
+    device = drive.device
+    check_tensor("drive", drive, device)
+    stride = row_stride("drive", drive)
+    code = dtype_code("drive", drive)
+    lanes, channels = drive.shape
+    if channels == 0:
+        raise ValueError("drive must have at least one channel")
+    decay_code, decay_stride, shared = _check_decay(decay, drive)
+    check_tensor("state", state, device, torch.float32, drive.shape)
+    state_stride = row_stride("state", state)
+    if lanes > 1 and state_stride < channels:
+        raise ValueError("the rows of state overlap")
+    with on_stream(device, stream, (drive, decay, state)) as raw:
+        output = torch.empty((lanes, channels), dtype=drive.dtype, device=device)
+        native.check(native.lib().leo_b200_gated_step(
+            device.index, lanes, channels, code, drive.data_ptr(), stride, decay_code, decay.data_ptr(), decay_stride,
+            shared, state.data_ptr(), state_stride, output.data_ptr(), raw))
+    return output

@@ -12,6 +12,7 @@ from .ctypes_types import (
     LeoB200BatchReport,
     LeoB200Config,
     LeoB200HostModel,
+    LeoB200LogitRules,
     LeoB200PackedUpdate,
     LeoB200ParameterChanges,
     LeoB200ParameterChangeSizes,
@@ -20,6 +21,7 @@ from .ctypes_types import (
     LeoB200StoryDeltas,
     LeoB200StoryDeltaSizes,
     LeoB200StorySummary,
+    LeoB200StoryTables,
 )
 
 PKG = Path(__file__).resolve().parent
@@ -109,6 +111,21 @@ def lib() -> C.CDLL:
     L.leo_b200_parameter_changes.argtypes = [vp, P(LeoB200ParameterChangeSizes), P(LeoB200ParameterChanges)]
     L.leo_b200_synchronize_packed_model.argtypes = [vp, P(LeoB200PackedUpdate)]
     L.leo_b200_commit_packed_host_model.argtypes = [vp, P(LeoB200PackedUpdate)]
+    i32, i64, f32 = C.c_int, C.c_int64, C.c_float
+    L.leo_b200_story_table.argtypes = [vp, u32, vp, vp, P(u32)]
+    L.leo_b200_gated_scan_workspace.argtypes = [u32, u32]
+    L.leo_b200_gated_scan_workspace.restype = sz
+    L.leo_b200_gated_scan_carry_count.argtypes = [u32, u32]
+    L.leo_b200_gated_scan_carry_count.restype = sz
+    L.leo_b200_gated_scan.argtypes = [i32, P(LeoB200StoryTables), u32, i32, vp, i64, i32, vp, i64, i32, vp, vp, vp, vp,
+                                      vp, sz, vp]
+    L.leo_b200_gated_scan_backward.argtypes = [i32, P(LeoB200StoryTables), u32, i32, vp, i64, vp, i64, i32, vp, i64,
+                                               i32, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+    L.leo_b200_gated_scan_status.argtypes = [i32, P(u32)]
+    L.leo_b200_gated_step.argtypes = [i32, u32, u32, i32, vp, i64, i32, vp, i64, i32, vp, i64, vp, vp]
+    L.leo_b200_adjust_logits.argtypes = [i32, i32, vp, i64, u32, u32, P(LeoB200LogitRules), vp, i64, vp]
+    L.leo_b200_pick_symbols.argtypes = [i32, i32, vp, i64, u32, u32, P(LeoB200LogitRules), vp, f32, vp, vp, vp, vp]
+    L.leo_b200_masked_cross_entropy.argtypes = [i32, i32, vp, i64, u32, u32, vp, vp, i64, u32, vp, vp, vp, vp, i64, vp]
     _lib = L
     return L
 
