@@ -4,23 +4,29 @@
 //   h[t] = a[t] h[t-1] + x[t]
 //   slope[t] = g[t] + a[t+1] slope[t+1];  dx = slope, da[t] = slope[t] h[t-1]
 //
-// Tiles.  The packed batch is cut into tiles of 128 tokens whatever its
-// stories are, so a ragged batch balances by itself; a block of 8 warps takes a
-// tile of 32 V channels, each thread 16 tokens in a row of V channels, which it
-// reads once into registers.  A span of tokens maps the state before it to the
-// state after it as h -> A h + H (A the product of the gates, H the state from
-// zero), or as h -> H if a story starts inside, and such maps compose: the
-// threads' maps give the tile's, the tiles' maps give the state before a tile,
-// and each thread then runs its 16 tokens again from registers and writes them.
-// The backward pass is the same from the right, with m -> A m + M for
-// m[t] = a[t] slope[t]; h is formed anew from the tile's carry.
+// Tiles.  The packed batch is cut into tiles of equal length whatever its
+// stories are, so a ragged batch balances by itself; a block of 16 warps takes
+// a tile of 64 channels, each thread a segment of a few tokens in a row of two
+// channels.  A span of tokens maps the state before it to the state after it
+// as h -> A h + H (A the product of the gates, H the state from zero), or as
+// h -> H if a story starts inside, and such maps compose: the segments' maps
+// give the tile's, the tiles' maps the state before a tile, and each thread
+// then runs its tokens again and writes them.  The backward pass is the same
+// from the right, with m -> A m + M for m[t] = a[t] slope[t]; h is formed anew
+// from the states that the forward pass keeps every 64 tokens.
 //
-// The state before a tile comes from the tiles before it in the same launch:
-// tiles are dealt by a ticket in token order, so a block only ever waits for
-// blocks that have started.  Each publishes its map; every kGroup-th tile
-// publishes the state after it instead, so that a tile reads at most kGroup
-// slots.  Which slots are read, and in which order they are composed, depends
-// on the layout alone: results are the same in every run.
+// Pipeline.  One block an SM works through tiles dealt by a ticket in token
+// order.  While the loads of tile i + 2 are in flight into its own third of
+// shared memory (each thread copies what it will use itself, so they need no
+// barrier), the threads map tile i + 1 and write tile i, and two more warps
+// compose tile i + 1.  Every input is read once and the loads never pause.
+//
+// Between tiles.  Each tile publishes its map, every kGroup-th the state after
+// it instead, so a tile reads at most kGroup slots of tiles with lower
+// tickets, which have started before it.  A slot and its mark are one 16-byte
+// word, written and read as one, so a slot that is there costs one trip to L2.
+// Which slots are read, and in which order they are composed, depends on the
+// layout alone: results are the same in every run.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -46,85 +52,105 @@ __device__ __forceinline__ void store(__half* p, float v) { *p = __float2half_rn
 
 constexpr uint32_t kThreads = 128;  // of the step and the reduction
 
-constexpr int kSegment = 16;                      // tokens of a thread
-constexpr int kTileWarps = 8;
-constexpr uint32_t kTile = kSegment * kTileWarps;  // tokens of a block
-constexpr uint32_t kTileThreads = 32 * kTileWarps;
-constexpr uint32_t kGroup = 16;                    // tiles between published states
-constexpr uint32_t kSpinLimit = 1u << 21;          // polls of a wait, 32 ns and a memory round trip apart
-static_assert(kTile % LEO_B200_STORY_WORD_TOKENS == 0 && LEO_B200_STORY_WORD_TOKENS % kSegment == 0, "story words");
+constexpr int kWarps = 16;                       // that map and write a tile
+constexpr int kColumns = 64;                     // channels of a tile
+constexpr int kCarryWarps = kColumns / 16;       // that compose it, two lanes a channel
+constexpr uint32_t kTileThreads = 32 * (kWarps + kCarryWarps);
+constexpr int kStages = 3;
+constexpr uint32_t kNone = 0xffffffffu;
+constexpr size_t kSharedLimit = 227 * 1024;
+constexpr uint32_t kKept = 64;                   // tokens between the states kept for the backward pass
+constexpr int kGroup = 16;                       // tiles between published states
+constexpr uint32_t kSpinLimit = 1u << 21;        // polls of a wait, a memory round trip and more apart
 
 __device__ uint32_t g_gave_up;
 
-// V elements of a row as they lie in memory, read or written once.
-template <typename T, int V> struct Packed;
-template <> struct Packed<float, 1> {
-    using Raw = float;
-    static __device__ __forceinline__ void unpack(Raw r, float (&v)[1]) { v[0] = r; }
-    static __device__ __forceinline__ Raw pack(const float (&v)[1]) { return v[0]; }
+// Two floats as the packed instructions take them.
+using Pair32 = unsigned long long;
+__device__ __forceinline__ Pair32 pair_of(float x, float y) {
+    Pair32 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 parts(Pair32 p) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+    return r;
+}
+__device__ __forceinline__ Pair32 fma2(Pair32 a, Pair32 b, Pair32 c) {
+    Pair32 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ Pair32 mul2(Pair32 a, Pair32 b) {
+    Pair32 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Pair32 add2(Pair32 a, Pair32 b) {
+    Pair32 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// Two neighbours of a row as they lie in memory.
+template <typename T> struct Packed;
+template <> struct Packed<float> {
+    using Raw = Pair32;
+    static __device__ __forceinline__ Pair32 unpack(Raw r) { return r; }
+    static __device__ __forceinline__ Raw pack(Pair32 v) { return v; }
 };
-template <> struct Packed<float, 2> {
-    using Raw = float2;
-    static __device__ __forceinline__ void unpack(Raw r, float (&v)[2]) { v[0] = r.x, v[1] = r.y; }
-    static __device__ __forceinline__ Raw pack(const float (&v)[2]) { return make_float2(v[0], v[1]); }
-};
-template <> struct Packed<__nv_bfloat16, 1> {
-    using Raw = unsigned short;
-    static __device__ __forceinline__ void unpack(Raw r, float (&v)[1]) { v[0] = __uint_as_float((uint32_t)r << 16); }
-    static __device__ __forceinline__ Raw pack(const float (&v)[1]) {
-        return __bfloat16_as_ushort(__float2bfloat16_rn(v[0]));
-    }
-};
-template <> struct Packed<__nv_bfloat16, 2> {
+template <> struct Packed<__nv_bfloat16> {
     using Raw = unsigned int;
-    static __device__ __forceinline__ void unpack(Raw r, float (&v)[2]) {
-        v[0] = __uint_as_float(r << 16), v[1] = __uint_as_float(r & 0xffff0000u);
+    static __device__ __forceinline__ Pair32 unpack(Raw r) {
+        return pair_of(__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u));
     }
-    static __device__ __forceinline__ Raw pack(const float (&v)[2]) {
-        return (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(v[0])) |
-               (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(v[1])) << 16;
+    static __device__ __forceinline__ Raw pack(Pair32 v) {
+        const float2 f = parts(v);
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+        return *reinterpret_cast<const Raw*>(&h);
     }
 };
-template <> struct Packed<__half, 1> {
-    using Raw = unsigned short;
-    static __device__ __forceinline__ void unpack(Raw r, float (&v)[1]) { v[0] = __half2float(__ushort_as_half(r)); }
-    static __device__ __forceinline__ Raw pack(const float (&v)[1]) { return __half_as_ushort(__float2half_rn(v[0])); }
-};
-template <> struct Packed<__half, 2> {
+template <> struct Packed<__half> {
     using Raw = unsigned int;
-    static __device__ __forceinline__ void unpack(Raw r, float (&v)[2]) {
-        v[0] = __half2float(__ushort_as_half((unsigned short)r));
-        v[1] = __half2float(__ushort_as_half((unsigned short)(r >> 16)));
+    static __device__ __forceinline__ Pair32 unpack(Raw r) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r));
+        return pair_of(f.x, f.y);
     }
-    static __device__ __forceinline__ Raw pack(const float (&v)[2]) {
-        return (uint32_t)__half_as_ushort(__float2half_rn(v[0])) |
-               (uint32_t)__half_as_ushort(__float2half_rn(v[1])) << 16;
+    static __device__ __forceinline__ Raw pack(Pair32 v) {
+        const float2 f = parts(v);
+        const __half2 h = __floats2half2_rn(f.x, f.y);
+        return *reinterpret_cast<const Raw*>(&h);
     }
 };
 
-template <typename T, int V>
-__device__ __forceinline__ typename Packed<T, V>::Raw read_once(const T* p) {
-    return __ldcs(reinterpret_cast<const typename Packed<T, V>::Raw*>(p));
+// What a tile tells the tiles behind it, in one 8-byte word: its map (A, H),
+// or the state after it as H.  All bits set: nothing yet (a NaN of that form
+// is written as another one).
+using Slot = unsigned long long;
+__device__ __forceinline__ void write_slot(Slot* p, float A, float H) {
+    uint32_t low = __float_as_uint(A);
+    if (low == kNone) low = 0x7fffffffu;
+    asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"((Slot)__float_as_uint(H) << 32 | low) : "memory");
 }
-template <typename T, int V>
-__device__ __forceinline__ void write_once(T* p, const float (&v)[V]) {
-    __stcs(reinterpret_cast<typename Packed<T, V>::Raw*>(p), Packed<T, V>::pack(v));
+__device__ __forceinline__ Slot read_slot(const Slot* p) {
+    Slot s;
+    asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(s) : "l"(p) : "memory");
+    return s;
 }
 
-// The scratch of one call: the ticket, a flag for every 32 channels of a tile,
-// a slot for every channel of a tile, and the partial sums of a shared gate's
-// gradient.  Ticket and flags are zeroed before the launch.
+// The scratch of one call: a slot for every channel of a tile (all bits set
+// before the launch), the ticket before them (set to -1 with them), and the
+// partial sums of a shared gate's gradient.
 struct Scratch {
     uint32_t* ticket;
-    uint32_t* flags;   // [tiles][flag_row]
-    double2* slots;    // [tiles][channels]: (A, H), or (-, state)
-    float* partials;   // [tiles][channels]
-    uint32_t flag_row;
+    Slot* slots;      // [tiles][channels]
+    float* partials;  // [tiles][channels]
 };
 
 struct ScanArgs {
     LeoB200StoryTables tables;
-    uint32_t channels, tiles, groups;  // groups: of 32 V channels
+    uint32_t channels, tiles, groups;  // groups: of 64 channels
     const void* drive;
     int64_t drive_stride;
     const void* decay;
@@ -132,7 +158,7 @@ struct ScanArgs {
     const float* initial;
     void* states;
     float* final_states;
-    float* carries;  // [tiles][channels]: the state before each tile
+    float* carries;  // [every 64 tokens][channels]: the state before them
     // backward
     const void* grad_states;
     int64_t grad_states_stride;
@@ -143,25 +169,25 @@ struct ScanArgs {
     Scratch scratch;
 };
 
-// A thread's 16 tokens among the stories.
+// A thread's tokens among the stories.
 struct Segment {
-    uint32_t first;    // token
-    int count;         // tokens before the batch's end
-    uint32_t starts;   // bit i: token first + i is the first of its story
-    uint32_t ends;     // bit i: ... the last
-    uint32_t rank;     // stories that start before `first`
+    int count;        // tokens before the batch's end
+    uint32_t starts;  // bit i: token i of the segment is the first of its story
+    uint32_t ends;    // bit i: ... the last
+    uint32_t rank;    // stories that start before the segment
 };
 
-__device__ __forceinline__ Segment segment_at(const LeoB200StoryTables& t, uint32_t first) {
-    Segment s{first, 0, 0, 0, 0};
+// `word`: the story word of token `first`.
+template <int Length>
+__device__ __forceinline__ Segment segment_of(const LeoB200StoryTables& t, uint4 word, uint32_t first) {
+    Segment s{0, 0, 0, 0};
     if (first >= t.tokens) return s;
-    s.count = (int)min(t.tokens - first, (uint32_t)kSegment);
-    const uint4 w = __ldg(reinterpret_cast<const uint4*>(t.words) + (first >> 5));  // starts, rank, begin, end
+    s.count = (int)min(t.tokens - first, (uint32_t)Length);
     const uint32_t base = first & ~31u, shift = first & 31u;
-    const uint32_t ends = (w.x >> 1) | (w.w <= base + 32u ? 1u << (w.w - 1u - base) : 0u);
-    s.starts = (w.x >> shift) & ((1u << kSegment) - 1u);
-    s.ends = (ends >> shift) & ((1u << kSegment) - 1u);
-    s.rank = w.y + __popc(w.x & ((1u << shift) - 1u));
+    const uint32_t ends = (word.x >> 1) | (word.w <= base + 32u ? 1u << (word.w - 1u - base) : 0u);
+    s.starts = (word.x >> shift) & ((1u << Length) - 1u);
+    s.ends = (ends >> shift) & ((1u << Length) - 1u);
+    s.rank = word.y + __popc(word.x & ((1u << shift) - 1u));
     return s;
 }
 // The story that starts at, or ends with, token i of the segment.
@@ -172,412 +198,575 @@ __device__ __forceinline__ uint32_t story_ending(const LeoB200StoryTables& t, co
     return __ldg(t.order + s.rank + __popc(s.starts & ((2u << i) - 1u)) - 1u);
 }
 
-template <int V>
-__device__ __forceinline__ void row_or_zero(const float* rows, uint32_t row, uint32_t channels, uint32_t c,
-                                            bool active, float (&v)[V]) {
-#pragma unroll
-    for (int k = 0; k < V; ++k) v[k] = rows && active ? __ldg(rows + (size_t)row * channels + c + k) : 0.0f;
-}
-
 // A product of gates as hi + lo: the rounding of every factor is kept
 // (p = hi a, e = hi a - p exactly), so that the map of a long span of slow
 // gates is exact to float32 where a plain product would drift by a rounding a
 // token, the same one in every span if the gates are constant.
-struct Product {
-    float hi = 1.0f, lo = 0.0f;
-    __device__ __forceinline__ void times(float a) {
-        const float p = hi * a;
-        lo = fmaf(lo, a, fmaf(hi, a, -p));
+struct Product2 {  // of two channels
+    Pair32 hi = pair_of(1.0f, 1.0f), lo = 0;
+    __device__ __forceinline__ void times(Pair32 a) {
+        const Pair32 p = mul2(hi, a);
+        lo = fma2(lo, a, fma2(hi, a, p ^ 0x8000000080000000ull));
         hi = p;
     }
-    __device__ __forceinline__ double value() const {
-        // an infinite product has no error term
-        return isfinite(hi) ? (double)hi + (double)lo : (double)hi;
-    }
 };
-
-// Waits until `flag` is set; false if it gave up.
-__device__ __forceinline__ bool wait_for(const uint32_t* flag) {
-    for (uint32_t n = 0; n < kSpinLimit; ++n) {
-        uint32_t v;
-        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(flag) : "memory");
-        if (v) return true;
-        __nanosleep(32);
-    }
-    atomicExch(&g_gave_up, 1u);
-    return false;
+__device__ __forceinline__ float2 product_of(float2 x, float2 y) {  // (hi, lo)
+    const float p = x.x * y.x;
+    return make_float2(p, fmaf(x.x, y.y, fmaf(x.y, y.x, fmaf(x.x, y.x, -p))));
+}
+__device__ __forceinline__ float value_of(float2 x) {
+    return x.y == x.y ? x.x + x.y : x.x;  // an infinite product has no error term
 }
 
-__device__ __forceinline__ double2 read_slot(const double2* p) {
-    return __ldcg(p);
-}
-
-// One warp, a channel a lane.  The state before tile `tile` in the direction
-// of the scan (+1: from the left), from the tile that holds the near end of the
-// story that crosses into it (`holder`) or a nearer one that published a state.
+// The state before a tile, out of the slots between it and the tile that holds
+// the near end of the story that crosses into it, or the nearest one that
+// published a state.  Direction +1: from the left; -1: from the right.
 template <int Direction>
-__device__ __forceinline__ double carry_into(const Scratch& s, uint32_t tile, uint32_t holder, uint32_t flag_at,
-                                             uint32_t channels, uint32_t c, bool active) {
-    const uint32_t lane = threadIdx.x & 31u;
-    // Tiles that publish a state: the last of a group of kGroup seen in the direction of the scan.
-    uint32_t from = holder;
-    if (Direction > 0) {
-        const uint32_t p = tile / kGroup * kGroup;  // its left neighbour ends a group
-        if (p > holder + 1) from = p - 1;
-    } else {
-        const uint32_t p = (tile / kGroup + 1) * kGroup;
-        if (p < holder) from = p;
+struct Lookback {
+    uint32_t from;  // tile whose slot is a state
+    int maps;       // tiles between it and this one; -1: no story crosses in
+    // The first or last token of the story that crosses into a tile, read ahead of time.
+    static __device__ __forceinline__ uint32_t end_of(const ScanArgs& a, uint32_t tile, uint32_t words_a_tile) {
+        if (a.tiles == 1 || tile == kNone) return 0;
+        const uint32_t words = (a.tables.tokens + 31) / 32;
+        if (Direction > 0) return __ldg(&a.tables.words[tile * words_a_tile].begin);
+        return __ldg(&a.tables.words[min((tile + 1) * words_a_tile, words) - 1].end) - 1;
     }
-    const uint32_t maps = Direction > 0 ? tile - 1 - from : from - tile - 1;  // below kGroup
-    bool ok = true;
-    if (lane < maps) {
-        const uint32_t at = Direction > 0 ? from + 1 + lane : from - 1 - lane;
-        ok = wait_for(s.flags + (size_t)at * s.flag_row + flag_at);
-    }
-    ok = __all_sync(0xffffffffu, ok);
-    __syncwarp();
-    double A = 1.0, H = 0.0;
-    if (active)
-        for (uint32_t j = 0; j < maps; ++j) {
-            const uint32_t at = Direction > 0 ? from + 1 + j : from - 1 - j;
-            const double2 m = read_slot(s.slots + (size_t)at * channels + c);
-            H = fma(m.x, H, m.y);
-            A *= m.x;
+    __device__ __forceinline__ Lookback(const ScanArgs& a, uint32_t tile, uint32_t end, uint32_t words_a_tile) {
+        maps = -1;
+        from = tile;
+        if (a.tiles == 1) return;
+        const uint32_t holder = end / (32 * words_a_tile);
+        if (holder == tile) return;
+        from = holder;
+        // A state is published by the last tile of a group of kGroup in the direction of the scan.
+        if (Direction > 0) {
+            const uint32_t p = tile / kGroup * kGroup;
+            if (p > holder + 1) from = p - 1;
+            maps = (int)(tile - 1 - from);
+        } else {
+            const uint32_t p = (tile / kGroup + 1) * kGroup;
+            if (p < holder) from = p;
+            maps = (int)(from - tile - 1);
         }
-    if (lane == 0) ok = ok && wait_for(s.flags + (size_t)from * s.flag_row + flag_at);
-    ok = __all_sync(0xffffffffu, ok);
-    __syncwarp();
-    if (!ok) return CUDART_NAN;
-    if (!active) return 0.0;
-    const double before = read_slot(s.slots + (size_t)from * channels + c).y;
-    return maps ? fma(A, before, H) : before;
-}
-
-__device__ __forceinline__ void publish(const Scratch& s, uint32_t tile, uint32_t flag_at, uint32_t channels,
-                                        uint32_t c, bool active, double A, double H) {
-    if (active) __stcg(s.slots + (size_t)tile * channels + c, make_double2(A, H));
-    __syncwarp();
-    if ((threadIdx.x & 31u) == 0) {
-        __threadfence();
-        asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(s.flags + (size_t)tile * s.flag_row + flag_at), "r"(1u)
-                     : "memory");
     }
-}
-
-// The maps of a tile's segments, and the states before them.
-template <int V>
-struct TileMaps {
-    double A[kTileWarps][32 * V];
-    float H[kTileWarps][32 * V];
-    float before[kTileWarps][32 * V];
-    uint32_t reset[kTileWarps];
-    uint32_t ticket;
+    // Reads half the slots of a channel once: the state and the first seven
+    // maps (half 0), or the other eight (half 1), composed as (A, H).  False if
+    // one of them is not there yet.
+    __device__ __forceinline__ bool read(const Slot* slots, uint32_t channels, uint32_t c, int half, float& A,
+                                         float& H) const {
+        const int64_t step = (int64_t)Direction * channels;
+        const int count = min(maps + 1 - half * 8, 8);
+        const Slot* p = slots + (size_t)from * channels + c + half * 8 * step;
+        Slot s[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < count) s[j] = read_slot(p + j * step);
+        uint32_t there = 1;
+        A = 1.0f, H = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < count) {
+                const uint32_t low = (uint32_t)s[j];
+                there &= low != kNone;
+                H = fmaf(__uint_as_float(low), H, __uint_as_float((uint32_t)(s[j] >> 32)));
+                A *= __uint_as_float(low);
+                if (j == 0 && half == 0) H = __uint_as_float((uint32_t)(s[j] >> 32));
+            }
+        return there;
+    }
 };
 
-// The block's tile and channel group.
-template <int V>
-__device__ __forceinline__ uint32_t take_ticket(const ScanArgs& a, TileMaps<V>& maps) {
-    if (a.tiles == 1) return blockIdx.x;
-    if (threadIdx.x == 0) maps.ticket = atomicAdd(a.scratch.ticket, 1u);
-    __syncthreads();
-    return maps.ticket;
+// The shape of a kernel: its tiles, and its shared memory.
+template <typename T, typename G, bool Shared, bool Backward>
+struct Shape {
+    // A token of a tile takes this much of a stage.
+    static constexpr int kRow = kColumns * (int)((Backward ? 2 : 1) * sizeof(T) + (Shared ? 0 : sizeof(G)));
+    struct Maps {
+        float2 A[kWarps][kColumns];                // hi, lo
+        float H[kWarps][kColumns];                 // then the state before each segment
+        float M[Backward ? kWarps : 1][kColumns];  // then the value before each segment from the right
+        uint8_t starts[kWarps], ends[kWarps];      // whether a story does in the segment
+    };
+    struct Control {
+        Maps maps[2];
+        float sums[Backward && Shared ? 2 : 1][Backward && Shared ? kWarps : 1][kColumns];
+        uint2 ring[8];  // the block's (tile, group)s; an entry is rewritten when no warp reads it any more
+    };
+    // 8 tokens a thread, or 4 where three stages of them would not fit.
+    static constexpr size_t kStageOf8 = (size_t)8 * kWarps * kRow;
+    static constexpr int kSegment = kStages * kStageOf8 + sizeof(Control) <= kSharedLimit ? 8 : 4;
+    static constexpr uint32_t kTile = kSegment * kWarps;
+    static constexpr size_t kStage = (size_t)kTile * kRow;
+    static constexpr size_t kBytes = kStages * kStage + sizeof(Control);
+};
+
+template <int Id>
+__device__ __forceinline__ void barrier_sync() {
+    asm volatile("bar.sync %0, %1;" ::"n"(Id), "n"(kTileThreads) : "memory");
+}
+template <int Id>
+__device__ __forceinline__ void barrier_arrive() {
+    asm volatile("bar.arrive %0, %1;" ::"n"(Id), "n"(kTileThreads) : "memory");
+}
+// Named barriers: 1, 2 the segments' maps are written; 3, 4 the states before them are.
+template <int Base>
+__device__ __forceinline__ void sync_of(uint32_t parity) {
+    parity ? barrier_sync<Base + 1>() : barrier_sync<Base>();
+}
+template <int Base>
+__device__ __forceinline__ void arrive_at(uint32_t parity) {
+    parity ? barrier_arrive<Base + 1>() : barrier_arrive<Base>();
 }
 
-// Composes the tile's segments after a barrier: the first V warps, a channel a
-// lane, publish the tile's map or state and write the state before each segment.
-// Returns the state before the tile in those warps.
-template <int V, int Direction>
-__device__ __forceinline__ double compose_tile(const ScanArgs& a, TileMaps<V>& maps, uint32_t tile, uint32_t group) {
-    const uint32_t warp = threadIdx.x >> 5;
-    double carry = 0.0;
-    if (warp < V) {
-        const uint32_t k = threadIdx.x;  // channel of the group
-        const uint32_t c = group * 32 * V + k, flag_at = group * V + warp;
-        const bool active = c < a.channels;
-        double A = 1.0, H = 0.0;
-        bool reset = false;
+template <int Bytes>
+__device__ __forceinline__ void copy_async(void* shared, const void* global) {
+    const uint32_t to = (uint32_t)__cvta_generic_to_shared(shared);
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(global), "n"(Bytes) : "memory");
+}
+
+// A thread's two channels of a row: a pair of neighbours, or, where the rows do
+// not allow that, two that lie 32 apart.
+template <bool Pair>
+struct Columns {
+    uint32_t at[2];  // in the tile
+    bool in[2];      // below the batch's channels
+    uint32_t c;      // the first channel
+    __device__ __forceinline__ Columns(uint32_t group, uint32_t channels) {
+        const uint32_t lane = threadIdx.x & 31u;
+        at[0] = Pair ? 2 * lane : lane;
+        at[1] = Pair ? at[0] + 1 : at[0] + 32;
+        c = group * kColumns + at[0];
+        in[0] = c < channels;
+        in[1] = c + (at[1] - at[0]) < channels;
+    }
+    template <typename E>
+    __device__ __forceinline__ void copy(E* tile_row, const E* row) const {
+        if constexpr (Pair) {
+            if (in[0]) copy_async<2 * sizeof(E)>(tile_row + at[0], row);
+        } else {
 #pragma unroll
-        for (int j = 0; j < kTileWarps; ++j) {
-            const int w = Direction > 0 ? j : kTileWarps - 1 - j;
-            if (maps.reset[w]) {
-                H = maps.H[w][k];
-                reset = true;
-            } else {
-                H = fma(maps.A[w][k], H, (double)maps.H[w][k]);
-                A *= maps.A[w][k];
-            }
-        }
-        // Does a story cross into the tile, and which tile holds its other end?
-        const uint32_t words = (a.tables.tokens + 31) / 32;
-        uint32_t holder = tile;
-        if (a.tiles > 1) {
-            if (Direction > 0)
-                holder = __ldg(&a.tables.words[tile * (kTile / 32)].begin) / kTile;
-            else
-                holder = (__ldg(&a.tables.words[min((tile + 1) * (kTile / 32), words) - 1].end) - 1) / kTile;
-        }
-        const bool last = Direction > 0 ? tile + 1 == a.tiles : tile == 0;
-        const bool state_tile = Direction > 0 ? (tile + 1) % kGroup == 0 : tile % kGroup == 0;
-        if (!last && (reset || !state_tile)) publish(a.scratch, tile, flag_at, a.channels, c, active, A, H);
-        if (holder != tile) {
-            carry = carry_into<Direction>(a.scratch, tile, holder, flag_at, a.channels, c, active);
-            if (!last && !reset && state_tile)
-                publish(a.scratch, tile, flag_at, a.channels, c, active, 0.0, fma(A, carry, H));
-        } else if (!last && !reset && state_tile) {
-            publish(a.scratch, tile, flag_at, a.channels, c, active, 0.0, H);
-        }
-        double before = carry;
-#pragma unroll
-        for (int j = 0; j < kTileWarps; ++j) {
-            const int w = Direction > 0 ? j : kTileWarps - 1 - j;
-            maps.before[w][k] = (float)before;
-            before = maps.reset[w] ? (double)maps.H[w][k] : fma(maps.A[w][k], before, (double)maps.H[w][k]);
+            for (int k = 0; k < 2; ++k)
+                if (in[k]) {
+                    if constexpr (sizeof(E) == 4)
+                        copy_async<4>(tile_row + at[k], row + 32 * k);
+                    else
+                        tile_row[at[k]] = row[32 * k];
+                }
         }
     }
-    return carry;
-}
+    template <typename E>
+    __device__ __forceinline__ Pair32 get(const E* tile_row) const {
+        if constexpr (Pair)
+            return Packed<E>::unpack(*reinterpret_cast<const typename Packed<E>::Raw*>(tile_row + at[0]));
+        else
+            return pair_of(load(tile_row + at[0]), load(tile_row + at[1]));
+    }
+    template <typename E>
+    __device__ __forceinline__ void put(E* row, Pair32 v) const {
+        if constexpr (Pair) {
+            if (in[0]) __stcs(reinterpret_cast<typename Packed<E>::Raw*>(row), Packed<E>::pack(v));
+        } else {
+            const float2 f = parts(v);
+            if (in[0]) store(row, f.x);
+            if (in[1]) store(row + 32, f.y);
+        }
+    }
+    // Of a row that all tokens share.
+    template <typename E>
+    __device__ __forceinline__ Pair32 get_shared(const E* row) const {
+        return pair_of(in[0] ? load(row + c) : 0.0f, in[1] ? load(row + c + (Pair ? 1 : 32)) : 0.0f);
+    }
+    // Of a row of [stories][channels] float: zero where there is none.
+    __device__ __forceinline__ Pair32 get_row(const float* rows, uint32_t row, uint32_t channels) const {
+        const float* p = rows + (size_t)row * channels + c;
+        return pair_of(rows && in[0] ? __ldg(p) : 0.0f, rows && in[1] ? __ldg(p + (Pair ? 1 : 32)) : 0.0f);
+    }
+    __device__ __forceinline__ void put_row(float* rows, uint32_t row, uint32_t channels, Pair32 v) const {
+        float* p = rows + (size_t)row * channels + c;
+        const float2 f = parts(v);
+        if (in[0]) p[0] = f.x;
+        if (in[1]) p[Pair ? 1 : 32] = f.y;
+    }
+};
 
-// Stories without a token keep their initial (forward) or final (backward) row.
-__device__ __forceinline__ void copy_empty(const LeoB200StoryTables& t, uint32_t channels, uint32_t c0, uint32_t width,
+// Stories without a token keep their initial (forward) or final (backward) value.
+__device__ __forceinline__ void copy_empty(const LeoB200StoryTables& t, uint32_t channels, uint32_t c,
                                            const float* from, float* to) {
+    if (c >= channels) return;
     for (uint32_t e = t.full; e < t.stories; ++e) {
-        const size_t row = (size_t)t.order[e] * channels;
-        for (uint32_t c = c0 + threadIdx.x; c < min(c0 + width, channels); c += kTileThreads)
-            to[row + c] = from ? from[row + c] : 0.0f;
+        const size_t at = (size_t)t.order[e] * channels + c;
+        to[at] = from ? from[at] : 0.0f;
     }
 }
 
-template <typename T, typename G, int V, bool Shared>
-__global__ void __launch_bounds__(kTileThreads, 3) scan_forward_kernel(const __grid_constant__ ScanArgs a) {
-    __shared__ TileMaps<V> maps;
-    const uint32_t ticket = take_ticket<V>(a, maps);
-    const uint32_t tile = ticket / a.groups, group = ticket % a.groups;
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
-    const uint32_t c = group * 32 * V + lane * V;
-    const bool active = c < a.channels;
-    const uint32_t first = tile * kTile + warp * kSegment;
+template <typename T, typename G, bool Pair, bool Shared, bool Backward>
+__global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_constant__ ScanArgs a) {
+    using S = Shape<T, G, Shared, Backward>;
+    constexpr int Length = S::kSegment;
+    constexpr uint32_t kTile = S::kTile, kWordsATile = kTile / 32;
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    typename S::Control& control = *reinterpret_cast<typename S::Control*>(dynamic + kStages * S::kStage);
+    const uint32_t warp = threadIdx.x >> 5;
+    const uint32_t total = a.tiles * a.groups;
 
-    typename Packed<T, V>::Raw x[kSegment];
-    typename Packed<G, V>::Raw gate[Shared ? 1 : kSegment];
-    const Segment s = segment_at(a.tables, first);
-    const T* xp = static_cast<const T*>(a.drive) + (int64_t)first * a.drive_stride + c;
-    const G* gp = static_cast<const G*>(a.decay) + (Shared ? 0 : (int64_t)first * a.decay_stride) + c;
-    float unit[V], none[V];
+    // A ticket's tile and channel group; kNone past the end.
+    const auto work_of = [&](uint32_t ticket) {
+        if (ticket >= total) return make_uint2(kNone, 0);
+        const uint32_t tile = ticket / a.groups;
+        return make_uint2(Backward ? a.tiles - 1 - tile : tile, ticket - tile * a.groups);
+    };
+    // The first tickets: one if there is a block for each, or three, drawn one
+    // after the other so that the blocks take turns: a block that held the next
+    // three in a row would keep its neighbours waiting for its third.
+    const bool one_each = gridDim.x == total;
+    if (threadIdx.x == 0) {
+        uint32_t t = a.tiles == 1 ? blockIdx.x : atomicAdd(a.scratch.ticket, 1u) + 1u;
+        control.ring[0] = work_of(t);
 #pragma unroll
-    for (int k = 0; k < V; ++k) unit[k] = 1.0f, none[k] = 0.0f;
-    if (Shared) gate[0] = active ? read_once<G, V>(gp) : Packed<G, V>::pack(unit);
-#pragma unroll
-    for (int i = 0; i < kSegment; ++i) {
-        const bool in = active && i < s.count;
-        x[i] = in ? read_once<T, V>(xp + i * a.drive_stride) : Packed<T, V>::pack(none);
-        if (!Shared) gate[i] = in ? read_once<G, V>(gp + i * a.decay_stride) : Packed<G, V>::pack(unit);
-    }
-
-    Product A[V];
-    float H[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) H[k] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kSegment; ++i) {
-        float xi[V], gi[V];
-        Packed<T, V>::unpack(x[i], xi);
-        Packed<G, V>::unpack(gate[Shared ? 0 : i], gi);
-        if (s.starts >> i & 1u) row_or_zero<V>(a.initial, story_starting(a.tables, s, i), a.channels, c, active, H);
-        const bool past = Shared && i >= s.count;  // a shared gate does not stop at the batch's end by itself
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-            H[k] = past ? H[k] : fmaf(gi[k], H[k], xi[k]);
-            if (!past) A[k].times(gi[k]);
+        for (int j = 1; j < 3; ++j) {
+            if (!one_each) t = atomicAdd(a.scratch.ticket + (t == kNone), 1u) + 1u;  // after the one before
+            control.ring[j] = work_of(one_each ? total : t);
         }
     }
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-        maps.A[warp][lane * V + k] = A[k].value();
-        maps.H[warp][lane * V + k] = H[k];
-    }
-    if (lane == 0) maps.reset[warp] = s.starts != 0;
     __syncthreads();
-    const double carry = compose_tile<V, 1>(a, maps, tile, group);
-    if (a.carries && warp < V && group * 32 * V + threadIdx.x < a.channels)
-        a.carries[(size_t)tile * a.channels + group * 32 * V + threadIdx.x] = (float)carry;
-    __syncthreads();
+    const auto work_at = [&](uint32_t i) { return control.ring[i & 7u]; };
 
-    float h[V];
+    if (warp < kWarps) {
+        // ------------------------------------------------ the threads that map and write
+        const auto stage_x = [&](uint32_t i) {
+            return reinterpret_cast<T*>(dynamic + (i % kStages) * S::kStage) + warp * Length * kColumns;
+        };
+        const auto stage_s = [&](uint32_t i) {
+            return reinterpret_cast<T*>(dynamic + (i % kStages) * S::kStage) + (kTile + warp * Length) * kColumns;
+        };
+        const auto stage_a = [&](uint32_t i) {
+            return reinterpret_cast<G*>(dynamic + (i % kStages) * S::kStage +
+                                        (size_t)(Backward ? 2 : 1) * kTile * kColumns * sizeof(T)) +
+                   warp * Length * kColumns;
+        };
+        const auto issue = [&](uint32_t i) -> uint4 {
+            uint4 word = make_uint4(0, 0, 0, 0);
+            const uint2 work = work_at(i);
+            if (work.x != kNone) {
+                const uint32_t first = work.x * kTile + warp * Length;
+                const Columns<Pair> col(work.y, a.channels);
+                const int count = first < a.tables.tokens ? (int)min(a.tables.tokens - first, (uint32_t)Length) : 0;
+                if (count) word = __ldg(reinterpret_cast<const uint4*>(a.tables.words) + (first >> 5));
+                const T* x = static_cast<const T*>(a.drive) + (int64_t)first * a.drive_stride + col.c;
+                const T* s = static_cast<const T*>(a.grad_states) + (int64_t)first * a.grad_states_stride + col.c;
+                const G* g = static_cast<const G*>(a.decay) + (int64_t)first * a.decay_stride + col.c;
+                T* to_x = stage_x(i);
+                T* to_s = stage_s(i);
+                G* to_a = stage_a(i);
 #pragma unroll
-    for (int k = 0; k < V; ++k) h[k] = maps.before[warp][lane * V + k];
-    T* out = static_cast<T*>(a.states) + (size_t)first * a.channels + c;
-#pragma unroll
-    for (int i = 0; i < kSegment; ++i) {
-        float xi[V], gi[V];
-        Packed<T, V>::unpack(x[i], xi);
-        Packed<G, V>::unpack(gate[Shared ? 0 : i], gi);
-        if (s.starts >> i & 1u) row_or_zero<V>(a.initial, story_starting(a.tables, s, i), a.channels, c, active, h);
-#pragma unroll
-        for (int k = 0; k < V; ++k) h[k] = fmaf(gi[k], h[k], xi[k]);
-        if (active && i < s.count) write_once<T, V>(out + (size_t)i * a.channels, h);
-        if (s.ends >> i & 1u) {
-            const size_t row = (size_t)story_ending(a.tables, s, i) * a.channels + c;
-#pragma unroll
-            for (int k = 0; k < V; ++k)
-                if (active) a.final_states[row + k] = h[k];
-        }
-    }
-    if (tile == 0 && a.tables.full < a.tables.stories)
-        copy_empty(a.tables, a.channels, group * 32 * V, 32 * V, a.initial, a.final_states);
-}
-
-template <typename T, typename G, int V, bool Shared>
-__global__ void __launch_bounds__(kTileThreads, 2) scan_backward_kernel(const __grid_constant__ ScanArgs a) {
-    __shared__ TileMaps<V> maps;
-    const uint32_t ticket = take_ticket<V>(a, maps);
-    const uint32_t tile = a.tiles - 1 - ticket / a.groups, group = ticket % a.groups;
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
-    const uint32_t c = group * 32 * V + lane * V;
-    const bool active = c < a.channels;
-    const uint32_t first = tile * kTile + warp * kSegment;
-
-    typename Packed<T, V>::Raw x[kSegment], g[kSegment];
-    typename Packed<G, V>::Raw gate[Shared ? 1 : kSegment];
-    const Segment s = segment_at(a.tables, first);
-    const T* xp = static_cast<const T*>(a.drive) + (int64_t)first * a.drive_stride + c;
-    const T* sp = static_cast<const T*>(a.grad_states) + (int64_t)first * a.grad_states_stride + c;
-    const G* gp = static_cast<const G*>(a.decay) + (Shared ? 0 : (int64_t)first * a.decay_stride) + c;
-    float unit[V], none[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) unit[k] = 1.0f, none[k] = 0.0f;
-    if (Shared) gate[0] = active ? read_once<G, V>(gp) : Packed<G, V>::pack(unit);
-#pragma unroll
-    for (int i = 0; i < kSegment; ++i) {
-        const bool in = active && i < s.count;
-        x[i] = in ? read_once<T, V>(xp + i * a.drive_stride) : Packed<T, V>::pack(none);
-        if (!Shared) gate[i] = in ? read_once<G, V>(gp + i * a.decay_stride) : Packed<G, V>::pack(unit);
-        g[i] = in ? read_once<T, V>(sp + i * a.grad_states_stride) : Packed<T, V>::pack(none);
-    }
-
-    // The segment's map from the left.
-    Product A[V];
-    float H[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) H[k] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kSegment; ++i) {
-        float xi[V], gi[V];
-        Packed<T, V>::unpack(x[i], xi);
-        Packed<G, V>::unpack(gate[Shared ? 0 : i], gi);
-        if (s.starts >> i & 1u) row_or_zero<V>(a.initial, story_starting(a.tables, s, i), a.channels, c, active, H);
-        const bool past = Shared && i >= s.count;
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-            H[k] = past ? H[k] : fmaf(gi[k], H[k], xi[k]);
-            if (!past) A[k].times(gi[k]);
-        }
-    }
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-        maps.A[warp][lane * V + k] = A[k].value();
-        maps.H[warp][lane * V + k] = H[k];
-    }
-    if (lane == 0) maps.reset[warp] = s.starts != 0;
-    __syncthreads();
-
-    // The state before each token: from the tile's carry through the segments before this one.
-    float h[kSegment][V];
-    {
-        float before[V];
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-            double b = active && s.count > 0 ? (double)__ldcs(a.carries + (size_t)tile * a.channels + c + k) : 0.0;
-            for (uint32_t w = 0; w < warp; ++w)
-                b = maps.reset[w] ? (double)maps.H[w][lane * V + k]
-                                  : fma(maps.A[w][lane * V + k], b, (double)maps.H[w][lane * V + k]);
-            before[k] = (float)b;
-        }
-#pragma unroll
-        for (int i = 0; i < kSegment; ++i) {
-            float xi[V], gi[V];
-            Packed<T, V>::unpack(x[i], xi);
-            Packed<G, V>::unpack(gate[Shared ? 0 : i], gi);
-            if (s.starts >> i & 1u)
-                row_or_zero<V>(a.initial, story_starting(a.tables, s, i), a.channels, c, active, before);
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                h[i][k] = before[k];
-                before[k] = fmaf(gi[k], before[k], xi[k]);
+                for (int j = 0; j < Length; ++j)
+                    if (j < count) {
+                        col.copy(to_x + j * kColumns, x + j * a.drive_stride);
+                        if constexpr (Backward) col.copy(to_s + j * kColumns, s + j * a.grad_states_stride);
+                        if constexpr (!Shared) col.copy(to_a + j * kColumns, g + j * a.decay_stride);
+                    }
             }
-        }
-    }
-    __syncthreads();
-
-    // The segment's map from the right: m[t] = a[t] (g[t] + m[t + 1]).
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            return word;
+        };
+        const auto map = [&](uint32_t i, uint4 word) {
+            const uint2 work = work_at(i);
+            const Columns<Pair> col(work.y, a.channels);
+            const Segment s = segment_of<Length>(a.tables, word, work.x * kTile + warp * Length);
+            const T* x = stage_x(i);
+            const T* sp = stage_s(i);
+            const G* ap = stage_a(i);
+            Product2 A;
+            Pair32 H = 0, M = 0, gate = 0;
+            if constexpr (Shared) gate = col.get_shared(static_cast<const G*>(a.decay));
+            const auto forward = [&](int j) {
+                if constexpr (!Shared) gate = col.get(ap + j * kColumns);
+                H = fma2(gate, H, col.get(x + j * kColumns));
+                A.times(gate);
+            };
+            const auto backward = [&](int j) {
+                if constexpr (!Shared) gate = col.get(ap + j * kColumns);
+                M = mul2(gate, add2(col.get(sp + j * kColumns), M));
+            };
+            if (s.count == Length && (s.starts | s.ends) == 0) {
 #pragma unroll
-    for (int k = 0; k < V; ++k) H[k] = 0.0f;
+                for (int j = 0; j < Length; ++j) forward(j);
+                if constexpr (Backward) {
 #pragma unroll
-    for (int i = kSegment - 1; i >= 0; --i) {
-        float si[V], gi[V];
-        Packed<T, V>::unpack(g[i], si);
-        Packed<G, V>::unpack(gate[Shared ? 0 : i], gi);
-        if (s.ends >> i & 1u) row_or_zero<V>(a.grad_final, story_ending(a.tables, s, i), a.channels, c, active, H);
-        const bool past = Shared && i >= s.count;
-#pragma unroll
-        for (int k = 0; k < V; ++k) H[k] = past ? H[k] : gi[k] * (si[k] + H[k]);
-    }
-#pragma unroll
-    for (int k = 0; k < V; ++k) maps.H[warp][lane * V + k] = H[k];
-    if (lane == 0) maps.reset[warp] = s.ends != 0;
-    __syncthreads();
-    compose_tile<V, -1>(a, maps, tile, group);
-    __syncthreads();
-
-    float m[V], sum[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) m[k] = maps.before[warp][lane * V + k], sum[k] = 0.0f;
-    T* out = static_cast<T*>(a.grad_drive) + (size_t)first * a.channels + c;
-    G* out_gate = static_cast<G*>(a.grad_decay) + (size_t)first * a.channels + c;
-#pragma unroll
-    for (int i = kSegment - 1; i >= 0; --i) {
-        float si[V], gi[V], term[V];
-        Packed<T, V>::unpack(g[i], si);
-        Packed<G, V>::unpack(gate[Shared ? 0 : i], gi);
-        if (s.ends >> i & 1u) row_or_zero<V>(a.grad_final, story_ending(a.tables, s, i), a.channels, c, active, m);
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-            si[k] += m[k];
-            term[k] = si[k] * h[i][k];
-            m[k] = gi[k] * si[k];
-        }
-        if (i < s.count) {
-            if (active) write_once<T, V>(out + (size_t)i * a.channels, si);
-            if (!Shared) {
-                if (active) write_once<G, V>(out_gate + (size_t)i * a.channels, term);
+                    for (int j = Length - 1; j >= 0; --j) backward(j);
+                }
             } else {
-#pragma unroll
-                for (int k = 0; k < V; ++k) sum[k] += term[k];
+#pragma unroll 1
+                for (int j = 0; j < s.count; ++j) {
+                    if (s.starts >> j & 1u) H = col.get_row(a.initial, story_starting(a.tables, s, j), a.channels);
+                    forward(j);
+                }
+                if constexpr (Backward) {
+#pragma unroll 1
+                    for (int j = s.count - 1; j >= 0; --j) {
+                        if (s.ends >> j & 1u) M = col.get_row(a.grad_final, story_ending(a.tables, s, j), a.channels);
+                        backward(j);
+                    }
+                }
             }
+            typename S::Maps& m = control.maps[i & 1u];
+            const float2 hi = parts(A.hi), lo = parts(A.lo), h = parts(H), r = parts(M);
+            m.A[warp][col.at[0]] = make_float2(hi.x, lo.x);
+            m.A[warp][col.at[1]] = make_float2(hi.y, lo.y);
+            m.H[warp][col.at[0]] = h.x, m.H[warp][col.at[1]] = h.y;
+            if constexpr (Backward) m.M[warp][col.at[0]] = r.x, m.M[warp][col.at[1]] = r.y;
+            if ((threadIdx.x & 31u) == 0) m.starts[warp] = s.starts != 0, m.ends[warp] = s.ends != 0;
+            arrive_at<1>(i & 1u);
+        };
+        const auto write = [&](uint32_t i, uint4 word) {
+            const uint2 work = work_at(i);
+            const Columns<Pair> col(work.y, a.channels);
+            const uint32_t first = work.x * kTile + warp * Length;
+            const Segment s = segment_of<Length>(a.tables, word, first);
+            const T* x = stage_x(i);
+            const T* sp = stage_s(i);
+            const G* ap = stage_a(i);
+            const typename S::Maps& m = control.maps[i & 1u];
+            Pair32 h = pair_of(m.H[warp][col.at[0]], m.H[warp][col.at[1]]), gate = 0;
+            if constexpr (Shared) gate = col.get_shared(static_cast<const G*>(a.decay));
+            const size_t row = (size_t)first * a.channels + col.c;
+            const bool plain = s.count == Length && (s.starts | s.ends) == 0;
+            if constexpr (!Backward) {
+                T* out = static_cast<T*>(a.states) + row;
+                const auto step = [&](int j) {
+                    if constexpr (!Shared) gate = col.get(ap + j * kColumns);
+                    h = fma2(gate, h, col.get(x + j * kColumns));
+                    col.put(out, h);
+                    out += a.channels;
+                };
+                if (plain) {
+#pragma unroll
+                    for (int j = 0; j < Length; ++j) step(j);
+                } else {
+#pragma unroll 1
+                    for (int j = 0; j < s.count; ++j) {
+                        if (s.starts >> j & 1u) h = col.get_row(a.initial, story_starting(a.tables, s, j), a.channels);
+                        step(j);
+                        if (s.ends >> j & 1u) col.put_row(a.final_states, story_ending(a.tables, s, j), a.channels, h);
+                    }
+                }
+            } else {
+                // The state before each token, then the slopes from the right.
+                Pair32 previous[Length];
+#pragma unroll
+                for (int j = 0; j < Length; ++j) {
+                    if (!plain && (s.starts >> j & 1u))
+                        h = col.get_row(a.initial, story_starting(a.tables, s, j), a.channels);
+                    if constexpr (!Shared) gate = col.get(ap + j * kColumns);
+                    previous[j] = h;
+                    h = fma2(gate, h, col.get(x + j * kColumns));
+                }
+                Pair32 n = pair_of(m.M[warp][col.at[0]], m.M[warp][col.at[1]]), sum = 0;
+                T* out = static_cast<T*>(a.grad_drive) + row + (size_t)(Length - 1) * a.channels;
+                G* out_gate = static_cast<G*>(a.grad_decay) + (Shared ? 0 : row + (size_t)(Length - 1) * a.channels);
+#pragma unroll
+                for (int j = Length - 1; j >= 0; --j) {
+                    if (plain || j < s.count) {
+                        if (!plain && (s.ends >> j & 1u))
+                            n = col.get_row(a.grad_final, story_ending(a.tables, s, j), a.channels);
+                        if constexpr (!Shared) gate = col.get(ap + j * kColumns);
+                        const Pair32 slope = add2(col.get(sp + j * kColumns), n);
+                        const Pair32 term = mul2(slope, previous[j]);
+                        n = mul2(gate, slope);
+                        col.put(out, slope);
+                        if constexpr (Shared)
+                            sum = add2(sum, term);
+                        else
+                            col.put(out_gate, term);
+                        if (!plain && a.grad_initial && (s.starts >> j & 1u))
+                            col.put_row(a.grad_initial, story_starting(a.tables, s, j), a.channels, n);
+                    }
+                    out -= a.channels;
+                    if constexpr (!Shared) out_gate -= a.channels;
+                }
+                if constexpr (Shared) {
+                    const float2 f = parts(sum);
+                    control.sums[i & 1u][warp][col.at[0]] = f.x, control.sums[i & 1u][warp][col.at[1]] = f.y;
+                }
+            }
+        };
+
+        uint4 word0 = issue(0), word1 = issue(1);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        if (work_at(0).x != kNone) map(0, word0);
+        for (uint32_t i = 0; work_at(i).x != kNone; ++i) {
+            const uint4 word2 = issue(i + 2);
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            if (work_at(i + 1).x != kNone) map(i + 1, word1);
+            sync_of<3>(i & 1u);
+            write(i, word0);
+            word0 = word1;
+            word1 = word2;
         }
-        if (a.grad_initial && (s.starts >> i & 1u)) {
-            const size_t row = (size_t)story_starting(a.tables, s, i) * a.channels + c;
+        if constexpr (Backward && Shared) arrive_at<1>(0);  // the last sums are written
+    } else {
+        // ------------------------------------------------ the warps that compose
+        // A lane takes half the segments of a channel, the nearer ones in the
+        // direction of the scan first, and half the slots; its partner is 16 lanes away.
+        constexpr int Direction = Backward ? -1 : 1;
+        constexpr int kHalf = kWarps / 2;
+        const uint32_t lane = threadIdx.x & 31u, half = lane >> 4, k = (warp - kWarps) * 16 + (lane & 15u);
+        const bool leader = threadIdx.x == 32 * kWarps;
+        const auto add_sums = [&](uint32_t i, uint2 work) {
+            const uint32_t c = work.y * kColumns + k;
+            float sum = 0.0f;
 #pragma unroll
-            for (int k = 0; k < V; ++k)
-                if (active) a.grad_initial[row + k] = m[k];
-        }
-    }
-    if (Shared) {
-        // The tile's sum, its segments in order.
-#pragma unroll
-        for (int k = 0; k < V; ++k) maps.H[warp][lane * V + k] = sum[k];
-        __syncthreads();
-        if (warp < V && group * 32 * V + threadIdx.x < a.channels) {
-            float total = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kTileWarps; ++w) total += maps.H[w][threadIdx.x];
+            for (int w = 0; w < kWarps; ++w) sum += control.sums[i & 1u][w][k];
+            if (c >= a.channels || half) return;
             if (a.tiles == 1)
-                store(static_cast<G*>(a.grad_decay) + group * 32 * V + threadIdx.x, total);
+                store(static_cast<G*>(a.grad_decay) + c, sum);
             else
-                a.scratch.partials[(size_t)tile * a.channels + group * 32 * V + threadIdx.x] = total;
+                a.scratch.partials[(size_t)work.x * a.channels + c] = sum;
+        };
+        (void)add_sums;
+        uint32_t i = 0;
+        uint2 before1 = make_uint2(kNone, 0), before2 = before1;  // the last two tiles
+        uint32_t end = Lookback<Direction>::end_of(a, work_at(0).x, kWordsATile);
+        for (;; ++i) {
+            const uint2 work = work_at(i);
+            const uint32_t tile = work.x, c = work.y * kColumns + k;
+            if (tile == kNone) break;
+            // For later turns: a ticket, whose loads are issued in the next one, and the next tile's table entry.
+            uint32_t later = total;
+            if (leader && !one_each) later = atomicAdd(a.scratch.ticket, 1u) + 1u;
+            const uint32_t next_end = Lookback<Direction>::end_of(a, work_at(i + 1).x, kWordsATile);
+            const bool active = c < a.channels;
+            float kept = 0.0f;
+            if (Backward && active && a.tables.tokens > 0)
+                kept = __ldcs(a.carries + (size_t)tile * (kTile / kKept) * a.channels + c);
+            const Lookback<Direction> back(a, tile, end, kWordsATile);
+            end = next_end;
+            if (leader) control.ring[(i + 3) & 7u] = work_of(later);
+            sync_of<1>(i & 1u);
+            typename S::Maps& m = control.maps[i & 1u];
+            if constexpr (Backward && Shared)
+                if (before2.x != kNone) add_sums(i, before2);
+
+            // The map of this half of the tile, then of the tile, in the direction of the scan.
+            const uint2 cut_bytes =
+                reinterpret_cast<const uint2*>(Backward ? m.ends : m.starts)[Backward ? 1 - half : half];
+            const auto segment = [&](int j) { return (Backward ? kWarps - 1 - j : j) + (Backward ? -1 : 1) * (int)half * kHalf; };
+            const auto cut_at = [&](int j) {  // of this half
+                const int byte = Backward ? kHalf - 1 - j : j;
+                return ((byte < 4 ? cut_bytes.x : cut_bytes.y) >> (byte & 3) * 8 & 1u) != 0;
+            };
+            float2 product = make_float2(1.0f, 0.0f);
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < kHalf; ++j) {
+                const int w = segment(j);
+                const float2 A = m.A[w][k];
+                const float v = Backward ? m.M[Backward ? w : 0][k] : m.H[w][k];
+                sum = cut_at(j) ? v : fmaf(value_of(A), sum, v);
+                product = product_of(product, A);
+            }
+            const bool cut = (cut_bytes.x | cut_bytes.y) != 0;
+            const bool other_cut = __shfl_xor_sync(kNone, cut, 16);
+            const float other_sum = __shfl_xor_sync(kNone, sum, 16);
+            const float2 other = make_float2(__shfl_xor_sync(kNone, product.x, 16), __shfl_xor_sync(kNone, product.y, 16));
+            const bool cuts = cut || other_cut;
+            // of the near and the far half
+            const float near_A = value_of(half ? other : product), near_sum = half ? other_sum : sum;
+            const bool near_cut = half ? other_cut : cut, far_cut = half ? cut : other_cut;
+            const float far_A = value_of(half ? product : other), far_sum = half ? sum : other_sum;
+            const float tile_A = value_of(product_of(product, other));
+            const float tile_sum = far_cut ? far_sum : fmaf(far_A, near_sum, far_sum);
+            const bool last = Backward ? tile == 0 : tile + 1 == a.tiles;
+            const bool state_tile = Backward ? tile % kGroup == 0 : (tile + 1) % kGroup == 0;
+            const bool writes = active && !last && half == 0;
+            Slot* mine = a.scratch.slots + (size_t)tile * a.channels + c;
+            if (writes && (cuts || !state_tile)) write_slot(mine, tile_A, tile_sum);
+
+            float carry = 0.0f;
+            if (back.maps >= 0) {
+                float A, H;
+                for (uint32_t n = 0;; ++n) {
+                    const bool there = !active || back.read(a.scratch.slots, a.channels, c, (int)half, A, H);
+                    if (__all_sync(kNone, there)) break;
+                    if (n >= kSpinLimit) {
+                        if (lane == 0) atomicExch(&g_gave_up, 1u);
+                        A = H = CUDART_NAN_F;
+                        break;
+                    }
+                }
+                const float other_A = __shfl_xor_sync(kNone, A, 16), other_H = __shfl_xor_sync(kNone, H, 16);
+                // the far half's map of the near half's state; one slot is the state itself
+                if (back.maps < 8)
+                    carry = half ? other_H : H;
+                else
+                    carry = half ? fmaf(A, other_H, H) : fmaf(other_A, H, other_H);
+            }
+            if (writes && !cuts && state_tile) write_slot(mine, 0.0f, fmaf(tile_A, carry, tile_sum));
+
+            // The value before each segment, in place of its map.
+            float before = half ? (near_cut ? near_sum : fmaf(near_A, carry, near_sum)) : carry;
+            float A[kHalf], v[kHalf];
+#pragma unroll
+            for (int j = 0; j < kHalf; ++j) {
+                const int w = segment(j);
+                A[j] = value_of(m.A[w][k]);
+                v[j] = Backward ? m.M[Backward ? w : 0][k] : m.H[w][k];
+            }
+#pragma unroll
+            for (int j = 0; j < kHalf; ++j) {
+                const int w = segment(j);
+                if constexpr (Backward) {
+                    m.M[w][k] = before;
+                } else {
+                    m.H[w][k] = before;
+                    if (a.carries && active && w % (kKept / Length) == 0 &&
+                        tile * kTile + (uint32_t)w * Length < a.tables.tokens)
+                        a.carries[((size_t)tile * (kTile / kKept) + w / (kKept / Length)) * a.channels + c] = before;
+                }
+                before = cut_at(j) ? v[j] : fmaf(A[j], before, v[j]);
+            }
+            if constexpr (Backward) {
+                // The state before each segment: this lane's half from the right is the other one from the left.
+                const uint2 starts = reinterpret_cast<const uint2*>(m.starts)[1 - half];
+                float h[kHalf];
+                float2 P = make_float2(1.0f, 0.0f);
+                float state = 0.0f;
+#pragma unroll
+                for (int j = 0; j < kHalf; ++j) h[j] = m.H[segment(kHalf - 1 - j)][k];
+                const auto start_at = [&](int j) { return ((j < 4 ? starts.x : starts.y) >> (j & 3) * 8 & 1u) != 0; };
+#pragma unroll
+                for (int j = 0; j < kHalf; ++j) {
+                    state = start_at(j) ? h[j] : fmaf(A[kHalf - 1 - j], state, h[j]);
+                    P.x *= A[kHalf - 1 - j];
+                }
+                // Lanes of half 1 hold the segments on the left, and pass the state after them on.
+                const bool left_cut = (starts.x | starts.y) != 0;
+                const float after = half ? (left_cut ? state : fmaf(P.x, kept, state)) : 0.0f;
+                const float from_left = __shfl_xor_sync(kNone, after, 16);
+                float at = half ? kept : from_left;
+#pragma unroll
+                for (int j = 0; j < kHalf; ++j) {
+                    m.H[segment(kHalf - 1 - j)][k] = at;
+                    at = start_at(j) ? h[j] : fmaf(A[kHalf - 1 - j], at, h[j]);
+                }
+            }
+            arrive_at<3>(i & 1u);
+            if (tile == 0 && a.tables.full < a.tables.stories && half == 0) {
+                if constexpr (!Backward)
+                    copy_empty(a.tables, a.channels, c, a.initial, a.final_states);
+                else if (a.grad_initial)
+                    copy_empty(a.tables, a.channels, c, a.grad_final, a.grad_initial);
+            }
+            before2 = before1;
+            before1 = work;
+        }
+        if constexpr (Backward && Shared) {
+            sync_of<1>(0);
+            if (before2.x != kNone) add_sums(i, before2);
+            if (before1.x != kNone) add_sums(i + 1, before1);
         }
     }
-    if (tile == 0 && a.grad_initial && a.tables.full < a.tables.stories)
-        copy_empty(a.tables, a.channels, group * 32 * V, 32 * V, a.grad_final, a.grad_initial);
 }
 
 // The gradient of a shared row of gates: the tiles' sums in double, a column of
@@ -639,22 +828,18 @@ void check_tables(const LeoB200StoryTables* t, uint32_t channels) {
     require(channels > 0 && channels < (1u << 31), "channels must be positive");
 }
 
-uint32_t tiles_of(uint32_t tokens) { return tokens == 0 ? 1 : (tokens - 1) / kTile + 1; }
+uint32_t tiles_of(uint32_t tokens, uint32_t length) { return tokens == 0 ? 1 : (tokens - 1) / length + 1; }
 
-// The parts of a call's scratch; returns its size.
+// The parts of a call's scratch, for the shortest tiles; returns its size.
 size_t lay_out(uint32_t tokens, uint32_t channels, void* base, Scratch* s) {
-    const size_t tiles = tiles_of(tokens);
+    const size_t tiles = tiles_of(tokens, kKept);
     if (tiles == 1) return 0;  // nothing crosses tiles
-    const size_t flag_row = ((size_t)channels + 63) / 64 * 2;
-    const size_t flags = 256, slots = (flags + tiles * flag_row * sizeof(uint32_t) + 255) / 256 * 256;
-    const size_t partials = slots + tiles * channels * sizeof(double2);
+    const size_t slots = 256, partials = slots + tiles * channels * sizeof(Slot);
     if (s) {
         char* p = static_cast<char*>(base);
         s->ticket = reinterpret_cast<uint32_t*>(p);
-        s->flags = reinterpret_cast<uint32_t*>(p + flags);
-        s->slots = reinterpret_cast<double2*>(p + slots);
+        s->slots = reinterpret_cast<Slot*>(p + slots);
         s->partials = reinterpret_cast<float*>(p + partials);
-        s->flag_row = (uint32_t)flag_row;
     }
     return partials + tiles * channels * sizeof(float);
 }
@@ -664,30 +849,40 @@ bool in_pairs(const void* p, int64_t stride, size_t size) {
     return reinterpret_cast<uintptr_t>(p) % (2 * size) == 0 && stride % 2 == 0;
 }
 
-// Fills the tiling of `a`, clears the scratch on `stream`; the number of blocks.
-uint32_t begin_scan(ScanArgs& a, int V, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
-    a.tiles = tiles_of(a.tables.tokens);
-    a.groups = (a.channels + 32 * V - 1) / (32 * V);
-    require((uint64_t)a.tiles * a.groups < (1ull << 31), "too many tokens and channels for one scan");
+// Launches one scan on `stream`: one block an SM, or one a tile if there are few.
+template <typename T, typename G, bool Pair, bool Shared, bool Backward>
+void launch_scan(ScanArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+    using S = Shape<T, G, Shared, Backward>;
+    static_assert(S::kBytes <= kSharedLimit && S::kTile % kKept == 0 && kKept % S::kSegment == 0, "shape");
+    static_assert(LEO_B200_STORY_WORD_TOKENS % S::kSegment == 0, "a segment lies in one story word");
+    a.tiles = tiles_of(a.tables.tokens, S::kTile);
+    a.groups = (a.channels + kColumns - 1) / kColumns;
+    const uint64_t total = (uint64_t)a.tiles * a.groups;
+    require(total < (1ull << 31) - 65536, "too many tokens and channels for one scan");
     const size_t size = lay_out(a.tables.tokens, a.channels, workspace, &a.scratch);
     if (size > 0) {
         require(workspace != nullptr && workspace_bytes >= size, "the workspace is too small");
         require(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "the workspace must be aligned to 16 bytes");
-        check(cudaMemsetAsync(workspace, 0, 256 + (size_t)a.tiles * a.scratch.flag_row * sizeof(uint32_t), stream),
-              "clear scan flags");
     }
-    return a.tiles * a.groups;
+    int device = 0, sms = 0;
+    check(cudaGetDevice(&device), "cudaGetDevice");
+    check(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device), "SM count");
+    const auto kernel = scan_kernel<T, G, Pair, Shared, Backward>;
+    check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kBytes), "shared memory");
+    if (a.tiles > 1)
+        check(cudaMemsetAsync(workspace, 0xff, 256 + (size_t)a.tiles * a.channels * sizeof(Slot), stream), "clear scan slots");
+    const uint32_t blocks = a.tiles == 1 || total <= 2u * (uint32_t)sms ? (uint32_t)total : (uint32_t)sms;
+    kernel<<<blocks, kTileThreads, S::kBytes, stream>>>(a);
+    check(cudaGetLastError(), "scan_kernel");
 }
 
-// Calls body(V, Shared) as types.
+// Calls body(Pair, Shared) as types.
 template <typename Body>
 void dispatch_shape(bool pairs, bool shared, Body&& body) {
-    using One = std::integral_constant<int, 1>;
-    using Two = std::integral_constant<int, 2>;
-    if (pairs && shared) body(Two{}, std::true_type{});
-    else if (pairs) body(Two{}, std::false_type{});
-    else if (shared) body(One{}, std::true_type{});
-    else body(One{}, std::false_type{});
+    if (pairs && shared) body(std::true_type{}, std::true_type{});
+    else if (pairs) body(std::true_type{}, std::false_type{});
+    else if (shared) body(std::false_type{}, std::true_type{});
+    else body(std::false_type{}, std::false_type{});
 }
 
 }  // namespace
@@ -733,7 +928,7 @@ size_t leo_b200_gated_scan_workspace(uint32_t tokens, uint32_t channels) {
 }
 
 size_t leo_b200_gated_scan_carry_count(uint32_t tokens, uint32_t channels) {
-    return (size_t)tiles_of(tokens) * channels;
+    return (size_t)tiles_of(tokens, kKept) * channels;
 }
 
 int leo_b200_gated_scan(int device, const LeoB200StoryTables* tables, uint32_t channels, int dtype,
@@ -762,10 +957,8 @@ int leo_b200_gated_scan(int device, const LeoB200StoryTables* tables, uint32_t c
                                in_pairs(decay, decay_shared ? 0 : decay_stride, sizeof(G)) &&
                                in_pairs(states, 0, sizeof(T));
             DeviceScope scope(device);
-            dispatch_shape(pairs, decay_shared != 0 && tables->tokens > 0, [&](auto v, auto shared) {
-                const uint32_t blocks = begin_scan(a, v(), workspace, workspace_bytes, (cudaStream_t)stream);
-                scan_forward_kernel<T, G, v(), shared()><<<blocks, kTileThreads, 0, (cudaStream_t)stream>>>(a);
-                check(cudaGetLastError(), "scan_forward_kernel");
+            dispatch_shape(pairs, decay_shared != 0 && tables->tokens > 0, [&](auto pair, auto shared) {
+                launch_scan<T, G, pair(), shared(), false>(a, workspace, workspace_bytes, (cudaStream_t)stream);
             });
         });
     });
@@ -781,7 +974,7 @@ int leo_b200_gated_scan_backward(int device, const LeoB200StoryTables* tables, u
         check_tables(tables, channels);
         require(tables->tokens == 0 || (grad_states && drive && decay && carries && grad_drive),
                 "scan arrays are null");
-        require(grad_decay != nullptr || (tables->tokens == 0 && !decay_shared), "scan arrays are null");
+        require((decay && grad_decay) || (tables->tokens == 0 && !decay_shared), "scan arrays are null");
         ScanArgs a{};
         a.tables = *tables;
         a.channels = channels;
@@ -805,10 +998,8 @@ int leo_b200_gated_scan_backward(int device, const LeoB200StoryTables* tables, u
                                in_pairs(grad_states, grad_states_stride, sizeof(T)) &&
                                in_pairs(grad_drive, 0, sizeof(T)) && in_pairs(grad_decay, 0, sizeof(G));
             DeviceScope scope(device);
-            dispatch_shape(pairs, decay_shared != 0, [&](auto v, auto shared) {
-                const uint32_t blocks = begin_scan(a, v(), workspace, workspace_bytes, (cudaStream_t)stream);
-                scan_backward_kernel<T, G, v(), shared()><<<blocks, kTileThreads, 0, (cudaStream_t)stream>>>(a);
-                check(cudaGetLastError(), "scan_backward_kernel");
+            dispatch_shape(pairs, decay_shared != 0, [&](auto pair, auto shared) {
+                launch_scan<T, G, pair(), shared(), true>(a, workspace, workspace_bytes, (cudaStream_t)stream);
                 if (decay_shared && a.tiles > 1) {
                     shared_decay_kernel<G><<<(channels + 31) / 32, kThreads, 0, (cudaStream_t)stream>>>(
                         a.scratch.partials, a.tiles, channels, static_cast<G*>(grad_decay));
