@@ -27,6 +27,7 @@
 // word, written and read as one, so a slot that is there costs one trip to L2.
 // Which slots are read, and in which order they are composed, depends on the
 // layout alone: results are the same in every run.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -52,8 +53,9 @@ __device__ __forceinline__ void store(__half* p, float v) { *p = __float2half_rn
 
 constexpr uint32_t kThreads = 128;  // of the step and the reduction
 
-constexpr int kWarps = 16;                       // that map and write a tile
-constexpr int kColumns = 64;                     // channels of a tile
+constexpr int kWarps = 8;                        // that map and write a tile
+constexpr int kSegments = 2 * kWarps;            // of a tile, half a warp each
+constexpr int kColumns = 64;                     // channels of a tile, four a thread
 constexpr int kCarryWarps = kColumns / 16;       // that compose it, two lanes a channel
 constexpr uint32_t kTileThreads = 32 * (kWarps + kCarryWarps);
 constexpr int kStages = 3;
@@ -93,34 +95,44 @@ __device__ __forceinline__ Pair32 add2(Pair32 a, Pair32 b) {
     return r;
 }
 
-// Two neighbours of a row as they lie in memory.
-template <typename T> struct Packed;
-template <> struct Packed<float> {
-    using Raw = Pair32;
-    static __device__ __forceinline__ Pair32 unpack(Raw r) { return r; }
-    static __device__ __forceinline__ Raw pack(Pair32 v) { return v; }
+// A thread's four channels.
+struct Quad {
+    Pair32 v[2] = {0, 0};
 };
-template <> struct Packed<__nv_bfloat16> {
-    using Raw = unsigned int;
-    static __device__ __forceinline__ Pair32 unpack(Raw r) {
-        return pair_of(__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u));
+
+// N neighbours of a row as they lie in memory, and pairs of them as floats.
+template <typename T, int N> struct Packed {
+    using Raw = std::conditional_t<N * sizeof(T) == 16, uint4, std::conditional_t<N * sizeof(T) == 8, uint2, uint32_t>>;
+};
+template <typename T> struct PairOf;
+template <> struct PairOf<float> {
+    static __device__ __forceinline__ Pair32 unpack(const uint32_t* r) {
+        return pair_of(__uint_as_float(r[0]), __uint_as_float(r[1]));
     }
-    static __device__ __forceinline__ Raw pack(Pair32 v) {
+    static __device__ __forceinline__ void pack(Pair32 v, uint32_t* r) {
+        const float2 f = parts(v);
+        r[0] = __float_as_uint(f.x), r[1] = __float_as_uint(f.y);
+    }
+};
+template <> struct PairOf<__nv_bfloat16> {
+    static __device__ __forceinline__ Pair32 unpack(const uint32_t* r) {
+        return pair_of(__uint_as_float(r[0] << 16), __uint_as_float(r[0] & 0xffff0000u));
+    }
+    static __device__ __forceinline__ void pack(Pair32 v, uint32_t* r) {
         const float2 f = parts(v);
         const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
-        return *reinterpret_cast<const Raw*>(&h);
+        r[0] = *reinterpret_cast<const uint32_t*>(&h);
     }
 };
-template <> struct Packed<__half> {
-    using Raw = unsigned int;
-    static __device__ __forceinline__ Pair32 unpack(Raw r) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r));
+template <> struct PairOf<__half> {
+    static __device__ __forceinline__ Pair32 unpack(const uint32_t* r) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(r));
         return pair_of(f.x, f.y);
     }
-    static __device__ __forceinline__ Raw pack(Pair32 v) {
+    static __device__ __forceinline__ void pack(Pair32 v, uint32_t* r) {
         const float2 f = parts(v);
         const __half2 h = __floats2half2_rn(f.x, f.y);
-        return *reinterpret_cast<const Raw*>(&h);
+        r[0] = *reinterpret_cast<const uint32_t*>(&h);
     }
 };
 
@@ -149,6 +161,7 @@ struct Scratch {
 };
 
 struct ScanArgs {
+    CUtensorMap drive_map, decay_map, grad_map;  // of the tiled loads
     LeoB200StoryTables tables;
     uint32_t channels, tiles, groups;  // groups: of 64 channels
     const void* drive;
@@ -202,12 +215,15 @@ __device__ __forceinline__ uint32_t story_ending(const LeoB200StoryTables& t, co
 // (p = hi a, e = hi a - p exactly), so that the map of a long span of slow
 // gates is exact to float32 where a plain product would drift by a rounding a
 // token, the same one in every span if the gates are constant.
-struct Product2 {  // of two channels
-    Pair32 hi = pair_of(1.0f, 1.0f), lo = 0;
-    __device__ __forceinline__ void times(Pair32 a) {
-        const Pair32 p = mul2(hi, a);
-        lo = fma2(lo, a, fma2(hi, a, p ^ 0x8000000080000000ull));
-        hi = p;
+struct Product4 {  // of four channels
+    Pair32 hi[2] = {0x3f8000003f800000ull, 0x3f8000003f800000ull}, lo[2] = {0, 0};
+    __device__ __forceinline__ void times(const Quad& a) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const Pair32 p = mul2(hi[q], a.v[q]);
+            lo[q] = fma2(lo[q], a.v[q], fma2(hi[q], a.v[q], p ^ 0x8000000080000000ull));
+            hi[q] = p;
+        }
     }
 };
 __device__ __forceinline__ float2 product_of(float2 x, float2 y) {  // (hi, lo)
@@ -283,20 +299,21 @@ struct Shape {
     // A token of a tile takes this much of a stage.
     static constexpr int kRow = kColumns * (int)((Backward ? 2 : 1) * sizeof(T) + (Shared ? 0 : sizeof(G)));
     struct Maps {
-        float2 A[kWarps][kColumns];                // hi, lo
-        float H[kWarps][kColumns];                 // then the state before each segment
-        float M[Backward ? kWarps : 1][kColumns];  // then the value before each segment from the right
-        uint8_t starts[kWarps], ends[kWarps];      // whether a story does in the segment
+        float2 A[kSegments][kColumns];                // hi, lo
+        float H[kSegments][kColumns];                 // then the state before each segment
+        float M[Backward ? kSegments : 1][kColumns];  // then the value before each segment from the right
+        uint8_t starts[kSegments], ends[kSegments];   // whether a story does in the segment
     };
     struct Control {
         Maps maps[2];
-        float sums[Backward && Shared ? 2 : 1][Backward && Shared ? kWarps : 1][kColumns];
+        float sums[Backward && Shared ? 2 : 1][Backward && Shared ? kSegments : 1][kColumns];
         uint2 ring[8];  // the block's (tile, group)s; an entry is rewritten when no warp reads it any more
+        uint64_t landed[kStages][kWarps];  // barriers of the tiled loads
     };
     // 8 tokens a thread, or 4 where three stages of them would not fit.
-    static constexpr size_t kStageOf8 = (size_t)8 * kWarps * kRow;
+    static constexpr size_t kStageOf8 = (size_t)8 * kSegments * kRow;
     static constexpr int kSegment = kStages * kStageOf8 + sizeof(Control) <= kSharedLimit ? 8 : 4;
-    static constexpr uint32_t kTile = kSegment * kWarps;
+    static constexpr uint32_t kTile = kSegment * kSegments;
     static constexpr size_t kStage = (size_t)kTile * kRow;
     static constexpr size_t kBytes = kStages * kStage + sizeof(Control);
 };
@@ -325,68 +342,147 @@ __device__ __forceinline__ void copy_async(void* shared, const void* global) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(global), "n"(Bytes) : "memory");
 }
 
-// A thread's two channels of a row: a pair of neighbours, or, where the rows do
-// not allow that, two that lie 32 apart.
-template <bool Pair>
-struct Columns {
-    uint32_t at[2];  // in the tile
-    bool in[2];      // below the batch's channels
-    uint32_t c;      // the first channel
-    __device__ __forceinline__ Columns(uint32_t group, uint32_t channels) {
-        const uint32_t lane = threadIdx.x & 31u;
-        at[0] = Pair ? 2 * lane : lane;
-        at[1] = Pair ? at[0] + 1 : at[0] + 32;
-        c = group * kColumns + at[0];
-        in[0] = c < channels;
-        in[1] = c + (at[1] - at[0]) < channels;
+// Tiled loads of a warp's tokens, counted in bytes at a barrier of the warp.
+__device__ __forceinline__ void expect_bytes(uint64_t* barrier, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared.b64 _, [%0], %1;" ::"r"((uint32_t)__cvta_generic_to_shared(barrier)),
+                 "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ void load_tile(void* to, const CUtensorMap* map, uint32_t channel, uint32_t token,
+                                          uint64_t* barrier) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            (uint32_t)__cvta_generic_to_shared(to)),
+        "l"(map), "r"(channel), "r"(token), "r"((uint32_t)__cvta_generic_to_shared(barrier))
+        : "memory");
+}
+__device__ __forceinline__ void wait_landed(uint64_t* barrier, uint32_t parity) {
+    const uint32_t at = (uint32_t)__cvta_generic_to_shared(barrier);
+    for (uint32_t n = 0; n < kSpinLimit; ++n) {
+        uint32_t done;
+        asm volatile(
+            "{ .reg .pred p; mbarrier.try_wait.parity.shared.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+            : "=r"(done)
+            : "r"(at), "r"(parity)
+            : "memory");
+        if (done) return;
     }
+    atomicExch(&g_gave_up, 1u);
+}
+
+// A thread's four channels of a row, Unit of them neighbours: all four where
+// rows are tiled loads (16-byte aligned), two where rows keep pairs aligned, or
+// one.  Half a warp covers a row in 4 / Unit accesses.
+template <int Unit>
+struct Columns {
+    uint32_t at0;       // first column of the tile
+    uint32_t c;         // its channel
+    uint32_t channels;
+    __device__ __forceinline__ Columns(uint32_t group, uint32_t channels_) {
+        at0 = (threadIdx.x & 15u) * Unit;
+        c = group * kColumns + at0;
+        channels = channels_;
+    }
+    // Offset of access u from the first column.
+    static __device__ __forceinline__ constexpr uint32_t step(int u) { return u * 16u * Unit; }
+    __device__ __forceinline__ bool in(int u) const { return c + step(u) < channels; }
     template <typename E>
     __device__ __forceinline__ void copy(E* tile_row, const E* row) const {
-        if constexpr (Pair) {
-            if (in[0]) copy_async<2 * sizeof(E)>(tile_row + at[0], row);
+#pragma unroll
+        for (int u = 0; u < 4 / Unit; ++u)
+            if (in(u)) copy_async<Unit * sizeof(E)>(tile_row + at0 + step(u), row + step(u));
+    }
+    template <typename E>
+    __device__ __forceinline__ Quad get(const E* tile_row) const {
+        Quad q;
+        if constexpr (Unit == 1) {
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+                q.v[p] = pair_of(load(tile_row + at0 + step(2 * p)), load(tile_row + at0 + step(2 * p + 1)));
+        } else {
+            using Raw = typename Packed<E, Unit>::Raw;
+            Raw raw[4 / Unit];
+#pragma unroll
+            for (int u = 0; u < 4 / Unit; ++u) raw[u] = *reinterpret_cast<const Raw*>(tile_row + at0 + step(u));
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+                q.v[p] = PairOf<E>::unpack(reinterpret_cast<const uint32_t*>(raw) + p * (sizeof(E) / 2));
+        }
+        return q;
+    }
+    template <typename E>
+    __device__ __forceinline__ void put(E* row, const Quad& q) const {
+        if constexpr (Unit == 1) {
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const float2 f = parts(q.v[p]);
+                if (in(2 * p)) store(row + step(2 * p), f.x);
+                if (in(2 * p + 1)) store(row + step(2 * p + 1), f.y);
+            }
+        } else {
+            using Raw = typename Packed<E, Unit>::Raw;
+            Raw raw[4 / Unit];
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+                PairOf<E>::pack(q.v[p], reinterpret_cast<uint32_t*>(raw) + p * (sizeof(E) / 2));
+#pragma unroll
+            for (int u = 0; u < 4 / Unit; ++u)
+                if (in(u)) __stcs(reinterpret_cast<Raw*>(row + step(u)), raw[u]);
+        }
+    }
+    // Column of element e of the four.
+    static __device__ __forceinline__ constexpr uint32_t offset(int e) { return step(e / Unit) + e % Unit; }
+    // Of a row in global memory, one element at a time; zero where there is none.
+    template <typename E>
+    __device__ __forceinline__ Quad get_row(const E* row) const {
+        float f[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = row && c + offset(e) < channels ? load(row + c + offset(e)) : 0.0f;
+        Quad q;
+        q.v[0] = pair_of(f[0], f[1]), q.v[1] = pair_of(f[2], f[3]);
+        return q;
+    }
+    __device__ __forceinline__ Quad get_row(const float* rows, uint32_t row) const {
+        return get_row(rows ? rows + (size_t)row * channels : nullptr);
+    }
+    __device__ __forceinline__ void put_row(float* rows, uint32_t row, const Quad& q) const {
+        float* p = rows + (size_t)row * channels + c;
+        const float2 x = parts(q.v[0]), y = parts(q.v[1]);
+        const float f[4] = {x.x, x.y, y.x, y.y};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + offset(e) < channels) p[offset(e)] = f[e];
+    }
+    // A row of float in shared memory, this thread's columns.
+    __device__ __forceinline__ Quad get_shared(const float* row) const { return get(row); }
+    __device__ __forceinline__ void put_shared(float* row, const Quad& q) const {
+        const float2 x = parts(q.v[0]), y = parts(q.v[1]);
+        const float f[4] = {x.x, x.y, y.x, y.y};
+        if constexpr (Unit == 4) {
+            *reinterpret_cast<float4*>(row + at0) = make_float4(f[0], f[1], f[2], f[3]);
         } else {
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
-                if (in[k]) {
-                    if constexpr (sizeof(E) == 4)
-                        copy_async<4>(tile_row + at[k], row + 32 * k);
-                    else
-                        tile_row[at[k]] = row[32 * k];
-                }
+            for (int e = 0; e < 4; ++e) row[at0 + offset(e)] = f[e];
         }
     }
+};
+
+// 16-bit elements of rows that no aligned copy reaches, on their way from
+// global to shared memory through registers.
+template <int Length>
+struct Pending {
+    unsigned short v[Length][4];
     template <typename E>
-    __device__ __forceinline__ Pair32 get(const E* tile_row) const {
-        if constexpr (Pair)
-            return Packed<E>::unpack(*reinterpret_cast<const typename Packed<E>::Raw*>(tile_row + at[0]));
-        else
-            return pair_of(load(tile_row + at[0]), load(tile_row + at[1]));
+    __device__ __forceinline__ void read(const Columns<1>& col, int j, const E* row) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (col.in(u)) v[j][u] = __ldcs(reinterpret_cast<const unsigned short*>(row + col.step(u)));
     }
     template <typename E>
-    __device__ __forceinline__ void put(E* row, Pair32 v) const {
-        if constexpr (Pair) {
-            if (in[0]) __stcs(reinterpret_cast<typename Packed<E>::Raw*>(row), Packed<E>::pack(v));
-        } else {
-            const float2 f = parts(v);
-            if (in[0]) store(row, f.x);
-            if (in[1]) store(row + 32, f.y);
-        }
-    }
-    // Of a row that all tokens share.
-    template <typename E>
-    __device__ __forceinline__ Pair32 get_shared(const E* row) const {
-        return pair_of(in[0] ? load(row + c) : 0.0f, in[1] ? load(row + c + (Pair ? 1 : 32)) : 0.0f);
-    }
-    // Of a row of [stories][channels] float: zero where there is none.
-    __device__ __forceinline__ Pair32 get_row(const float* rows, uint32_t row, uint32_t channels) const {
-        const float* p = rows + (size_t)row * channels + c;
-        return pair_of(rows && in[0] ? __ldg(p) : 0.0f, rows && in[1] ? __ldg(p + (Pair ? 1 : 32)) : 0.0f);
-    }
-    __device__ __forceinline__ void put_row(float* rows, uint32_t row, uint32_t channels, Pair32 v) const {
-        float* p = rows + (size_t)row * channels + c;
-        const float2 f = parts(v);
-        if (in[0]) p[0] = f.x;
-        if (in[1]) p[Pair ? 1 : 32] = f.y;
+    __device__ __forceinline__ void write(const Columns<1>& col, int j, E* tile_row) const {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            reinterpret_cast<unsigned short*>(tile_row)[col.at0 + col.step(u)] = v[j][u];
     }
 };
 
@@ -400,16 +496,16 @@ __device__ __forceinline__ void copy_empty(const LeoB200StoryTables& t, uint32_t
     }
 }
 
-template <typename T, typename G, bool Pair, bool Shared, bool Backward>
+template <typename T, typename G, int Unit, bool Shared, bool Backward>
 __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_constant__ ScanArgs a) {
     using S = Shape<T, G, Shared, Backward>;
     constexpr int Length = S::kSegment;
     constexpr uint32_t kTile = S::kTile, kWordsATile = kTile / 32;
-    extern __shared__ __align__(16) unsigned char dynamic[];
+    constexpr bool Tiled = Unit == 4;
+    extern __shared__ __align__(128) unsigned char dynamic[];
     typename S::Control& control = *reinterpret_cast<typename S::Control*>(dynamic + kStages * S::kStage);
     const uint32_t warp = threadIdx.x >> 5;
     const uint32_t total = a.tiles * a.groups;
-
     // A ticket's tile and channel group; kNone past the end.
     const auto work_of = [&](uint32_t ticket) {
         if (ticket >= total) return make_uint2(kNone, 0);
@@ -428,66 +524,128 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
             if (!one_each) t = atomicAdd(a.scratch.ticket + (t == kNone), 1u) + 1u;  // after the one before
             control.ring[j] = work_of(one_each ? total : t);
         }
+        if constexpr (Tiled) {
+            for (int j = 0; j < kStages * kWarps; ++j)
+                asm volatile("mbarrier.init.shared.b64 [%0], 1;" ::"r"(
+                    (uint32_t)__cvta_generic_to_shared(&control.landed[0][0] + j))
+                             : "memory");
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
     }
     __syncthreads();
     const auto work_at = [&](uint32_t i) { return control.ring[i & 7u]; };
 
     if (warp < kWarps) {
         // ------------------------------------------------ the threads that map and write
-        const auto stage_x = [&](uint32_t i) {
-            return reinterpret_cast<T*>(dynamic + (i % kStages) * S::kStage) + warp * Length * kColumns;
+        const uint32_t lane = threadIdx.x & 31u, segment = warp * 2 + (lane >> 4);
+        const auto stage = [&](uint32_t i) { return dynamic + (i % kStages) * S::kStage; };
+        const auto stage_x = [&](uint32_t i, uint32_t seg) {
+            return reinterpret_cast<T*>(stage(i)) + seg * Length * kColumns;
         };
-        const auto stage_s = [&](uint32_t i) {
-            return reinterpret_cast<T*>(dynamic + (i % kStages) * S::kStage) + (kTile + warp * Length) * kColumns;
+        const auto stage_s = [&](uint32_t i, uint32_t seg) {
+            return reinterpret_cast<T*>(stage(i)) + (kTile + seg * Length) * kColumns;
         };
-        const auto stage_a = [&](uint32_t i) {
-            return reinterpret_cast<G*>(dynamic + (i % kStages) * S::kStage +
-                                        (size_t)(Backward ? 2 : 1) * kTile * kColumns * sizeof(T)) +
-                   warp * Length * kColumns;
+        const auto stage_a = [&](uint32_t i, uint32_t seg) {
+            return reinterpret_cast<G*>(stage(i) + (size_t)(Backward ? 2 : 1) * kTile * kColumns * sizeof(T)) +
+                   seg * Length * kColumns;
+        };
+        constexpr bool Pends = Unit == 1 && sizeof(T) == 2, GatePends = Unit == 1 && sizeof(G) == 2 && !Shared;
+        Pending<Pends ? Length : 1> pending_x, pending_s;
+        Pending<GatePends ? Length : 1> pending_a;
+        (void)pending_x, (void)pending_s, (void)pending_a;
+        // What the issue before left in registers.
+        const auto settle = [&](uint32_t i) {
+            if constexpr (Pends) {
+                const Columns<1> col(0, a.channels);
+#pragma unroll
+                for (int j = 0; j < Length; ++j) {
+                    pending_x.write(col, j, stage_x(i, segment) + j * kColumns);
+                    if constexpr (Backward) pending_s.write(col, j, stage_s(i, segment) + j * kColumns);
+                    if constexpr (GatePends) pending_a.write(col, j, stage_a(i, segment) + j * kColumns);
+                }
+            }
         };
         const auto issue = [&](uint32_t i) -> uint4 {
             uint4 word = make_uint4(0, 0, 0, 0);
             const uint2 work = work_at(i);
+            if (Pends && i > 0) settle(i - 1);
             if (work.x != kNone) {
-                const uint32_t first = work.x * kTile + warp * Length;
-                const Columns<Pair> col(work.y, a.channels);
-                const int count = first < a.tables.tokens ? (int)min(a.tables.tokens - first, (uint32_t)Length) : 0;
-                if (count) word = __ldg(reinterpret_cast<const uint4*>(a.tables.words) + (first >> 5));
-                const T* x = static_cast<const T*>(a.drive) + (int64_t)first * a.drive_stride + col.c;
-                const T* s = static_cast<const T*>(a.grad_states) + (int64_t)first * a.grad_states_stride + col.c;
-                const G* g = static_cast<const G*>(a.decay) + (int64_t)first * a.decay_stride + col.c;
-                T* to_x = stage_x(i);
-                T* to_s = stage_s(i);
-                G* to_a = stage_a(i);
-#pragma unroll
-                for (int j = 0; j < Length; ++j)
-                    if (j < count) {
-                        col.copy(to_x + j * kColumns, x + j * a.drive_stride);
-                        if constexpr (Backward) col.copy(to_s + j * kColumns, s + j * a.grad_states_stride);
-                        if constexpr (!Shared) col.copy(to_a + j * kColumns, g + j * a.decay_stride);
+                const uint32_t first = work.x * kTile + segment * Length;
+                if (first < a.tables.tokens) word = __ldg(reinterpret_cast<const uint4*>(a.tables.words) + (first >> 5));
+                if constexpr (Tiled) {
+                    // The warp's stage was read by its own lanes only.
+                    __syncwarp();
+                    const uint32_t token = work.x * kTile + warp * 2 * Length;
+                    if (lane == 0) {
+                        uint64_t* barrier = &control.landed[i % kStages][warp];
+                        const bool any = token < a.tables.tokens;  // if not, the barrier still turns
+                        expect_bytes(barrier, any ? 2 * Length * S::kRow : 0);
+                        if (any) {
+                            load_tile(stage_x(i, 2 * warp), &a.drive_map, work.y * kColumns, token, barrier);
+                            if constexpr (Backward)
+                                load_tile(stage_s(i, 2 * warp), &a.grad_map, work.y * kColumns, token, barrier);
+                            if constexpr (!Shared)
+                                load_tile(stage_a(i, 2 * warp), &a.decay_map, work.y * kColumns, token, barrier);
+                        }
                     }
+                } else {
+                    const Columns<Unit> col(work.y, a.channels);
+                    const int count = first < a.tables.tokens ? (int)min(a.tables.tokens - first, (uint32_t)Length) : 0;
+                    const T* x = static_cast<const T*>(a.drive) + (int64_t)first * a.drive_stride + col.c;
+                    const T* s = static_cast<const T*>(a.grad_states) + (int64_t)first * a.grad_states_stride + col.c;
+                    const G* g = static_cast<const G*>(a.decay) + (int64_t)first * a.decay_stride + col.c;
+#pragma unroll
+                    for (int j = 0; j < Length; ++j)
+                        if (j < count) {
+                            if constexpr (Pends) {
+                                pending_x.read(col, j, x + j * a.drive_stride);
+                                if constexpr (Backward) pending_s.read(col, j, s + j * a.grad_states_stride);
+                            } else {
+                                col.copy(stage_x(i, segment) + j * kColumns, x + j * a.drive_stride);
+                                if constexpr (Backward)
+                                    col.copy(stage_s(i, segment) + j * kColumns, s + j * a.grad_states_stride);
+                            }
+                            if constexpr (GatePends)
+                                pending_a.read(col, j, g + j * a.decay_stride);
+                            else if constexpr (!Shared)
+                                col.copy(stage_a(i, segment) + j * kColumns, g + j * a.decay_stride);
+                        }
+                }
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
+            if constexpr (!Tiled) asm volatile("cp.async.commit_group;" ::: "memory");
             return word;
+        };
+        // Waits for the loads of tile i, those of tile i + 1 being issued.
+        const auto landed = [&](uint32_t i) {
+            if constexpr (Tiled) {
+                wait_landed(&control.landed[i % kStages][warp], i / kStages & 1u);
+            } else {
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+            }
         };
         const auto map = [&](uint32_t i, uint4 word) {
             const uint2 work = work_at(i);
-            const Columns<Pair> col(work.y, a.channels);
-            const Segment s = segment_of<Length>(a.tables, word, work.x * kTile + warp * Length);
-            const T* x = stage_x(i);
-            const T* sp = stage_s(i);
-            const G* ap = stage_a(i);
-            Product2 A;
-            Pair32 H = 0, M = 0, gate = 0;
-            if constexpr (Shared) gate = col.get_shared(static_cast<const G*>(a.decay));
+            landed(i);
+            const Columns<Unit> col(work.y, a.channels);
+            const Segment s = segment_of<Length>(a.tables, word, work.x * kTile + segment * Length);
+            const T* x = stage_x(i, segment);
+            const T* sp = stage_s(i, segment);
+            const G* ap = stage_a(i, segment);
+            Product4 A;
+            Quad H, M, gate;
+            if constexpr (Shared) gate = col.get_row(static_cast<const G*>(a.decay));
             const auto forward = [&](int j) {
                 if constexpr (!Shared) gate = col.get(ap + j * kColumns);
-                H = fma2(gate, H, col.get(x + j * kColumns));
+                const Quad v = col.get(x + j * kColumns);
+#pragma unroll
+                for (int q = 0; q < 2; ++q) H.v[q] = fma2(gate.v[q], H.v[q], v.v[q]);
                 A.times(gate);
             };
             const auto backward = [&](int j) {
                 if constexpr (!Shared) gate = col.get(ap + j * kColumns);
-                M = mul2(gate, add2(col.get(sp + j * kColumns), M));
+                const Quad v = col.get(sp + j * kColumns);
+#pragma unroll
+                for (int q = 0; q < 2; ++q) M.v[q] = mul2(gate.v[q], add2(v.v[q], M.v[q]));
             };
             if (s.count == Length && (s.starts | s.ends) == 0) {
 #pragma unroll
@@ -499,44 +657,54 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
             } else {
 #pragma unroll 1
                 for (int j = 0; j < s.count; ++j) {
-                    if (s.starts >> j & 1u) H = col.get_row(a.initial, story_starting(a.tables, s, j), a.channels);
+                    if (s.starts >> j & 1u) H = col.get_row(a.initial, story_starting(a.tables, s, j));
                     forward(j);
                 }
                 if constexpr (Backward) {
 #pragma unroll 1
                     for (int j = s.count - 1; j >= 0; --j) {
-                        if (s.ends >> j & 1u) M = col.get_row(a.grad_final, story_ending(a.tables, s, j), a.channels);
+                        if (s.ends >> j & 1u) M = col.get_row(a.grad_final, story_ending(a.tables, s, j));
                         backward(j);
                     }
                 }
             }
             typename S::Maps& m = control.maps[i & 1u];
-            const float2 hi = parts(A.hi), lo = parts(A.lo), h = parts(H), r = parts(M);
-            m.A[warp][col.at[0]] = make_float2(hi.x, lo.x);
-            m.A[warp][col.at[1]] = make_float2(hi.y, lo.y);
-            m.H[warp][col.at[0]] = h.x, m.H[warp][col.at[1]] = h.y;
-            if constexpr (Backward) m.M[warp][col.at[0]] = r.x, m.M[warp][col.at[1]] = r.y;
-            if ((threadIdx.x & 31u) == 0) m.starts[warp] = s.starts != 0, m.ends[warp] = s.ends != 0;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const float2 hi = parts(A.hi[q]), lo = parts(A.lo[q]);
+                float2* row = m.A[segment] + col.at0;
+                if constexpr (Unit == 1) {
+                    row[col.offset(2 * q)] = make_float2(hi.x, lo.x);
+                    row[col.offset(2 * q + 1)] = make_float2(hi.y, lo.y);
+                } else {
+                    *reinterpret_cast<float4*>(row + col.offset(2 * q)) = make_float4(hi.x, lo.x, hi.y, lo.y);
+                }
+            }
+            col.put_shared(m.H[segment], H);
+            if constexpr (Backward) col.put_shared(m.M[segment], M);
+            if ((lane & 15u) == 0) m.starts[segment] = s.starts != 0, m.ends[segment] = s.ends != 0;
             arrive_at<1>(i & 1u);
         };
         const auto write = [&](uint32_t i, uint4 word) {
             const uint2 work = work_at(i);
-            const Columns<Pair> col(work.y, a.channels);
-            const uint32_t first = work.x * kTile + warp * Length;
+            const Columns<Unit> col(work.y, a.channels);
+            const uint32_t first = work.x * kTile + segment * Length;
             const Segment s = segment_of<Length>(a.tables, word, first);
-            const T* x = stage_x(i);
-            const T* sp = stage_s(i);
-            const G* ap = stage_a(i);
+            const T* x = stage_x(i, segment);
+            const T* sp = stage_s(i, segment);
+            const G* ap = stage_a(i, segment);
             const typename S::Maps& m = control.maps[i & 1u];
-            Pair32 h = pair_of(m.H[warp][col.at[0]], m.H[warp][col.at[1]]), gate = 0;
-            if constexpr (Shared) gate = col.get_shared(static_cast<const G*>(a.decay));
+            Quad h = col.get_shared(m.H[segment]), gate;
+            if constexpr (Shared) gate = col.get_row(static_cast<const G*>(a.decay));
             const size_t row = (size_t)first * a.channels + col.c;
             const bool plain = s.count == Length && (s.starts | s.ends) == 0;
             if constexpr (!Backward) {
                 T* out = static_cast<T*>(a.states) + row;
                 const auto step = [&](int j) {
                     if constexpr (!Shared) gate = col.get(ap + j * kColumns);
-                    h = fma2(gate, h, col.get(x + j * kColumns));
+                    const Quad v = col.get(x + j * kColumns);
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) h.v[q] = fma2(gate.v[q], h.v[q], v.v[q]);
                     col.put(out, h);
                     out += a.channels;
                 };
@@ -546,58 +714,57 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
                 } else {
 #pragma unroll 1
                     for (int j = 0; j < s.count; ++j) {
-                        if (s.starts >> j & 1u) h = col.get_row(a.initial, story_starting(a.tables, s, j), a.channels);
+                        if (s.starts >> j & 1u) h = col.get_row(a.initial, story_starting(a.tables, s, j));
                         step(j);
-                        if (s.ends >> j & 1u) col.put_row(a.final_states, story_ending(a.tables, s, j), a.channels, h);
+                        if (s.ends >> j & 1u) col.put_row(a.final_states, story_ending(a.tables, s, j), h);
                     }
                 }
             } else {
                 // The state before each token, then the slopes from the right.
-                Pair32 previous[Length];
+                Quad previous[Length];
 #pragma unroll
                 for (int j = 0; j < Length; ++j) {
-                    if (!plain && (s.starts >> j & 1u))
-                        h = col.get_row(a.initial, story_starting(a.tables, s, j), a.channels);
+                    if (!plain && (s.starts >> j & 1u)) h = col.get_row(a.initial, story_starting(a.tables, s, j));
                     if constexpr (!Shared) gate = col.get(ap + j * kColumns);
                     previous[j] = h;
-                    h = fma2(gate, h, col.get(x + j * kColumns));
+                    const Quad v = col.get(x + j * kColumns);
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) h.v[q] = fma2(gate.v[q], h.v[q], v.v[q]);
                 }
-                Pair32 n = pair_of(m.M[warp][col.at[0]], m.M[warp][col.at[1]]), sum = 0;
+                Quad n = col.get_shared(m.M[segment]), sum;
                 T* out = static_cast<T*>(a.grad_drive) + row + (size_t)(Length - 1) * a.channels;
                 G* out_gate = static_cast<G*>(a.grad_decay) + (Shared ? 0 : row + (size_t)(Length - 1) * a.channels);
 #pragma unroll
                 for (int j = Length - 1; j >= 0; --j) {
                     if (plain || j < s.count) {
                         if (!plain && (s.ends >> j & 1u))
-                            n = col.get_row(a.grad_final, story_ending(a.tables, s, j), a.channels);
+                            n = col.get_row(a.grad_final, story_ending(a.tables, s, j));
                         if constexpr (!Shared) gate = col.get(ap + j * kColumns);
-                        const Pair32 slope = add2(col.get(sp + j * kColumns), n);
-                        const Pair32 term = mul2(slope, previous[j]);
-                        n = mul2(gate, slope);
+                        const Quad v = col.get(sp + j * kColumns);
+                        Quad slope, term;
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            slope.v[q] = add2(v.v[q], n.v[q]);
+                            term.v[q] = mul2(slope.v[q], previous[j].v[q]);
+                            n.v[q] = mul2(gate.v[q], slope.v[q]);
+                            if constexpr (Shared) sum.v[q] = add2(sum.v[q], term.v[q]);
+                        }
                         col.put(out, slope);
-                        if constexpr (Shared)
-                            sum = add2(sum, term);
-                        else
-                            col.put(out_gate, term);
+                        if constexpr (!Shared) col.put(out_gate, term);
                         if (!plain && a.grad_initial && (s.starts >> j & 1u))
-                            col.put_row(a.grad_initial, story_starting(a.tables, s, j), a.channels, n);
+                            col.put_row(a.grad_initial, story_starting(a.tables, s, j), n);
                     }
                     out -= a.channels;
                     if constexpr (!Shared) out_gate -= a.channels;
                 }
-                if constexpr (Shared) {
-                    const float2 f = parts(sum);
-                    control.sums[i & 1u][warp][col.at[0]] = f.x, control.sums[i & 1u][warp][col.at[1]] = f.y;
-                }
+                if constexpr (Shared) col.put_shared(control.sums[i & 1u][segment], sum);
             }
         };
 
         uint4 word0 = issue(0), word1 = issue(1);
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
         if (work_at(0).x != kNone) map(0, word0);
         for (uint32_t i = 0; work_at(i).x != kNone; ++i) {
             const uint4 word2 = issue(i + 2);
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
             if (work_at(i + 1).x != kNone) map(i + 1, word1);
             sync_of<3>(i & 1u);
             write(i, word0);
@@ -610,14 +777,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
         // A lane takes half the segments of a channel, the nearer ones in the
         // direction of the scan first, and half the slots; its partner is 16 lanes away.
         constexpr int Direction = Backward ? -1 : 1;
-        constexpr int kHalf = kWarps / 2;
+        constexpr int kHalf = kSegments / 2;
         const uint32_t lane = threadIdx.x & 31u, half = lane >> 4, k = (warp - kWarps) * 16 + (lane & 15u);
         const bool leader = threadIdx.x == 32 * kWarps;
         const auto add_sums = [&](uint32_t i, uint2 work) {
             const uint32_t c = work.y * kColumns + k;
             float sum = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) sum += control.sums[i & 1u][w][k];
+            for (int w = 0; w < kSegments; ++w) sum += control.sums[i & 1u][w][k];
             if (c >= a.channels || half) return;
             if (a.tiles == 1)
                 store(static_cast<G*>(a.grad_decay) + c, sum);
@@ -642,7 +809,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
                 kept = __ldcs(a.carries + (size_t)tile * (kTile / kKept) * a.channels + c);
             const Lookback<Direction> back(a, tile, end, kWordsATile);
             end = next_end;
-            if (leader) control.ring[(i + 3) & 7u] = work_of(later);
             sync_of<1>(i & 1u);
             typename S::Maps& m = control.maps[i & 1u];
             if constexpr (Backward && Shared)
@@ -651,7 +817,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
             // The map of this half of the tile, then of the tile, in the direction of the scan.
             const uint2 cut_bytes =
                 reinterpret_cast<const uint2*>(Backward ? m.ends : m.starts)[Backward ? 1 - half : half];
-            const auto segment = [&](int j) { return (Backward ? kWarps - 1 - j : j) + (Backward ? -1 : 1) * (int)half * kHalf; };
+            const auto segment = [&](int j) { return (Backward ? kSegments - 1 - j : j) + (Backward ? -1 : 1) * (int)half * kHalf; };
             const auto cut_at = [&](int j) {  // of this half
                 const int byte = Backward ? kHalf - 1 - j : j;
                 return ((byte < 4 ? cut_bytes.x : cut_bytes.y) >> (byte & 3) * 8 & 1u) != 0;
@@ -751,6 +917,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
                     at = start_at(j) ? h[j] : fmaf(A[kHalf - 1 - j], at, h[j]);
                 }
             }
+            if (leader) control.ring[(i + 3) & 7u] = work_of(later);
             arrive_at<3>(i & 1u);
             if (tile == 0 && a.tables.full < a.tables.stories && half == 0) {
                 if constexpr (!Backward)
@@ -844,13 +1011,46 @@ size_t lay_out(uint32_t tokens, uint32_t channels, void* base, Scratch* s) {
     return partials + tiles * channels * sizeof(float);
 }
 
-// Whether rows of `channels` elements of `size` bytes can be moved two at a time.
-bool in_pairs(const void* p, int64_t stride, size_t size) {
-    return reinterpret_cast<uintptr_t>(p) % (2 * size) == 0 && stride % 2 == 0;
+// Neighbours of a row that can be moved at once, going by its address and stride.
+int unit_of(const void* p, int64_t stride, size_t size) {
+    const auto fits = [&](size_t bytes) {
+        return reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride * (int64_t)size % (int64_t)bytes == 0;
+    };
+    return fits(16) ? 4 : fits(2 * size) ? 2 : 1;
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+    static const EncodeTiled found = [] {
+        void* entry = nullptr;
+        cudaDriverEntryPointQueryResult result{};
+        check(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &entry, cudaEnableDefault, &result),
+              "cuTensorMapEncodeTiled");
+        require(entry != nullptr && result == cudaDriverEntryPointSuccess, "cuTensorMapEncodeTiled is missing");
+        return reinterpret_cast<EncodeTiled>(entry);
+    }();
+    return found;
+}
+
+// Boxes of `rows` tokens of kColumns channels.
+template <typename E>
+void describe(CUtensorMap* map, const void* p, int64_t stride, uint32_t tokens, uint32_t channels, uint32_t rows) {
+    const CUtensorMapDataType type = std::is_same_v<E, float>    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : std::is_same_v<E, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const cuuint64_t sizes[2] = {channels, tokens}, strides[1] = {(cuuint64_t)stride * sizeof(E)};
+    const cuuint32_t box[2] = {kColumns, rows}, steps[2] = {1, 1};
+    const CUresult r = encode_tiled()(map, type, 2, const_cast<void*>(p), sizes, strides, box, steps,
+                                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    require(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled refused a tensor");
 }
 
 // Launches one scan on `stream`: one block an SM, or one a tile if there are few.
-template <typename T, typename G, bool Pair, bool Shared, bool Backward>
+template <typename T, typename G, int Unit, bool Shared, bool Backward>
 void launch_scan(ScanArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
     using S = Shape<T, G, Shared, Backward>;
     static_assert(S::kBytes <= kSharedLimit && S::kTile % kKept == 0 && kKept % S::kSegment == 0, "shape");
@@ -867,8 +1067,15 @@ void launch_scan(ScanArgs& a, void* workspace, size_t workspace_bytes, cudaStrea
     int device = 0, sms = 0;
     check(cudaGetDevice(&device), "cudaGetDevice");
     check(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device), "SM count");
-    const auto kernel = scan_kernel<T, G, Pair, Shared, Backward>;
+    const auto kernel = scan_kernel<T, G, Unit, Shared, Backward>;
     check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kBytes), "shared memory");
+    if constexpr (Unit == 4) {
+        const uint32_t rows = 2 * S::kSegment;
+        describe<T>(&a.drive_map, a.drive, a.drive_stride, a.tables.tokens, a.channels, rows);
+        if constexpr (!Shared) describe<G>(&a.decay_map, a.decay, a.decay_stride, a.tables.tokens, a.channels, rows);
+        if constexpr (Backward)
+            describe<T>(&a.grad_map, a.grad_states, a.grad_states_stride, a.tables.tokens, a.channels, rows);
+    }
     if (a.tiles > 1)
         check(cudaMemsetAsync(workspace, 0xff, 256 + (size_t)a.tiles * a.channels * sizeof(Slot), stream), "clear scan slots");
     const uint32_t blocks = a.tiles == 1 || total <= 2u * (uint32_t)sms ? (uint32_t)total : (uint32_t)sms;
@@ -876,13 +1083,22 @@ void launch_scan(ScanArgs& a, void* workspace, size_t workspace_bytes, cudaStrea
     check(cudaGetLastError(), "scan_kernel");
 }
 
-// Calls body(Pair, Shared) as types.
+// Calls body(Unit, Shared) as types.
 template <typename Body>
-void dispatch_shape(bool pairs, bool shared, Body&& body) {
-    if (pairs && shared) body(std::true_type{}, std::true_type{});
-    else if (pairs) body(std::true_type{}, std::false_type{});
-    else if (shared) body(std::false_type{}, std::true_type{});
-    else body(std::false_type{}, std::false_type{});
+void dispatch_shape(int unit, bool shared, Body&& body) {
+    const auto with = [&](auto u) { shared ? body(u, std::true_type{}) : body(u, std::false_type{}); };
+    if (unit == 4) with(std::integral_constant<int, 4>{});
+    else if (unit == 2) with(std::integral_constant<int, 2>{});
+    else with(std::integral_constant<int, 1>{});
+}
+
+// Tiled loads and rows of neighbours need every tensor of the call to allow
+// them; a stride of zero has no tiled form.
+int unit_of_call(uint32_t channels, uint32_t tokens, int64_t stride0, int64_t stride1, int64_t stride2, int least) {
+    int unit = std::min(least, channels % 4 == 0 ? 4 : channels % 2 == 0 ? 2 : 1);
+    const bool strided = stride0 > 0 && stride1 > 0 && stride2 > 0;
+    if (unit == 4 && (!strided || tokens == 0)) unit = 2;
+    return unit;
 }
 
 }  // namespace
@@ -953,12 +1169,13 @@ int leo_b200_gated_scan(int device, const LeoB200StoryTables* tables, uint32_t c
         dispatch(dtype, decay_dtype, [&](auto* t, auto* g) {
             using T = std::remove_pointer_t<decltype(t)>;
             using G = std::remove_pointer_t<decltype(g)>;
-            const bool pairs = channels % 2 == 0 && in_pairs(drive, drive_stride, sizeof(T)) &&
-                               in_pairs(decay, decay_shared ? 0 : decay_stride, sizeof(G)) &&
-                               in_pairs(states, 0, sizeof(T));
+            const bool shared = decay_shared != 0 && tables->tokens > 0;
+            int unit = std::min(unit_of(drive, drive_stride, sizeof(T)), unit_of(states, channels, sizeof(T)));
+            if (!shared) unit = std::min(unit, unit_of(decay, decay_stride, sizeof(G)));
+            unit = unit_of_call(channels, tables->tokens, drive_stride, shared ? 1 : decay_stride, 1, unit);
             DeviceScope scope(device);
-            dispatch_shape(pairs, decay_shared != 0 && tables->tokens > 0, [&](auto pair, auto shared) {
-                launch_scan<T, G, pair(), shared(), false>(a, workspace, workspace_bytes, (cudaStream_t)stream);
+            dispatch_shape(unit, shared, [&](auto u, auto is_shared) {
+                launch_scan<T, G, u(), is_shared(), false>(a, workspace, workspace_bytes, (cudaStream_t)stream);
             });
         });
     });
@@ -993,13 +1210,16 @@ int leo_b200_gated_scan_backward(int device, const LeoB200StoryTables* tables, u
         dispatch(dtype, decay_dtype, [&](auto* t, auto* g) {
             using T = std::remove_pointer_t<decltype(t)>;
             using G = std::remove_pointer_t<decltype(g)>;
-            const bool pairs = channels % 2 == 0 && in_pairs(drive, drive_stride, sizeof(T)) &&
-                               in_pairs(decay, decay_shared ? 0 : decay_stride, sizeof(G)) &&
-                               in_pairs(grad_states, grad_states_stride, sizeof(T)) &&
-                               in_pairs(grad_drive, 0, sizeof(T)) && in_pairs(grad_decay, 0, sizeof(G));
+            const bool shared = decay_shared != 0;
+            int unit = std::min(unit_of(drive, drive_stride, sizeof(T)),
+                                unit_of(grad_states, grad_states_stride, sizeof(T)));
+            unit = std::min(unit, unit_of(grad_drive, channels, sizeof(T)));
+            if (!shared)
+                unit = std::min({unit, unit_of(decay, decay_stride, sizeof(G)), unit_of(grad_decay, channels, sizeof(G))});
+            unit = unit_of_call(channels, tables->tokens, drive_stride, shared ? 1 : decay_stride, grad_states_stride, unit);
             DeviceScope scope(device);
-            dispatch_shape(pairs, decay_shared != 0, [&](auto pair, auto shared) {
-                launch_scan<T, G, pair(), shared(), true>(a, workspace, workspace_bytes, (cudaStream_t)stream);
+            dispatch_shape(unit, shared, [&](auto u, auto is_shared) {
+                launch_scan<T, G, u(), is_shared(), true>(a, workspace, workspace_bytes, (cudaStream_t)stream);
                 if (decay_shared && a.tiles > 1) {
                     shared_decay_kernel<G><<<(channels + 31) / 32, kThreads, 0, (cudaStream_t)stream>>>(
                         a.scratch.partials, a.tiles, channels, static_cast<G*>(grad_decay));
