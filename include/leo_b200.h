@@ -329,21 +329,23 @@ size_t leo_b200_sparse_apply_scratch_bytes(int device);
    device is restored, and they can be captured into a CUDA graph.  Outputs
    must not overlap inputs unless said otherwise. */
 
-/* The story table of a packed batch, on the host: story s owns tokens
-   offsets[s] .. offsets[s + 1] (offsets[0] == 0, fewer than 2^31 tokens).
-   `words` receives ceil(tokens / 32) entries, `order` one per story, `full`
-   the number of stories with a token; the caller copies both arrays to the
-   device and fills a LeoB200StoryTables.  The device calls trust its contents. */
-int leo_b200_story_table(const uint64_t* offsets, uint32_t stories, LeoB200StoryWord* words, uint32_t* order,
-                         uint32_t* full);
+/* The story table of a packed batch: story s owns tokens offsets[s] ..
+   offsets[s + 1] (host memory; offsets[0] == 0, fewer than 2^31 tokens).
+   leo_b200_story_table_bytes returns its size, 0 for offsets that are refused.
+   leo_b200_story_table writes it to host memory and fills `tables` with
+   pointers into `device_table`, where the caller copies it (both aligned to 16
+   bytes).  The device calls trust its contents. */
+size_t leo_b200_story_table_bytes(const uint64_t* offsets, uint32_t stories);
+int leo_b200_story_table(const uint64_t* offsets, uint32_t stories, void* table, size_t bytes, const void* device_table,
+                         LeoB200StoryTables* tables);
 
-/* Bytes of device scratch (any contents) that one call of
-   leo_b200_gated_scan or leo_b200_gated_scan_backward needs for `tokens`
-   tokens of `channels` channels; calls that may overlap in time, or that are
-   captured into different graphs, need scratch of their own. */
-size_t leo_b200_gated_scan_workspace(uint32_t tokens, uint32_t channels);
+/* Bytes of device scratch (any contents, aligned to 16 bytes) that one call of
+   leo_b200_gated_scan or leo_b200_gated_scan_backward needs; calls that may
+   overlap in time, or that are captured into different graphs, need scratch of
+   their own. */
+size_t leo_b200_gated_scan_workspace(const LeoB200StoryTables* tables, uint32_t channels);
 /* Floats that leo_b200_gated_scan keeps for its backward pass. */
-size_t leo_b200_gated_scan_carry_count(uint32_t tokens, uint32_t channels);
+size_t leo_b200_gated_scan_carry_count(const LeoB200StoryTables* tables, uint32_t channels);
 
 /* The gated linear recurrence of every story and channel, as the decaying
    states of the per-byte step are, over whole stories:

@@ -360,23 +360,34 @@ enum LeoB200Dtype {
 };
 
 #define LEO_B200_STORY_WORD_TOKENS 32u
+#define LEO_B200_TILE_TOKENS 128u
 
-/* Where stories begin and end in a word of 32 consecutive tokens of a packed
-   batch (leo_b200_story_table).  "A story of the word" has a token in it. */
+/* Where stories with a token start in 32 consecutive tokens of a packed batch. */
 typedef struct LeoB200StoryWord {
-    uint32_t starts; /* bit i: token 32 w + i is the first of its story */
-    uint32_t rank;   /* stories with a token that start before token 32 w */
-    uint32_t begin;  /* first token of the story that token 32 w belongs to */
-    uint32_t end;    /* one past the last token of the story that the word's last token belongs to */
+    uint32_t starts; /* bit i: token 32 w + i is the first of its story, or one past the batch's last */
+    uint32_t rank;   /* stories that start before token 32 w */
 } LeoB200StoryWord;
 
-/* The device copy of a story table. */
+/* A run of tokens that a scan handles at a time. */
+typedef struct LeoB200StoryTile {
+    uint32_t first;
+    uint32_t count;
+    uint32_t tile;   /* its place in the order of tokens */
+    uint32_t kept;   /* the kept state before it; one for every 64 tokens */
+    uint32_t holder; /* the tile where the story that crosses into it starts (backward: ends); its own if none does */
+    uint32_t onward; /* whether a story crosses out of it */
+    uint32_t unused[2];
+} LeoB200StoryTile;
+
+/* The parts of a story table on the device, filled by leo_b200_story_table. */
 typedef struct LeoB200StoryTables {
-    const LeoB200StoryWord* words; /* device, [ceil(tokens / 32)] */
-    const uint32_t* order;         /* device, [stories]: the stories with a token in order, then those without */
+    const LeoB200StoryWord* words;
+    const uint32_t* order;                  /* the stories with a token in order, then those without */
+    const LeoB200StoryTile* schedule[2][2]; /* tiles of 128, of 64 tokens; forward, backward */
+    uint32_t tiles[2];                      /* how many of 128, of 64 tokens or fewer */
     uint32_t tokens;
     uint32_t stories;
-    uint32_t full;                 /* stories with a token */
+    uint32_t full;                          /* stories with a token */
 } LeoB200StoryTables;
 
 /* What acts on a row of logits before it is used, in this order: penalties

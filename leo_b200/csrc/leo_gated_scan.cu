@@ -4,29 +4,32 @@
 //   h[t] = a[t] h[t-1] + x[t]
 //   slope[t] = g[t] + a[t+1] slope[t+1];  dx = slope, da[t] = slope[t] h[t-1]
 //
-// Tiles.  The packed batch is cut into tiles of equal length whatever its
-// stories are, so a ragged batch balances by itself; a block of 16 warps takes
-// a tile of 64 channels, each thread a segment of a few tokens in a row of two
-// channels.  A span of tokens maps the state before it to the state after it
-// as h -> A h + H (A the product of the gates, H the state from zero), or as
-// h -> H if a story starts inside, and such maps compose: the segments' maps
-// give the tile's, the tiles' maps the state before a tile, and each thread
-// then runs its tokens again and writes them.  The backward pass is the same
-// from the right, with m -> A m + M for m[t] = a[t] slope[t]; h is formed anew
-// from the states that the forward pass keeps every 64 tokens.
+// Maps.  A span of tokens maps the state before it to the state after it as
+// h -> A h + H (A the product of the gates, H the state from zero), or as
+// h -> H if a story starts inside, and such maps compose.  The batch is cut into
+// tiles of 128 tokens or fewer (leo_b200_story_table): a block takes a tile of
+// 64 channels, each thread a segment of 8 tokens of four channels.  The
+// segments' maps give the tile's, the tiles' maps the state before a tile, and
+// each thread then runs its tokens again and writes them.  The backward pass is
+// the same from the right, with m -> A m + M for m[t] = a[t] slope[t]; h is
+// formed anew from the states that the forward pass keeps every 64 tokens.
 //
-// Pipeline.  One block an SM works through tiles dealt by a ticket in token
-// order.  While the loads of tile i + 2 are in flight into its own third of
-// shared memory (each thread copies what it will use itself, so they need no
-// barrier), the threads map tile i + 1 and write tile i, and two more warps
-// compose tile i + 1.  Every input is read once and the loads never pause.
+// Pipeline.  One block an SM works through tiles dealt by a ticket.  While the
+// loads of tile i + 2 are in flight into its own third of shared memory (each
+// warp loads what it will use itself, so they need no barrier), eight warps map
+// tile i + 1 and write tile i, and four more compose tile i + 1.  Every input
+// is read once and the loads never pause.
 //
 // Between tiles.  Each tile publishes its map, every kGroup-th the state after
-// it instead, so a tile reads at most kGroup slots of tiles with lower
-// tickets, which have started before it.  A slot and its mark are one 16-byte
-// word, written and read as one, so a slot that is there costs one trip to L2.
-// Which slots are read, and in which order they are composed, depends on the
-// layout alone: results are the same in every run.
+// it instead, so a tile reads at most kGroup slots.  A slot and its mark are one
+// 8-byte word, so a slot that is there costs one trip to L2.  Tickets deal the
+// first tiles of all stories, then their second ones, and so on: a tile's
+// predecessors have lower tickets, so they have started before it and every wait
+// ends, and with many stories they are long done when it reads them.  Tiles in
+// the order of their tokens wait for neighbours that are mapped in the same
+// moment: 81,920 tokens x 1,024 channels of 64 stories took 236 us that way,
+// 127 us without any wait.  Which slots are read, and in which order they are
+// composed, depends on the layout alone: results are the same in every run.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -35,7 +38,9 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <cstring>
 #include <type_traits>
+#include <vector>
 
 #include "../../include/leo_b200.h"
 #include "leo_operator_host.h"
@@ -61,7 +66,7 @@ constexpr uint32_t kTileThreads = 32 * (kWarps + kCarryWarps);
 constexpr int kStages = 3;
 constexpr uint32_t kNone = 0xffffffffu;
 constexpr size_t kSharedLimit = 227 * 1024;
-constexpr uint32_t kKept = 64;                   // tokens between the states kept for the backward pass
+constexpr uint32_t kKept = LEO_B200_TILE_TOKENS / 2;  // tokens between the states kept for the backward pass
 constexpr int kGroup = 16;                       // tiles between published states
 constexpr uint32_t kSpinLimit = 1u << 21;        // polls of a wait, a memory round trip and more apart
 
@@ -163,6 +168,7 @@ struct Scratch {
 struct ScanArgs {
     CUtensorMap drive_map, decay_map, grad_map;  // of the tiled loads
     LeoB200StoryTables tables;
+    const LeoB200StoryTile* schedule;  // the tiles in the order of their tickets
     uint32_t channels, tiles, groups;  // groups: of 64 channels
     const void* drive;
     int64_t drive_stride;
@@ -184,23 +190,28 @@ struct ScanArgs {
 
 // A thread's tokens among the stories.
 struct Segment {
-    int count;        // tokens before the batch's end
+    int count;        // tokens of the tile
     uint32_t starts;  // bit i: token i of the segment is the first of its story
     uint32_t ends;    // bit i: ... the last
     uint32_t rank;    // stories that start before the segment
 };
 
-// `word`: the story word of token `first`.
-template <int Length>
-__device__ __forceinline__ Segment segment_of(const LeoB200StoryTables& t, uint4 word, uint32_t first) {
-    Segment s{0, 0, 0, 0};
-    if (first >= t.tokens) return s;
-    s.count = (int)min(t.tokens - first, (uint32_t)Length);
-    const uint32_t base = first & ~31u, shift = first & 31u;
-    const uint32_t ends = (word.x >> 1) | (word.w <= base + 32u ? 1u << (word.w - 1u - base) : 0u);
-    s.starts = (word.x >> shift) & ((1u << Length) - 1u);
-    s.ends = (ends >> shift) & ((1u << Length) - 1u);
-    s.rank = word.y + __popc(word.x & ((1u << shift) - 1u));
+// The two words of the story table that a segment's tokens lie in.
+struct StoryBits {
+    uint2 low, high;  // starts, rank
+};
+__device__ __forceinline__ StoryBits story_bits(const LeoB200StoryTables& t, uint32_t first) {
+    const uint2* p = reinterpret_cast<const uint2*>(t.words) + (first >> 5);
+    return {__ldg(p), __ldg(p + 1)};
+}
+__device__ __forceinline__ Segment segment_of(const StoryBits& b, uint32_t first, int count) {
+    Segment s{count, 0, 0, 0};
+    if (count <= 0) return s;
+    const uint32_t shift = first & 31u, mask = (1u << count) - 1u;
+    const uint32_t bits = (uint32_t)(((uint64_t)b.high.x << 32 | b.low.x) >> shift);
+    s.starts = bits & mask;
+    s.ends = bits >> 1 & mask;
+    s.rank = b.low.y + __popc(b.low.x & ((1u << shift) - 1u));
     return s;
 }
 // The story that starts at, or ends with, token i of the segment.
@@ -241,20 +252,10 @@ template <int Direction>
 struct Lookback {
     uint32_t from;  // tile whose slot is a state
     int maps;       // tiles between it and this one; -1: no story crosses in
-    // The first or last token of the story that crosses into a tile, read ahead of time.
-    static __device__ __forceinline__ uint32_t end_of(const ScanArgs& a, uint32_t tile, uint32_t words_a_tile) {
-        if (a.tiles == 1 || tile == kNone) return 0;
-        const uint32_t words = (a.tables.tokens + 31) / 32;
-        if (Direction > 0) return __ldg(&a.tables.words[tile * words_a_tile].begin);
-        return __ldg(&a.tables.words[min((tile + 1) * words_a_tile, words) - 1].end) - 1;
-    }
-    __device__ __forceinline__ Lookback(const ScanArgs& a, uint32_t tile, uint32_t end, uint32_t words_a_tile) {
+    __device__ __forceinline__ Lookback(uint32_t tile, uint32_t holder) {
         maps = -1;
-        from = tile;
-        if (a.tiles == 1) return;
-        const uint32_t holder = end / (32 * words_a_tile);
-        if (holder == tile) return;
         from = holder;
+        if (holder == tile) return;
         // A state is published by the last tile of a group of kGroup in the direction of the scan.
         if (Direction > 0) {
             const uint32_t p = tile / kGroup * kGroup;
@@ -266,31 +267,44 @@ struct Lookback {
             maps = (int)(from - tile - 1);
         }
     }
-    // Reads half the slots of a channel once: the state and the first seven
-    // maps (half 0), or the other eight (half 1), composed as (A, H).  False if
-    // one of them is not there yet.
-    __device__ __forceinline__ bool read(const Slot* slots, uint32_t channels, uint32_t c, int half, float& A,
-                                         float& H) const {
+    // Half the slots of a channel: the state and the first seven maps (half 0),
+    // or the other eight (half 1).
+    __device__ __forceinline__ void load(const Slot* slots, uint32_t channels, uint32_t c, int half, Slot (&s)[8]) const {
         const int64_t step = (int64_t)Direction * channels;
-        const int count = min(maps + 1 - half * 8, 8);
+        const int count = maps + 1 - half * 8;
         const Slot* p = slots + (size_t)from * channels + c + half * 8 * step;
-        Slot s[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             if (j < count) s[j] = read_slot(p + j * step);
-        uint32_t there = 1;
+    }
+    // Composes them as (A, H); false if one of them was not there yet.
+    __device__ __forceinline__ bool compose(const Slot (&s)[8], int half, float& A, float& H) const {
+        const int count = maps + 1 - half * 8;
+        bool there = true;
         A = 1.0f, H = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             if (j < count) {
                 const uint32_t low = (uint32_t)s[j];
-                there &= low != kNone;
-                H = fmaf(__uint_as_float(low), H, __uint_as_float((uint32_t)(s[j] >> 32)));
+                const float value = __uint_as_float((uint32_t)(s[j] >> 32));
+                there = there && low != kNone;
+                H = j == 0 && half == 0 ? value : fmaf(__uint_as_float(low), H, value);
                 A *= __uint_as_float(low);
-                if (j == 0 && half == 0) H = __uint_as_float((uint32_t)(s[j] >> 32));
             }
         return there;
     }
+};
+
+// A tile of a channel group.
+struct Work {
+    uint32_t first;   // token
+    uint32_t count;   // tokens; kNone: no more work
+    uint32_t tile;
+    uint32_t group;
+    uint32_t holder;  // the tile where the story that crosses into this one begins (forward) or ends; or this one
+    uint32_t kept;    // the kept state before it
+    uint32_t onward;  // whether a story crosses out of it
+    uint32_t unused;
 };
 
 // The shape of a kernel: its tiles, and its shared memory.
@@ -307,7 +321,7 @@ struct Shape {
     struct Control {
         Maps maps[2];
         float sums[Backward && Shared ? 2 : 1][Backward && Shared ? kSegments : 1][kColumns];
-        uint2 ring[8];  // the block's (tile, group)s; an entry is rewritten when no warp reads it any more
+        Work ring[8];  // the block's work; an entry is rewritten when no warp reads it any more
         uint64_t landed[kStages][kWarps];  // barriers of the tiled loads
     };
     // 8 tokens a thread, or 4 where three stages of them would not fit.
@@ -500,17 +514,19 @@ template <typename T, typename G, int Unit, bool Shared, bool Backward>
 __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_constant__ ScanArgs a) {
     using S = Shape<T, G, Shared, Backward>;
     constexpr int Length = S::kSegment;
-    constexpr uint32_t kTile = S::kTile, kWordsATile = kTile / 32;
+    constexpr uint32_t kTile = S::kTile;
     constexpr bool Tiled = Unit == 4;
     extern __shared__ __align__(128) unsigned char dynamic[];
     typename S::Control& control = *reinterpret_cast<typename S::Control*>(dynamic + kStages * S::kStage);
     const uint32_t warp = threadIdx.x >> 5;
     const uint32_t total = a.tiles * a.groups;
-    // A ticket's tile and channel group; kNone past the end.
     const auto work_of = [&](uint32_t ticket) {
-        if (ticket >= total) return make_uint2(kNone, 0);
-        const uint32_t tile = ticket / a.groups;
-        return make_uint2(Backward ? a.tiles - 1 - tile : tile, ticket - tile * a.groups);
+        Work w{0, kNone, 0, 0, 0, 0, 0, 0};
+        if (ticket >= total) return w;
+        const uint32_t place = ticket / a.groups;
+        const uint4* entry = reinterpret_cast<const uint4*>(a.schedule + place);
+        const uint4 x = __ldg(entry), y = __ldg(entry + 1);  // first, count, tile, kept; holder, onward
+        return Work{x.x, x.y, x.z, ticket - place * a.groups, y.x, x.w, y.y, 0};
     };
     // The first tickets: one if there is a block for each, or three, drawn one
     // after the other so that the blocks take turns: a block that held the next
@@ -533,7 +549,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
         }
     }
     __syncthreads();
-    const auto work_at = [&](uint32_t i) { return control.ring[i & 7u]; };
+    const auto work_at = [&](uint32_t i) -> const Work& { return control.ring[i & 7u]; };
 
     if (warp < kWarps) {
         // ------------------------------------------------ the threads that map and write
@@ -565,32 +581,36 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
                 }
             }
         };
-        const auto issue = [&](uint32_t i) -> uint4 {
-            uint4 word = make_uint4(0, 0, 0, 0);
-            const uint2 work = work_at(i);
+        // Tokens of the thread's segment.
+        const auto tokens_of = [&](const Work& work) {
+            return max(min((int)work.count - (int)segment * Length, Length), 0);
+        };
+        const auto issue = [&](uint32_t i) -> StoryBits {
+            StoryBits bits{};
+            const Work& work = work_at(i);
             if (Pends && i > 0) settle(i - 1);
-            if (work.x != kNone) {
-                const uint32_t first = work.x * kTile + segment * Length;
-                if (first < a.tables.tokens) word = __ldg(reinterpret_cast<const uint4*>(a.tables.words) + (first >> 5));
+            if (work.count != kNone) {
+                const uint32_t first = work.first + segment * Length, group = work.group;
+                const int count = tokens_of(work);
+                if (count) bits = story_bits(a.tables, first);
                 if constexpr (Tiled) {
                     // The warp's stage was read by its own lanes only.
                     __syncwarp();
-                    const uint32_t token = work.x * kTile + warp * 2 * Length;
                     if (lane == 0) {
                         uint64_t* barrier = &control.landed[i % kStages][warp];
-                        const bool any = token < a.tables.tokens;  // if not, the barrier still turns
+                        const uint32_t token = work.first + warp * 2 * Length;
+                        const bool any = warp * 2 * Length < work.count;  // if not, the barrier still turns
                         expect_bytes(barrier, any ? 2 * Length * S::kRow : 0);
                         if (any) {
-                            load_tile(stage_x(i, 2 * warp), &a.drive_map, work.y * kColumns, token, barrier);
+                            load_tile(stage_x(i, 2 * warp), &a.drive_map, group * kColumns, token, barrier);
                             if constexpr (Backward)
-                                load_tile(stage_s(i, 2 * warp), &a.grad_map, work.y * kColumns, token, barrier);
+                                load_tile(stage_s(i, 2 * warp), &a.grad_map, group * kColumns, token, barrier);
                             if constexpr (!Shared)
-                                load_tile(stage_a(i, 2 * warp), &a.decay_map, work.y * kColumns, token, barrier);
+                                load_tile(stage_a(i, 2 * warp), &a.decay_map, group * kColumns, token, barrier);
                         }
                     }
                 } else {
-                    const Columns<Unit> col(work.y, a.channels);
-                    const int count = first < a.tables.tokens ? (int)min(a.tables.tokens - first, (uint32_t)Length) : 0;
+                    const Columns<Unit> col(group, a.channels);
                     const T* x = static_cast<const T*>(a.drive) + (int64_t)first * a.drive_stride + col.c;
                     const T* s = static_cast<const T*>(a.grad_states) + (int64_t)first * a.grad_states_stride + col.c;
                     const G* g = static_cast<const G*>(a.decay) + (int64_t)first * a.decay_stride + col.c;
@@ -613,7 +633,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
                 }
             }
             if constexpr (!Tiled) asm volatile("cp.async.commit_group;" ::: "memory");
-            return word;
+            return bits;
         };
         // Waits for the loads of tile i, those of tile i + 1 being issued.
         const auto landed = [&](uint32_t i) {
@@ -623,11 +643,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
                 asm volatile("cp.async.wait_group 1;" ::: "memory");
             }
         };
-        const auto map = [&](uint32_t i, uint4 word) {
-            const uint2 work = work_at(i);
+        const auto map = [&](uint32_t i, const StoryBits& bits) {
+            const Work& work = work_at(i);
             landed(i);
-            const Columns<Unit> col(work.y, a.channels);
-            const Segment s = segment_of<Length>(a.tables, word, work.x * kTile + segment * Length);
+            const Columns<Unit> col(work.group, a.channels);
+            const Segment s = segment_of(bits, work.first + segment * Length, tokens_of(work));
             const T* x = stage_x(i, segment);
             const T* sp = stage_s(i, segment);
             const G* ap = stage_a(i, segment);
@@ -685,11 +705,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
             if ((lane & 15u) == 0) m.starts[segment] = s.starts != 0, m.ends[segment] = s.ends != 0;
             arrive_at<1>(i & 1u);
         };
-        const auto write = [&](uint32_t i, uint4 word) {
-            const uint2 work = work_at(i);
-            const Columns<Unit> col(work.y, a.channels);
-            const uint32_t first = work.x * kTile + segment * Length;
-            const Segment s = segment_of<Length>(a.tables, word, first);
+        const auto write = [&](uint32_t i, const StoryBits& bits) {
+            const Work& work = work_at(i);
+            const Columns<Unit> col(work.group, a.channels);
+            const uint32_t first = work.first + segment * Length;
+            const Segment s = segment_of(bits, first, tokens_of(work));
             const T* x = stage_x(i, segment);
             const T* sp = stage_s(i, segment);
             const G* ap = stage_a(i, segment);
@@ -761,15 +781,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
             }
         };
 
-        uint4 word0 = issue(0), word1 = issue(1);
-        if (work_at(0).x != kNone) map(0, word0);
-        for (uint32_t i = 0; work_at(i).x != kNone; ++i) {
-            const uint4 word2 = issue(i + 2);
-            if (work_at(i + 1).x != kNone) map(i + 1, word1);
+        StoryBits bits0 = issue(0), bits1 = issue(1);
+        if (work_at(0).count != kNone) map(0, bits0);
+        for (uint32_t i = 0; work_at(i).count != kNone; ++i) {
+            const StoryBits bits2 = issue(i + 2);
+            if (work_at(i + 1).count != kNone) map(i + 1, bits1);
             sync_of<3>(i & 1u);
-            write(i, word0);
-            word0 = word1;
-            word1 = word2;
+            write(i, bits0);
+            bits0 = bits1;
+            bits1 = bits2;
         }
         if constexpr (Backward && Shared) arrive_at<1>(0);  // the last sums are written
     } else {
@@ -780,7 +800,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
         constexpr int kHalf = kSegments / 2;
         const uint32_t lane = threadIdx.x & 31u, half = lane >> 4, k = (warp - kWarps) * 16 + (lane & 15u);
         const bool leader = threadIdx.x == 32 * kWarps;
-        const auto add_sums = [&](uint32_t i, uint2 work) {
+        const auto add_sums = [&](uint32_t i, uint2 work) {  // (tile, group)
             const uint32_t c = work.y * kColumns + k;
             float sum = 0.0f;
 #pragma unroll
@@ -794,21 +814,38 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
         (void)add_sums;
         uint32_t i = 0;
         uint2 before1 = make_uint2(kNone, 0), before2 = before1;  // the last two tiles
-        uint32_t end = Lookback<Direction>::end_of(a, work_at(0).x, kWordsATile);
+        const auto draw = [&] {
+            uint32_t t = kNone - 1u;
+            if (leader && !one_each)
+                asm volatile("atom.relaxed.gpu.global.add.u32 %0, [%1], 1;" : "=r"(t) : "l"(a.scratch.ticket) : "memory");
+            return t;
+        };
+        // What comes from memory is asked for a turn before it is used: the slots and the kept state of the
+        // next tile, the schedule's entry of a ticket, the ticket after that.
+        uint32_t drawn = draw();  // for turn 3
+        Lookback<Direction> back(work_at(0).tile, work_at(0).holder);
+        Slot slots[8] = {};
+        float kept = 0.0f;
+        const auto ask = [&](const Work& work, const Lookback<Direction>& back, Slot (&s)[8], float& kept) {
+            const uint32_t c = work.group * kColumns + k;
+            if (work.count == kNone || c >= a.channels) return;
+            if (back.maps >= 0) back.load(a.scratch.slots, a.channels, c, (int)half, s);
+            if (Backward && work.count > 0) kept = __ldcs(a.carries + (size_t)work.kept * a.channels + c);
+        };
+        ask(work_at(0), back, slots, kept);
         for (;; ++i) {
-            const uint2 work = work_at(i);
-            const uint32_t tile = work.x, c = work.y * kColumns + k;
-            if (tile == kNone) break;
-            // For later turns: a ticket, whose loads are issued in the next one, and the next tile's table entry.
-            uint32_t later = total;
-            if (leader && !one_each) later = atomicAdd(a.scratch.ticket, 1u) + 1u;
-            const uint32_t next_end = Lookback<Direction>::end_of(a, work_at(i + 1).x, kWordsATile);
+            const Work work = work_at(i);
+            if (work.count == kNone) break;
+            const uint32_t tile = work.tile, c = work.group * kColumns + k;
             const bool active = c < a.channels;
-            float kept = 0.0f;
-            if (Backward && active && a.tables.tokens > 0)
-                kept = __ldcs(a.carries + (size_t)tile * (kTile / kKept) * a.channels + c);
-            const Lookback<Direction> back(a, tile, end, kWordsATile);
-            end = next_end;
+            const uint32_t drawn_next = draw(), ticket = drawn + 1u, place = min(ticket / a.groups, a.tiles - 1u);
+            const uint4* entry = reinterpret_cast<const uint4*>(a.schedule + place);
+            uint4 entry_x = make_uint4(0, 0, 0, 0), entry_y = entry_x;
+            if (leader) entry_x = __ldg(entry), entry_y = __ldg(entry + 1);
+            Lookback<Direction> back_next(work_at(i + 1).tile, work_at(i + 1).holder);
+            Slot slots_next[8] = {};
+            float kept_next = 0.0f;
+            ask(work_at(i + 1), back_next, slots_next, kept_next);
             sync_of<1>(i & 1u);
             typename S::Maps& m = control.maps[i & 1u];
             if constexpr (Backward && Shared)
@@ -843,22 +880,24 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
             const float far_A = value_of(half ? product : other), far_sum = half ? sum : other_sum;
             const float tile_A = value_of(product_of(product, other));
             const float tile_sum = far_cut ? far_sum : fmaf(far_A, near_sum, far_sum);
-            const bool last = Backward ? tile == 0 : tile + 1 == a.tiles;
             const bool state_tile = Backward ? tile % kGroup == 0 : (tile + 1) % kGroup == 0;
-            const bool writes = active && !last && half == 0;
+            const bool writes = active && work.onward && half == 0;
             Slot* mine = a.scratch.slots + (size_t)tile * a.channels + c;
             if (writes && (cuts || !state_tile)) write_slot(mine, tile_A, tile_sum);
 
             float carry = 0.0f;
             if (back.maps >= 0) {
                 float A, H;
-                for (uint32_t n = 0;; ++n) {
-                    const bool there = !active || back.read(a.scratch.slots, a.channels, c, (int)half, A, H);
-                    if (__all_sync(kNone, there)) break;
+                bool there = back.compose(slots, (int)half, A, H) || !active;
+                for (uint32_t n = 0; !__all_sync(kNone, there); ++n) {
                     if (n >= kSpinLimit) {
                         if (lane == 0) atomicExch(&g_gave_up, 1u);
                         A = H = CUDART_NAN_F;
                         break;
+                    }
+                    if (active) {
+                        back.load(a.scratch.slots, a.channels, c, (int)half, slots);
+                        there = back.compose(slots, (int)half, A, H);
                     }
                 }
                 const float other_A = __shfl_xor_sync(kNone, A, 16), other_H = __shfl_xor_sync(kNone, H, 16);
@@ -886,9 +925,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
                     m.M[w][k] = before;
                 } else {
                     m.H[w][k] = before;
-                    if (a.carries && active && w % (kKept / Length) == 0 &&
-                        tile * kTile + (uint32_t)w * Length < a.tables.tokens)
-                        a.carries[((size_t)tile * (kTile / kKept) + w / (kKept / Length)) * a.channels + c] = before;
+                    if (a.carries && active && w % (kKept / Length) == 0 && (uint32_t)w * Length < work.count)
+                        a.carries[(size_t)(work.kept + w / (kKept / Length)) * a.channels + c] = before;
                 }
                 before = cut_at(j) ? v[j] : fmaf(A[j], before, v[j]);
             }
@@ -917,7 +955,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
                     at = start_at(j) ? h[j] : fmaf(A[kHalf - 1 - j], at, h[j]);
                 }
             }
-            if (leader) control.ring[(i + 3) & 7u] = work_of(later);
+            if (leader) {
+                const bool any = !one_each && ticket < total;
+                control.ring[(i + 3) & 7u] = Work{entry_x.x, any ? entry_x.y : kNone, entry_x.z, ticket - place * a.groups,
+                                                  entry_y.x, entry_x.w, entry_y.y, 0};
+            }
             arrive_at<3>(i & 1u);
             if (tile == 0 && a.tables.full < a.tables.stories && half == 0) {
                 if constexpr (!Backward)
@@ -926,7 +968,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
                     copy_empty(a.tables, a.channels, c, a.grad_final, a.grad_initial);
             }
             before2 = before1;
-            before1 = work;
+            before1 = make_uint2(tile, work.group);
+            drawn = drawn_next;
+            back = back_next;
+            kept = kept_next;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) slots[j] = slots_next[j];
         }
         if constexpr (Backward && Shared) {
             sync_of<1>(0);
@@ -991,15 +1038,15 @@ void check_tables(const LeoB200StoryTables* t, uint32_t channels) {
     require(t->stories > 0, "a batch needs at least one story");
     require(t->tokens < (1u << 31), "too many tokens for one scan");
     require(t->full <= t->stories && (t->full > 0) == (t->tokens > 0), "story tables are inconsistent");
-    require(t->order != nullptr && (t->tokens == 0 || t->words != nullptr), "story tables are null");
+    require(t->words && t->order && t->schedule[0][0] && t->schedule[0][1] && t->schedule[1][0] && t->schedule[1][1],
+            "story tables are null");
+    require(t->tiles[0] > 0 && t->tiles[1] >= t->tiles[0], "story tables are inconsistent");
     require(channels > 0 && channels < (1u << 31), "channels must be positive");
 }
 
-uint32_t tiles_of(uint32_t tokens, uint32_t length) { return tokens == 0 ? 1 : (tokens - 1) / length + 1; }
-
 // The parts of a call's scratch, for the shortest tiles; returns its size.
-size_t lay_out(uint32_t tokens, uint32_t channels, void* base, Scratch* s) {
-    const size_t tiles = tiles_of(tokens, kKept);
+size_t lay_out(const LeoB200StoryTables& t, uint32_t channels, void* base, Scratch* s) {
+    const size_t tiles = t.tiles[1];
     if (tiles == 1) return 0;  // nothing crosses tiles
     const size_t slots = 256, partials = slots + tiles * channels * sizeof(Slot);
     if (s) {
@@ -1009,6 +1056,96 @@ size_t lay_out(uint32_t tokens, uint32_t channels, void* base, Scratch* s) {
         s->partials = reinterpret_cast<float*>(p + partials);
     }
     return partials + tiles * channels * sizeof(float);
+}
+
+// Where the parts of a story table lie, in bytes.
+struct TableLayout {
+    size_t words, order, schedule[2][2], size;
+    TableLayout(uint32_t tokens, uint32_t stories, const uint32_t (&tiles)[2]) {
+        schedule[0][0] = 0;
+        schedule[0][1] = schedule[0][0] + tiles[0] * sizeof(LeoB200StoryTile);
+        schedule[1][0] = schedule[0][1] + tiles[0] * sizeof(LeoB200StoryTile);
+        schedule[1][1] = schedule[1][0] + tiles[1] * sizeof(LeoB200StoryTile);
+        words = schedule[1][1] + tiles[1] * sizeof(LeoB200StoryTile);
+        order = words + ((size_t)tokens / LEO_B200_STORY_WORD_TOKENS + 2) * sizeof(LeoB200StoryWord);
+        size = order + stories * sizeof(uint32_t);
+    }
+};
+
+// The tiles of a batch, in the order of their tokens.  A story that does not
+// fit the rest of the tile before it begins a tile of its own, so that only
+// the tiles of one story depend on one another; short stories share one.
+std::vector<LeoB200StoryTile> cut(const uint64_t* offsets, uint32_t stories) {
+    std::vector<LeoB200StoryTile> tiles;
+    for (uint32_t s = 0; s < stories; ++s) {
+        const uint32_t begin = (uint32_t)offsets[s], length = (uint32_t)(offsets[s + 1] - offsets[s]);
+        if (length == 0) continue;
+        if (!tiles.empty() && tiles.back().count + length <= LEO_B200_TILE_TOKENS) {
+            tiles.back().count += length;
+            continue;
+        }
+        for (uint32_t at = 0; at < length; at += LEO_B200_TILE_TOKENS) {
+            LeoB200StoryTile t{};
+            t.first = begin + at;
+            t.count = std::min(length - at, LEO_B200_TILE_TOKENS);
+            tiles.push_back(t);
+        }
+    }
+    if (tiles.empty()) tiles.push_back({});  // a batch without tokens
+    return tiles;
+}
+
+// Numbers the tiles and finds, for every one, the tiles where the stories that
+// cross its ends begin and end.  `starts(t)`: a story starts at token t (the
+// batch's end counts as one).
+template <typename Starts>
+void link(std::vector<LeoB200StoryTile>& tiles, std::vector<uint32_t>& begins, std::vector<uint32_t>& ends,
+          Starts&& starts) {
+    const uint32_t n = (uint32_t)tiles.size();
+    begins.resize(n);
+    ends.resize(n);
+    const auto starts_in = [&](const LeoB200StoryTile& t) {  // after its first token too
+        for (uint32_t i = 0; i < t.count; ++i)
+            if (starts(t.first + i)) return true;
+        return false;
+    };
+    for (uint32_t i = 0; i < n; ++i) {
+        tiles[i].tile = i;
+        const bool crossed = i > 0 && !starts(tiles[i].first);
+        // the story that crosses in began in the tile before, or crossed into that one too
+        begins[i] = !crossed ? i : starts_in(tiles[i - 1]) ? i - 1 : begins[i - 1];
+    }
+    for (uint32_t i = n; i-- > 0;) {
+        const bool crossed = i + 1 < n && !starts(tiles[i + 1].first);
+        const auto ends_in = [&](const LeoB200StoryTile& t) {
+            for (uint32_t k = 0; k < t.count; ++k)
+                if (starts(t.first + k + 1)) return true;
+            return false;
+        };
+        ends[i] = !crossed ? i : ends_in(tiles[i + 1]) ? i + 1 : ends[i + 1];
+    }
+}
+
+// The tiles in the order of their tickets: by their distance from `holders`,
+// so that a tile follows every tile it reads from.
+void schedule(const std::vector<LeoB200StoryTile>& tiles, const std::vector<uint32_t>& holders,
+              const std::vector<uint32_t>& onward, LeoB200StoryTile* out, bool backward) {
+    const uint32_t n = (uint32_t)tiles.size();
+    std::vector<uint32_t> rank(n), first;
+    for (uint32_t k = 0; k < n; ++k) {
+        const uint32_t i = backward ? n - 1 - k : k;
+        rank[i] = holders[i] == i ? 0 : rank[backward ? i + 1 : i - 1] + 1;
+        if (rank[i] + 2 > first.size()) first.resize(rank[i] + 2, 0);
+        ++first[rank[i] + 1];
+    }
+    for (size_t r = 1; r < first.size(); ++r) first[r] += first[r - 1];
+    for (uint32_t k = 0; k < n; ++k) {
+        const uint32_t i = backward ? n - 1 - k : k;
+        LeoB200StoryTile& t = out[first[rank[i]]++];
+        t = tiles[i];
+        t.holder = holders[i];
+        t.onward = onward[i] != i;
+    }
 }
 
 // Neighbours of a row that can be moved at once, going by its address and stride.
@@ -1053,13 +1190,15 @@ void describe(CUtensorMap* map, const void* p, int64_t stride, uint32_t tokens, 
 template <typename T, typename G, int Unit, bool Shared, bool Backward>
 void launch_scan(ScanArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
     using S = Shape<T, G, Shared, Backward>;
-    static_assert(S::kBytes <= kSharedLimit && S::kTile % kKept == 0 && kKept % S::kSegment == 0, "shape");
-    static_assert(LEO_B200_STORY_WORD_TOKENS % S::kSegment == 0, "a segment lies in one story word");
-    a.tiles = tiles_of(a.tables.tokens, S::kTile);
+    static_assert(S::kBytes <= kSharedLimit && kKept % S::kSegment == 0, "shape");
+    static_assert(S::kTile == LEO_B200_TILE_TOKENS || S::kTile == LEO_B200_TILE_TOKENS / 2, "tiles of the story table");
+    constexpr int halves = S::kTile < LEO_B200_TILE_TOKENS;
+    a.tiles = a.tables.tiles[halves];
+    a.schedule = a.tables.schedule[halves][Backward];
     a.groups = (a.channels + kColumns - 1) / kColumns;
     const uint64_t total = (uint64_t)a.tiles * a.groups;
     require(total < (1ull << 31) - 65536, "too many tokens and channels for one scan");
-    const size_t size = lay_out(a.tables.tokens, a.channels, workspace, &a.scratch);
+    const size_t size = lay_out(a.tables, a.channels, workspace, &a.scratch);
     if (size > 0) {
         require(workspace != nullptr && workspace_bytes >= size, "the workspace is too small");
         require(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "the workspace must be aligned to 16 bytes");
@@ -1105,46 +1244,100 @@ int unit_of_call(uint32_t channels, uint32_t tokens, int64_t stride0, int64_t st
 
 extern "C" {
 
-int leo_b200_story_table(const uint64_t* offsets, uint32_t stories, LeoB200StoryWord* words, uint32_t* order,
-                         uint32_t* full) {
-    return guarded([&] {
-        require(offsets != nullptr && order != nullptr && full != nullptr, "story table arrays are null");
-        require(stories > 0, "a batch needs at least one story");
+size_t leo_b200_story_table_bytes(const uint64_t* offsets, uint32_t stories) {
+    size_t bytes = 0;
+    guarded([&] {
+        require(offsets != nullptr && stories > 0, "a batch needs at least one story");
         require(offsets[0] == 0, "story offsets must start at 0");
         for (uint32_t s = 0; s < stories; ++s)
             require(offsets[s + 1] >= offsets[s], "story offsets must be non-decreasing");
         require(offsets[stories] < (1ull << 31), "too many tokens for one batch");
+        uint32_t tiles[2] = {0, 0};
+        for (const LeoB200StoryTile& t : cut(offsets, stories)) {
+            ++tiles[0];
+            tiles[1] += t.count > LEO_B200_TILE_TOKENS / 2 ? 2 : 1;
+        }
+        bytes = TableLayout((uint32_t)offsets[stories], stories, tiles).size;
+    });
+    return bytes;
+}
+
+int leo_b200_story_table(const uint64_t* offsets, uint32_t stories, void* table, size_t bytes, const void* device_table,
+                         LeoB200StoryTables* out) {
+    return guarded([&] {
+        const size_t needed = leo_b200_story_table_bytes(offsets, stories);
+        if (needed == 0) throw Failure(leo_b200_last_error());
+        require(table != nullptr && out != nullptr, "story table arrays are null");
+        require(bytes >= needed, "the story table is too small");
+        require(reinterpret_cast<uintptr_t>(table) % 16 == 0 && reinterpret_cast<uintptr_t>(device_table) % 16 == 0,
+                "the story table must be aligned to 16 bytes");
         const uint32_t tokens = (uint32_t)offsets[stories];
-        require(tokens == 0 || words != nullptr, "story table arrays are null");
+        // Whole tiles, and their halves; a state is kept before each half.
+        std::vector<LeoB200StoryTile> whole = cut(offsets, stories), halves;
+        for (LeoB200StoryTile& t : whole) {
+            t.kept = (uint32_t)halves.size();
+            for (uint32_t at = 0; at == 0 || at < t.count; at += LEO_B200_TILE_TOKENS / 2) {
+                LeoB200StoryTile h = t;
+                h.first += at;
+                h.count = std::min(t.count - at, LEO_B200_TILE_TOKENS / 2);
+                h.kept = (uint32_t)halves.size();
+                halves.push_back(h);
+            }
+        }
+        const uint32_t tiles[2] = {(uint32_t)whole.size(), (uint32_t)halves.size()};
+        const TableLayout at(tokens, stories, tiles);
+        std::memset(table, 0, at.size);
+        char* base = static_cast<char*>(table);
+        auto* words = reinterpret_cast<LeoB200StoryWord*>(base + at.words);
+        auto* order = reinterpret_cast<uint32_t*>(base + at.order);
         uint32_t n = 0;
         for (uint32_t s = 0; s < stories; ++s)
-            if (offsets[s + 1] > offsets[s]) order[n++] = s;
-        *full = n;
-        for (uint32_t s = 0, e = n; s < stories; ++s)
-            if (offsets[s + 1] == offsets[s]) order[e++] = s;
-        uint32_t next = 0;  // the next story of the order that has not started
-        for (uint64_t first = 0, w = 0; first < tokens; first += LEO_B200_STORY_WORD_TOKENS, ++w) {
-            LeoB200StoryWord& word = words[w];
-            const uint64_t past = std::min<uint64_t>(first + LEO_B200_STORY_WORD_TOKENS, tokens);
-            word.starts = 0;
-            word.rank = next;
-            while (next < n && offsets[order[next]] < past) {
-                word.starts |= 1u << (offsets[order[next]] - first);
-                ++next;
+            if (offsets[s + 1] > offsets[s]) {
+                words[offsets[s] / LEO_B200_STORY_WORD_TOKENS].starts |= 1u << offsets[s] % LEO_B200_STORY_WORD_TOKENS;
+                order[n++] = s;
             }
-            const uint32_t holder = (word.starts & 1u) ? word.rank : word.rank - 1;
-            word.begin = (uint32_t)offsets[order[holder]];
-            word.end = (uint32_t)offsets[order[next - 1] + 1];
+        const uint32_t full = n;
+        for (uint32_t s = 0; s < stories; ++s)
+            if (offsets[s + 1] == offsets[s]) order[n++] = s;
+        words[tokens / LEO_B200_STORY_WORD_TOKENS].starts |= 1u << tokens % LEO_B200_STORY_WORD_TOKENS;
+        uint32_t rank = 0;
+        for (size_t w = 0; w < (size_t)tokens / LEO_B200_STORY_WORD_TOKENS + 2; ++w) {
+            words[w].rank = rank;
+            for (uint32_t b = words[w].starts; b; b &= b - 1) ++rank;
         }
+        const auto starts = [&](uint32_t t) {
+            return (words[t / LEO_B200_STORY_WORD_TOKENS].starts >> t % LEO_B200_STORY_WORD_TOKENS & 1u) != 0;
+        };
+        for (int k = 0; k < 2; ++k) {
+            std::vector<LeoB200StoryTile>& list = k ? halves : whole;
+            std::vector<uint32_t> begins, ends;
+            link(list, begins, ends, starts);
+            for (int d = 0; d < 2; ++d)
+                schedule(list, d ? ends : begins, d ? begins : ends,
+                         reinterpret_cast<LeoB200StoryTile*>(base + at.schedule[k][d]), d != 0);
+        }
+        const char* device = static_cast<const char*>(device_table);
+        LeoB200StoryTables t{};
+        t.words = reinterpret_cast<const LeoB200StoryWord*>(device + at.words);
+        t.order = reinterpret_cast<const uint32_t*>(device + at.order);
+        for (int k = 0; k < 2; ++k) {
+            t.tiles[k] = tiles[k];
+            for (int d = 0; d < 2; ++d)
+                t.schedule[k][d] = reinterpret_cast<const LeoB200StoryTile*>(device + at.schedule[k][d]);
+        }
+        t.tokens = tokens;
+        t.stories = stories;
+        t.full = full;
+        *out = t;
     });
 }
 
-size_t leo_b200_gated_scan_workspace(uint32_t tokens, uint32_t channels) {
-    return lay_out(tokens, channels, nullptr, nullptr);
+size_t leo_b200_gated_scan_workspace(const LeoB200StoryTables* tables, uint32_t channels) {
+    return tables ? lay_out(*tables, channels, nullptr, nullptr) : 0;
 }
 
-size_t leo_b200_gated_scan_carry_count(uint32_t tokens, uint32_t channels) {
-    return (size_t)tiles_of(tokens, kKept) * channels;
+size_t leo_b200_gated_scan_carry_count(const LeoB200StoryTables* tables, uint32_t channels) {
+    return tables ? (size_t)tables->tiles[1] * channels : 0;
 }
 
 int leo_b200_gated_scan(int device, const LeoB200StoryTables* tables, uint32_t channels, int dtype,

@@ -283,13 +283,27 @@ F32, BF16, F16 = 0, 1, 2
 
 
 class LeoB200StoryWord(C.Structure):
-    _fields_ = [("starts", C.c_uint32), ("rank", C.c_uint32), ("begin", C.c_uint32), ("end", C.c_uint32)]
+    _fields_ = [("starts", C.c_uint32), ("rank", C.c_uint32)]
+
+
+class LeoB200StoryTile(C.Structure):
+    _fields_ = [
+        ("first", C.c_uint32),
+        ("count", C.c_uint32),
+        ("tile", C.c_uint32),
+        ("kept", C.c_uint32),
+        ("holder", C.c_uint32),
+        ("onward", C.c_uint32),
+        ("unused", C.c_uint32 * 2),
+    ]
 
 
 class LeoB200StoryTables(C.Structure):
     _fields_ = [
         ("words", C.c_void_p),
         ("order", C.c_void_p),
+        ("schedule", (C.c_void_p * 2) * 2),
+        ("tiles", C.c_uint32 * 2),
         ("tokens", C.c_uint32),
         ("stories", C.c_uint32),
         ("full", C.c_uint32),

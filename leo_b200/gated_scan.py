@@ -28,7 +28,7 @@ import numpy as np
 import torch
 
 from . import native
-from .ctypes_types import LeoB200StoryTables, LeoB200StoryWord
+from .ctypes_types import LeoB200StoryTables
 from .device_tensors import check_contiguous, check_tensor, dtype_code, on_stream, pointer, row_stride
 
 
@@ -49,24 +49,32 @@ class StoryLayout:
         if device.type != "cuda":
             raise ValueError("a story layout lives on a CUDA device")
         stories = offsets.size - 1
-        words = np.zeros((min(int(offsets[-1]), 2**31) + 31) // 32 * 4, dtype=np.uint32)
-        order = np.zeros(stories, dtype=np.uint32)
-        full = C.c_uint32()
-        native.check(native.lib().leo_b200_story_table(offsets.ctypes.data, stories, words.ctypes.data,
-                                                        order.ctypes.data, C.byref(full)))
+        L = native.lib()
+        size = L.leo_b200_story_table_bytes(offsets.ctypes.data, stories)
+        native.check(0 if size else -1)
         if device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
         self.device = device
         self.stories = stories
         self.tokens = int(offsets[-1])
-        tables = np.concatenate([words, order]).view(np.int32)
-        self._tables = torch.from_numpy(tables).to(device)  # waits for the copy
-        base = self._tables.data_ptr()
-        self._c = LeoB200StoryTables(base, base + words.nbytes, self.tokens, stories, full.value)
+        host = torch.empty(size, dtype=torch.uint8)
+        self._table = torch.empty(size, dtype=torch.uint8, device=device)
+        self._c = LeoB200StoryTables()
         self._ref = C.byref(self._c)
+        native.check(L.leo_b200_story_table(offsets.ctypes.data, stories, host.data_ptr(), size,
+                                            self._table.data_ptr(), self._ref))
+        self._table.copy_(host)  # waits for the copy
+        # (scratch bytes, carries) by channels: what every call asks for
+        self._sizes: dict[int, tuple[int, int]] = {}
 
-
-assert C.sizeof(LeoB200StoryWord) == 16
+    def _needs(self, channels: int) -> tuple[int, int]:
+        needs = self._sizes.get(channels)
+        if needs is None:
+            L = native.lib()
+            needs = (L.leo_b200_gated_scan_workspace(self._ref, channels),
+                     L.leo_b200_gated_scan_carry_count(self._ref, channels))
+            self._sizes[channels] = needs
+        return needs
 
 
 class GatedScan(NamedTuple):
@@ -130,14 +138,13 @@ def gated_scan(drive, decay, layout: StoryLayout, initial=None, keep_carries: bo
     code, stride, (decay_code, decay_stride, shared) = _check_scan(drive, decay, layout, initial)
     tokens, channels = drive.shape
     L = native.lib()
+    size, kept = layout._needs(channels)
     with on_stream(drive.device, stream, (drive, decay, initial)) as raw:
         states = torch.empty((tokens, channels), dtype=drive.dtype, device=drive.device)
         final = torch.empty((layout.stories, channels), dtype=torch.float32, device=drive.device)
         carries = None
         if keep_carries:
-            carries = torch.empty(L.leo_b200_gated_scan_carry_count(tokens, channels), dtype=torch.float32,
-                                  device=drive.device)
-        size = L.leo_b200_gated_scan_workspace(tokens, channels)
+            carries = torch.empty(kept, dtype=torch.float32, device=drive.device)
         scratch = torch.empty(size, dtype=torch.uint8, device=drive.device) if size else None
         native.check(L.leo_b200_gated_scan(
             drive.device.index, layout._ref, channels, code, drive.data_ptr(), stride, decay_code, decay.data_ptr(),
@@ -164,7 +171,8 @@ def gated_scan_backward(grad_states, drive, decay, layout: StoryLayout, carries,
     L = native.lib()
     if carries is None:
         raise ValueError("the backward pass needs the carries of gated_scan(..., keep_carries=True)")
-    check_tensor("carries", carries, device, torch.float32, (L.leo_b200_gated_scan_carry_count(tokens, channels),))
+    size, kept = layout._needs(channels)
+    check_tensor("carries", carries, device, torch.float32, (kept,))
     check_contiguous("carries", carries)
     with on_stream(device, stream, (grad_states, drive, decay, carries, initial, grad_final)) as raw:
         grad_drive = torch.empty((tokens, channels), dtype=drive.dtype, device=device)
@@ -172,7 +180,6 @@ def gated_scan_backward(grad_states, drive, decay, layout: StoryLayout, carries,
         grad_initial = None
         if initial is not None:
             grad_initial = torch.empty((layout.stories, channels), dtype=torch.float32, device=device)
-        size = L.leo_b200_gated_scan_workspace(tokens, channels)
         scratch = torch.empty(size, dtype=torch.uint8, device=device) if size else None
         native.check(L.leo_b200_gated_scan_backward(
             device.index, layout._ref, channels, code, grad_states.data_ptr(), grad_stride, drive.data_ptr(), stride,

@@ -112,10 +112,12 @@ def lib() -> C.CDLL:
     L.leo_b200_synchronize_packed_model.argtypes = [vp, P(LeoB200PackedUpdate)]
     L.leo_b200_commit_packed_host_model.argtypes = [vp, P(LeoB200PackedUpdate)]
     i32, i64, f32 = C.c_int, C.c_int64, C.c_float
-    L.leo_b200_story_table.argtypes = [vp, u32, vp, vp, P(u32)]
-    L.leo_b200_gated_scan_workspace.argtypes = [u32, u32]
+    L.leo_b200_story_table_bytes.argtypes = [vp, u32]
+    L.leo_b200_story_table_bytes.restype = sz
+    L.leo_b200_story_table.argtypes = [vp, u32, vp, sz, vp, P(LeoB200StoryTables)]
+    L.leo_b200_gated_scan_workspace.argtypes = [P(LeoB200StoryTables), u32]
     L.leo_b200_gated_scan_workspace.restype = sz
-    L.leo_b200_gated_scan_carry_count.argtypes = [u32, u32]
+    L.leo_b200_gated_scan_carry_count.argtypes = [P(LeoB200StoryTables), u32]
     L.leo_b200_gated_scan_carry_count.restype = sz
     L.leo_b200_gated_scan.argtypes = [i32, P(LeoB200StoryTables), u32, i32, vp, i64, i32, vp, i64, i32, vp, vp, vp, vp,
                                       vp, sz, vp]

@@ -95,44 +95,87 @@ def close(got, want, error, what):
 
 
 def table_of(native_lib, offsets):
-    from leo_b200.ctypes_types import LeoB200StoryWord
+    """(bytes, tables) of a story table, its pointers offsets from 0."""
+    from leo_b200.ctypes_types import LeoB200StoryTables
     from leo_b200.native import check
 
     off = np.array(offsets, dtype=np.uint64)
-    words = (LeoB200StoryWord * max((offsets[-1] + 31) // 32, 1))()
-    order = np.zeros(max(len(offsets) - 1, 1), dtype=np.uint32)
-    full = C.c_uint32()
-    check(native_lib.leo_b200_story_table(off.ctypes.data, len(offsets) - 1, words, order.ctypes.data, C.byref(full)))
-    return words, order, full.value
+    size = native_lib.leo_b200_story_table_bytes(off.ctypes.data, len(offsets) - 1)
+    check(0 if size else -1)
+    host, tables = torch.empty(size, dtype=torch.uint8), LeoB200StoryTables()
+    check(native_lib.leo_b200_story_table(off.ctypes.data, len(offsets) - 1, host.data_ptr(), size, None,
+                                          C.byref(tables)))
+    return host.numpy().tobytes(), tables
 
 
-@pytest.mark.parametrize("lengths", [[1], [0], [0, 0, 7, 0], [32, 32], [31, 1, 33], [5] * 40, [100, 0, 1, 64, 0, 3]])
+@pytest.mark.parametrize("lengths", [[1], [0], [0, 0, 7, 0], [32, 32], [31, 1, 33], [5] * 40, [100, 0, 1, 64, 0, 3],
+                                     [128, 1], [129, 0, 300], [40, 2000, 7, 700, 128, 65, 64, 1], [5000]])
 def test_story_table(native_lib, lengths):
+    """Starts and ranks of the tokens; tiles that cover them once; every tile behind those that it reads from."""
+    from leo_b200.ctypes_types import LeoB200StoryTile
+
     offsets = offsets_of(lengths)
-    words, order, full = table_of(native_lib, offsets)
+    tokens = offsets[-1]
+    raw, t = table_of(native_lib, offsets)
     with_tokens = [s for s, n in enumerate(lengths) if n]
-    assert full == len(with_tokens)
+    assert (t.tokens, t.stories, t.full) == (tokens, len(lengths), len(with_tokens))
+    order = np.frombuffer(raw, np.uint32, len(lengths), t.order or 0)
     assert order.tolist() == with_tokens + [s for s, n in enumerate(lengths) if not n]
-    story = [s for s, n in enumerate(lengths) for _ in range(n)]
-    for w in range((offsets[-1] + 31) // 32):
-        tokens = range(32 * w, min(32 * w + 32, offsets[-1]))
-        assert words[w].starts == sum(1 << (t % 32) for t in tokens if t in offsets)
-        assert words[w].rank == sum(1 for s in with_tokens if offsets[s] < 32 * w)
-        assert words[w].begin == offsets[story[tokens[0]]]
-        assert words[w].end == offsets[story[tokens[-1]] + 1]
+    words = np.frombuffer(raw, np.uint32, 2 * (tokens // 32 + 2), t.words or 0).reshape(-1, 2)
+    begins = [offsets[s] for s in with_tokens] + [tokens]
+    for w, (starts, rank) in enumerate(words.tolist()):
+        assert starts == sum(1 << (b - 32 * w) for b in begins if b // 32 == w)
+        assert rank == sum(1 for b in begins if b < 32 * w)
+    for k, longest in enumerate((128, 64)):
+        for d in range(2):
+            listed = [LeoB200StoryTile.from_buffer_copy(raw, (t.schedule[k][d] or 0) + 32 * i)
+                      for i in range(t.tiles[k])]
+            turn = {x.tile: i for i, x in enumerate(listed)}
+            tiles = sorted(listed, key=lambda x: x.tile)
+            assert [x.tile for x in tiles] == list(range(t.tiles[k]))
+            assert [x.first for x in tiles] == [0] + np.cumsum([x.count for x in tiles]).tolist()[:-1]
+            assert sum(x.count for x in tiles) == tokens and max(x.count for x in tiles) <= longest
+            story = [i for i in range(len(begins) - 1) for _ in range(begins[i], begins[i + 1])]
+            for x in tiles if tokens else []:
+                last = x.first + x.count - 1
+                into = story[x.first] if d == 0 else story[last]
+                out = story[last] if d == 0 else story[x.first]
+                where = begins[into] if d == 0 else begins[into + 1] - 1
+                holder = next(y.tile for y in tiles if y.first <= where < y.first + y.count)
+                assert x.holder == holder
+                far = begins[out + 1] - 1 if d == 0 else begins[out]
+                assert x.onward == int(not x.first <= far <= last)
+                step = 1 if holder <= x.tile else -1
+                assert all(turn[y] < turn[x.tile] for y in range(holder, x.tile, step))
+    halves = {x.tile: x for x in (LeoB200StoryTile.from_buffer_copy(raw, (t.schedule[1][0] or 0) + 32 * i)
+                                  for i in range(t.tiles[1]))}
+    for i in range(t.tiles[0]):
+        x = LeoB200StoryTile.from_buffer_copy(raw, (t.schedule[0][0] or 0) + 32 * i)
+        assert halves[x.kept].first == x.first and halves[x.kept].kept == x.kept
+        if x.count > 64:
+            assert halves[x.kept + 1].first == x.first + 64
 
 
-@pytest.mark.parametrize("offsets", [[1, 2], [0, 5, 3], [0, 2**31]])
+@pytest.mark.parametrize("offsets", [[1, 2], [0, 5, 3], [0, 2**31], [0]])
 def test_story_table_refuses(native_lib, offsets):
     from leo_b200.native import LeoError
 
     with pytest.raises(LeoError):
-        off = np.array(offsets, dtype=np.uint64)
-        order, full = np.zeros(4, np.uint32), C.c_uint32()
-        from leo_b200.native import check
+        table_of(native_lib, offsets)
 
-        check(native_lib.leo_b200_story_table(off.ctypes.data, len(offsets) - 1, None, order.ctypes.data,
-                                              C.byref(full)))
+
+def test_story_table_refuses_bad_memory(native_lib):
+    from leo_b200.ctypes_types import LeoB200StoryTables
+
+    off = np.array([0, 500], dtype=np.uint64)
+    size = native_lib.leo_b200_story_table_bytes(off.ctypes.data, 1)
+    host, tables = torch.empty(size + 16, dtype=torch.uint8), C.byref(LeoB200StoryTables())
+    call = native_lib.leo_b200_story_table
+    assert call(off.ctypes.data, 1, host.data_ptr(), size - 1, None, tables) == -1
+    assert call(off.ctypes.data, 1, host.data_ptr() + 4, size, None, tables) == -1
+    assert call(off.ctypes.data, 1, host.data_ptr(), size, 8, tables) == -1
+    assert call(off.ctypes.data, 1, None, size, None, tables) == -1
+    assert call(off.ctypes.data, 1, host.data_ptr(), size, None, None) == -1
 
 
 @pytest.mark.parametrize("offsets", [[], [0], [[0, 1]], [0.0, 1.0], [0, -1], [1, 2], [0, 2, 1]])
@@ -163,13 +206,13 @@ def test_cpu_tensors_are_refused(native_lib):
         gated_step(x, x, x)
 
 
-@pytest.mark.parametrize("bad", ["stories", "tokens", "channels", "dtype", "decay", "null", "final"])
+@pytest.mark.parametrize("bad", ["stories", "tokens", "channels", "dtype", "decay", "null", "final", "workspace"])
 def test_entry_point_refuses_before_device_work(native_lib, bad):
     from leo_b200.ctypes_types import LeoB200StoryTables
 
     p = 256
-    t = LeoB200StoryTables(p, p, 1000, 3, 3)
-    args = dict(channels=70, dtype=1, decay_dtype=0, drive=p, final=p)
+    t = LeoB200StoryTables(p, p, ((p, p), (p, p)), (8, 16), 1000, 3, 3)
+    args = dict(channels=70, dtype=1, decay_dtype=0, drive=p, final=p)  # and no workspace
     if bad == "stories":
         t.stories = 0
     elif bad == "tokens":
