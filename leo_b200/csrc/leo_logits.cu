@@ -1,12 +1,19 @@
 // Operators on rows of logits (include/leo_b200.h): penalties, biases and
 // grammar masks; the pick of the next symbol; the cross entropy over the
-// allowed symbols with its gradient.  One thread block takes one row.
+// allowed symbols with its gradient.
+//
+// All three are bound by reading the logits once (and writing as much, except
+// the pick).  Rows start anywhere, so they are read in groups of eight symbols
+// laid so that the addresses are multiples of 16 bytes, the ends of a row one by
+// one; a row of 257 classes and the like is one warp's in the loss.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math_constants.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -16,10 +23,9 @@
 namespace {
 
 using namespace leo_operator;
+namespace cg = cooperative_groups;
 
-constexpr uint32_t kThreads = 256;
-constexpr uint32_t kWarps = kThreads / 32;
-constexpr uint32_t kChunk = 4096;  // symbols whose counts are held in shared memory at a time
+constexpr uint32_t kAll = 0xffffffffu;
 
 __device__ __forceinline__ float load(const float* p) { return *p; }
 __device__ __forceinline__ float load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
@@ -28,12 +34,90 @@ __device__ __forceinline__ void store(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void store(__half* p, float v) { *p = __float2half_rn(v); }
 
+// Eight neighbours of a row as they lie in memory.
+template <typename T> struct Eight {
+    uint4 raw[sizeof(T) / 2];
+    __device__ __forceinline__ float operator[](int i) const {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(raw);
+        if constexpr (std::is_same_v<T, float>) {
+            return __uint_as_float(w[i]);
+        } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+            return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+        } else {
+            return __half2float(__ushort_as_half((unsigned short)(w[i / 2] >> 16 * (i & 1))));
+        }
+    }
+    __device__ __forceinline__ void set(int i, float v) {  // i ascending
+        uint32_t* w = reinterpret_cast<uint32_t*>(raw);
+        if constexpr (std::is_same_v<T, float>) {
+            w[i] = __float_as_uint(v);
+        } else {
+            uint32_t bits;
+            if constexpr (std::is_same_v<T, __nv_bfloat16>)
+                bits = __bfloat16_as_ushort(__float2bfloat16_rn(v));
+            else
+                bits = __half_as_ushort(__float2half_rn(v));
+            w[i / 2] = i & 1 ? w[i / 2] | bits << 16 : bits;
+        }
+    }
+};
+
+// A row in groups of eight symbols whose addresses are multiples of 16 bytes:
+// group g holds symbols first + 8 g and on; the first and the last may be short.
+template <typename T>
+struct Row {
+    const T* p;
+    int32_t first;  // at most 0
+    uint32_t vocabulary, groups;
+    __device__ __forceinline__ Row(const T* row, uint32_t vocabulary_) : p(row), vocabulary(vocabulary_) {
+        const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(row) / sizeof(T)) % (16 / sizeof(T));
+        first = -(int32_t)off;
+        groups = (vocabulary + off + 7) / 8;
+    }
+    __device__ __forceinline__ bool whole(int32_t v) const { return v >= 0 && (uint32_t)v + 8 <= vocabulary; }
+    __device__ __forceinline__ bool in(int32_t v) const { return (uint32_t)v < vocabulary; }
+    // Symbols v .. v + 7; zero outside the row.
+    __device__ __forceinline__ Eight<T> read(int32_t v) const {
+        Eight<T> e;
+        if (whole(v)) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) e.raw[i] = __ldcs(reinterpret_cast<const uint4*>(p + v) + i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e.set(i, in(v + i) ? load(p + v + i) : 0.0f);
+        }
+        return e;
+    }
+    // The same symbols of another row: whole groups at once where it is aligned alike.
+    __device__ __forceinline__ bool alike(const T* other) const {
+        return (reinterpret_cast<uintptr_t>(other) ^ reinterpret_cast<uintptr_t>(p)) % 16 == 0;
+    }
+    __device__ __forceinline__ void write(T* out, bool aligned, int32_t v, const Eight<T>& e) const {
+        if (aligned && whole(v)) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) __stcs(reinterpret_cast<uint4*>(out + v) + i, e.raw[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (in(v + i)) store(out + v + i, e[i]);
+        }
+    }
+};
+
 // What a row of the mask table says: all symbols, none, or its words.
 struct MaskRow {
     const uint32_t* words;  // nullptr: see `open`
     bool open;
     __device__ __forceinline__ bool allows(uint32_t v) const {
         return words ? (words[v >> 5] >> (v & 31u)) & 1u : open;
+    }
+    // Bit i: symbol v + i is allowed, of those inside the row.
+    __device__ __forceinline__ uint32_t eight(int32_t v, uint32_t vocabulary) const {
+        if (!words) return open ? 0xffu : 0u;
+        const int32_t low = max(v, 0) >> 5, high = min(v + 7, (int32_t)vocabulary - 1) >> 5;
+        const uint64_t bits = (uint64_t)__ldg(words + high) << 32 | __ldg(words + low);
+        // two words of one number are the same word
+        return v < 0 ? (uint32_t)bits << -v & 0xffu : (uint32_t)((low == high ? bits & 0xffffffffu : bits) >> (v & 31)) & 0xffu;
     }
 };
 
@@ -69,26 +153,30 @@ __device__ __forceinline__ RowRules row_rules(const LeoB200LogitRules& r, uint32
     return k;
 }
 
-// Counts of the history's symbols in [first, first + span).
-__device__ void count_history(const RowRules& k, uint32_t first, uint32_t span, uint32_t* counts) {
-    for (uint32_t i = threadIdx.x; i < span; i += kThreads) counts[i] = 0;
+// Counts of the history's symbols in [first, first + Span), by the whole block.
+template <uint32_t Span>
+__device__ __forceinline__ void count_history(const RowRules& k, int32_t first, uint32_t* counts) {
+    for (uint32_t i = threadIdx.x; i < Span / 4; i += blockDim.x)
+        reinterpret_cast<uint4*>(counts)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < k.length; i += kThreads) {
-        const uint32_t v = (uint32_t)k.history[i] - first;
-        if (v < span) atomicAdd(&counts[v], 1u);
+#pragma unroll 4
+    for (uint32_t i = threadIdx.x; i < k.length; i += blockDim.x) {
+        const int32_t symbol = __ldg(k.history + i);
+        const uint32_t v = (uint32_t)(symbol - first);
+        if (symbol >= 0 && v < Span) atomicAdd(&counts[v], 1u);
     }
     __syncthreads();
 }
 
 // The penalties, the bias and the mask, every operation rounded by itself in F.
 template <typename F>
-__device__ __forceinline__ F adjusted(F z, uint32_t v, uint32_t count, const RowRules& k) {
+__device__ __forceinline__ F adjusted(F z, uint32_t count, const RowRules& k, float bias, bool allowed) {
     if (count) {
         z = z > (F)0 ? z / (F)k.repetition : z * (F)k.repetition;
         z -= (F)k.presence + (F)k.frequency * (F)count;
     }
-    if (k.bias) z += (F)k.bias[v];
-    return k.mask.allows(v) ? z : -(F)CUDART_INF;
+    if (k.bias) z += (F)bias;
+    return allowed ? z : -(F)CUDART_INF;
 }
 
 struct LogitArgs {
@@ -106,122 +194,375 @@ struct LogitArgs {
     float* log_probability;
 };
 
+// Biases of symbols v .. v + 7.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) adjust_kernel(LogitArgs a) {
-    __shared__ uint32_t counts[kChunk];
-    const uint32_t row = blockIdx.x;
-    const RowRules k = row_rules(a.rules, row);
-    const T* in = static_cast<const T*>(a.logits) + (int64_t)row * a.logits_stride;
-    T* out = static_cast<T*>(a.out) + (int64_t)row * a.out_stride;
-    for (uint32_t first = 0; first < a.vocabulary; first += kChunk) {
-        const uint32_t span = min(kChunk, a.vocabulary - first);
-        count_history(k, first, span, counts);
-        for (uint32_t i = threadIdx.x; i < span; i += kThreads)
-            store(out + first + i, adjusted(load(in + first + i), first + i, counts[i], k));
-        __syncthreads();
+__device__ __forceinline__ void read_bias(const RowRules& k, const Row<T>& row, int32_t v, float (&bias)[8]) {
+    if (!k.bias) return;
+    if (row.whole(v) && reinterpret_cast<uintptr_t>(k.bias + v) % 16 == 0) {
+        const float4 x = __ldg(reinterpret_cast<const float4*>(k.bias + v)),
+                     y = __ldg(reinterpret_cast<const float4*>(k.bias + v) + 1);
+        bias[0] = x.x, bias[1] = x.y, bias[2] = x.z, bias[3] = x.w;
+        bias[4] = y.x, bias[5] = y.y, bias[6] = y.z, bias[7] = y.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) bias[i] = row.in(v + i) ? __ldg(k.bias + v + i) : 0.0f;
     }
 }
 
-// The larger of two (value, symbol) pairs, the lower symbol of equal values.
-__device__ __forceinline__ void keep_best(double& v, uint32_t& at, double other, uint32_t other_at) {
-    if (other > v || (other == v && other_at < at)) {
-        v = other;
-        at = other_at;
+// A block takes a chunk of a row, two groups a thread, which it reads before it
+// counts the history's symbols of the chunk in shared memory: any vocabulary
+// and history fit, and the chunks of a long row run side by side.
+constexpr uint32_t kAdjustThreads = 256;
+constexpr uint32_t kAdjustGroups = 2;
+constexpr uint32_t kAdjustSpan = kAdjustThreads * kAdjustGroups * 8;
+
+template <typename T>
+__global__ void __launch_bounds__(kAdjustThreads) adjust_kernel(const __grid_constant__ LogitArgs a, uint32_t chunks) {
+    __shared__ __align__(16) uint32_t counts[kAdjustSpan];
+    const uint32_t at = blockIdx.x / chunks, chunk = blockIdx.x - at * chunks;
+    const Row<T> row(static_cast<const T*>(a.logits) + (int64_t)at * a.logits_stride, a.vocabulary);
+    T* out = static_cast<T*>(a.out) + (int64_t)at * a.out_stride;
+    const RowRules k = row_rules(a.rules, at);
+    const bool aligned = row.alike(out);
+    const int32_t first = row.first + (int32_t)(chunk * kAdjustSpan);
+    Eight<T> e[kAdjustGroups];
+    float bias[kAdjustGroups][8] = {};
+#pragma unroll
+    for (uint32_t j = 0; j < kAdjustGroups; ++j) {
+        const int32_t v = first + (int32_t)(j * blockDim.x + threadIdx.x) * 8;
+        if (v < (int32_t)a.vocabulary) {
+            e[j] = row.read(v);
+            read_bias(k, row, v, bias[j]);
+        }
+    }
+    if (k.length) count_history<kAdjustSpan>(k, first, counts);
+#pragma unroll
+    for (uint32_t j = 0; j < kAdjustGroups; ++j) {
+        const uint32_t within = (j * blockDim.x + threadIdx.x) * 8;
+        const int32_t v = first + (int32_t)within;
+        if (v >= (int32_t)a.vocabulary) continue;
+        const uint32_t ok = k.mask.eight(v, a.vocabulary);
+        uint32_t c[8] = {};
+        if (k.length) {
+            const uint4 x = *reinterpret_cast<const uint4*>(counts + within),
+                        y = *reinterpret_cast<const uint4*>(counts + within + 4);
+            c[0] = x.x, c[1] = x.y, c[2] = x.z, c[3] = x.w, c[4] = y.x, c[5] = y.y, c[6] = y.z, c[7] = y.w;
+        }
+        Eight<T> r;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r.set(i, adjusted(e[j][i], c[i], k, bias[j][i], ok >> i & 1u));
+        row.write(out, aligned, v, r);
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) pick_kernel(LogitArgs a) {
-    __shared__ uint32_t counts[kChunk];
-    __shared__ double warp_value[kWarps];
-    __shared__ uint32_t warp_at[kWarps];
-    __shared__ double running;
-    __shared__ uint32_t found, last;
-    __shared__ int bad;
-    const uint32_t row = blockIdx.x, lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
-    const RowRules k = row_rules(a.rules, row);
-    const T* in = static_cast<const T*>(a.logits) + (int64_t)row * a.logits_stride;
-    const float temperature = a.temperature ? a.temperature[row] : a.temperature_value;
-    if (threadIdx.x == 0) bad = !(temperature >= 0.0f);
-    // pass 1: the largest adjusted logit
-    double best = -CUDART_INF;
-    uint32_t best_at = 0xffffffffu;
-    for (uint32_t first = 0; first < a.vocabulary; first += kChunk) {
-        const uint32_t span = min(kChunk, a.vocabulary - first);
-        count_history(k, first, span, counts);
-        for (uint32_t i = threadIdx.x; i < span; i += kThreads) {
-            const double z = adjusted((double)load(in + first + i), first + i, counts[i], k);
-            if (z != z) bad = 1;
-            if (z > best) best = z, best_at = first + i;
-        }
-        __syncthreads();
-    }
-    for (int off = 16; off > 0; off >>= 1) {
-        const double v = __shfl_xor_sync(0xffffffffu, best, off);
-        const uint32_t at = __shfl_xor_sync(0xffffffffu, best_at, off);
-        keep_best(best, best_at, v, at);
-    }
-    if (lane == 0) warp_value[warp] = best, warp_at[warp] = best_at;
-    __syncthreads();
-    for (uint32_t w = 0; w < kWarps; ++w) keep_best(best, best_at, warp_value[w], warp_at[w]);
-    if (bad || best_at == 0xffffffffu) {
-        if (threadIdx.x == 0) {
-            a.symbols[row] = -1;
-            if (a.log_probability) a.log_probability[row] = bad ? CUDART_NAN_F : -CUDART_INF_F;
-        }
-        return;
-    }
+// exp(x) for x <= 0 after Tang's table-driven method (P. T. P. Tang, ACM TOMS
+// 15, 1989): x = (32 q + j) ln 2 / 32 + r, exp x = 2^q 2^(j/32) exp r, with a
+// Taylor polynomial of degree 6 for |r| <= ln 2 / 64 (its rest is below 2^-58)
+// and ln 2 / 32 in two parts so that r is exact to the last bits.
+__device__ const double kTwoTo[32] = {
+    0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0,
+    0x1.172b83c7d517bp+0, 0x1.1d4873168b9aap+0, 0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0,
+    0x1.306fe0a31b715p+0, 0x1.371a7373aa9cbp+0, 0x1.3dea64c123422p+0, 0x1.44e086061892dp+0,
+    0x1.4bfdad5362a27p+0, 0x1.5342b569d4f82p+0, 0x1.5ab07dd485429p+0, 0x1.6247eb03a5585p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.71f75e8ec5f74p+0, 0x1.7a11473eb0187p+0, 0x1.82589994cce13p+0,
+    0x1.8ace5422aa0dbp+0, 0x1.93737b0cdc5e5p+0, 0x1.9c49182a3f090p+0, 0x1.a5503b23e255dp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0,
+    0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0, 0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0};
+__device__ __forceinline__ double exp_down(double x, const double* two_to) {
+    if (!(x > -700.0)) return exp(x);  // subnormal results, -inf and NaN
+    const double magic = 0x1.8p52;
+    const double shifted = fma(x, 0x1.71547652b82fep+5, magic);
+    const int32_t n = __double2loint(shifted);
+    const double whole = shifted - magic;
+    double r = fma(whole, -0x1.62e42fee00000p-6, x);
+    r = fma(whole, -0x1.a39ef35793c76p-38, r);
+    double p = fma(r, 1.0 / 720.0, 1.0 / 120.0);
+    p = fma(p, r, 1.0 / 24.0);
+    p = fma(p, r, 1.0 / 6.0);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    const double scale = two_to[n & 31];
+    const double y = fma(scale, p * r, scale);
+    return __hiloint2double(__double2hiint(y) + ((n >> 5) << 20), __double2loint(y));
+}
+
+// A sum of weights exp((z - top) / heat), by its own top.
+struct Weights {
+    double top, sum;
+};
+__device__ __forceinline__ Weights no_weights() { return {-CUDART_INF, 0.0}; }
+__device__ __forceinline__ double weight_of(double z, double top, double cold, const double* two_to) {
+    return z == top ? 1.0 : z == -CUDART_INF || top == CUDART_INF ? 0.0 : exp_down((z - top) * cold, two_to);
+}
+__device__ __forceinline__ Weights both(const Weights& x, const Weights& y, double cold, const double* two_to) {
+    const double top = fmax(x.top, y.top);
+    if (top == -CUDART_INF) return no_weights();
+    return {top, x.sum * weight_of(x.top, top, cold, two_to) + y.sum * weight_of(y.top, top, cold, two_to)};
+}
+
+// What a part of a row knows: its weights, its largest logit and the lowest
+// symbol of that value, and whether a NaN is among them.
+struct Part {
+    Weights weights;
+    uint32_t best;
+    uint32_t bad;
+};
+
+// A cluster of blocks takes a row, each block a run of rounds, a warp of it
+// Steps x 32 groups of a round.  One pass over the logits gives each of these
+// stretches its weights (by its own top, so the row's is not needed first); the
+// blocks exchange theirs through distributed shared memory, which says in which
+// stretch the running sum passes u * total, and one warp walks that stretch
+// again.  Everything is in 64 bits: among 131,072 borders between symbols a
+// float32 sum would put one in a hundred draws on the wrong side.
+template <typename T, int Warps, int Steps>
+struct PickShape {
+    static constexpr uint32_t kSpan = Warps * Steps * 256;  // symbols of a round
+    static constexpr uint32_t kMaxRounds = 64;
+};
+
+template <typename T, int Warps, int Steps>
+__global__ void __launch_bounds__(32 * Warps) pick_kernel(const __grid_constant__ LogitArgs a, uint32_t rounds) {
+    using S = PickShape<T, Warps, Steps>;
+    __shared__ __align__(16) uint32_t counts[S::kSpan];
+    __shared__ double two_to[32];
+    __shared__ Weights stretches[S::kMaxRounds * Warps];
+    __shared__ Part warp_parts[Warps], mine;
+    __shared__ double warp_best[Warps], block_best;
+    __shared__ uint32_t chosen;  // stretch
+    __shared__ double before, target, row_best, row_total;
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t blocks = cluster.num_blocks(), rank = cluster.block_rank();
+    const uint32_t at = blockIdx.x / blocks, lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const Row<T> row(static_cast<const T*>(a.logits) + (int64_t)at * a.logits_stride, a.vocabulary);
+    const RowRules k = row_rules(a.rules, at);
+    const float temperature = a.temperature ? a.temperature[at] : a.temperature_value;
     const bool greedy = temperature == 0.0f;
-    const double heat = greedy ? 1.0 : (double)temperature;
-    const auto weight = [&](double z) {
-        return z == best ? 1.0 : z == -CUDART_INF ? 0.0 : exp((z - best) / heat);
+    const double heat = greedy ? 1.0 : (double)temperature, cold = 1.0 / heat;
+    for (uint32_t j = threadIdx.x; j < 32; j += 32 * Warps) two_to[j] = kTwoTo[j];
+
+    // Symbols of a group after the rules; the logits read before.
+    const auto symbols_at = [&](uint32_t round, uint32_t w, int step) {
+        return row.first + (int32_t)((rank * rounds + round) * S::kSpan + ((w * Steps + step) * 32 + lane) * 8);
     };
-    // pass 2: the sum of the weights; pass 3: where the sums in symbol order pass u * total
-    double total = 0.0, target = 0.0;
-    for (int pass = 2; pass <= (greedy ? 2 : 3); ++pass) {
-        __syncthreads();
-        if (threadIdx.x == 0) running = 0.0, found = 0xffffffffu, last = 0;
-        __syncthreads();
-        for (uint32_t first = 0; first < a.vocabulary; first += kChunk) {
-            const uint32_t span = min(kChunk, a.vocabulary - first);
-            count_history(k, first, span, counts);
-            for (uint32_t at = 0; at < span; at += kThreads) {
-                const uint32_t i = at + threadIdx.x;
-                const double w =
-                    i < span ? weight(adjusted((double)load(in + first + i), first + i, counts[i], k)) : 0.0;
-                double sum = w;
-                for (int off = 1; off < 32; off <<= 1) {
-                    const double v = __shfl_up_sync(0xffffffffu, sum, off);
-                    if (lane >= (uint32_t)off) sum += v;
-                }
-                if (lane == 31) warp_value[warp] = sum;
-                __syncthreads();
-                double before = running;
-                for (uint32_t j = 0; j < warp; ++j) before += warp_value[j];
-                if (pass == 3 && w > 0.0) {
-                    atomicMax(&last, first + i);
-                    if (before + sum > target) atomicMin(&found, first + i);
-                }
-                __syncthreads();
-                if (threadIdx.x == kThreads - 1) running = before + sum;
-                __syncthreads();
+    const auto adjust = [&](const Eight<T>& e, const float (&bias)[8], int32_t v, int32_t first, double (&z)[8]) {
+        const uint32_t ok = k.mask.eight(v, a.vocabulary);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t count = k.length ? counts[(uint32_t)(v + i - first)] : 0u;
+            z[i] = adjusted((double)e[i], count, k, bias[i], row.in(v + i) && (ok >> i & 1u));
+        }
+    };
+
+    Part part{no_weights(), kAll, !(temperature >= 0.0f)};
+    double best_value = -CUDART_INF;
+    for (uint32_t round = 0; round < rounds; ++round) {
+        const int32_t first = row.first + (int32_t)((rank * rounds + round) * S::kSpan);
+        if (first >= (int32_t)a.vocabulary) {
+            if (lane == 0) stretches[round * Warps + warp] = no_weights();
+            continue;
+        }
+        Eight<T> e[Steps];
+#pragma unroll
+        for (int step = 0; step < Steps; ++step) {
+            const int32_t v = symbols_at(round, warp, step);
+            if (v < (int32_t)a.vocabulary) e[step] = row.read(v);
+        }
+        __syncthreads();  // the table, or the counts of the round before
+        if (k.length) count_history<S::kSpan>(k, first, counts);
+        Weights w = no_weights();
+#pragma unroll
+        for (int step = 0; step < Steps; ++step) {
+            const int32_t v = symbols_at(round, warp, step);
+            if (v >= (int32_t)a.vocabulary) continue;
+            float bias[8] = {};
+            read_bias(k, row, v, bias);
+            double z[8];
+            adjust(e[step], bias, v, first, z);
+            double top = w.top;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (z[i] != z[i]) part.bad = 1;
+                if (z[i] > best_value) best_value = z[i], part.best = (uint32_t)(v + i);
+                top = fmax(top, z[i]);
             }
-            __syncthreads();
+            if (top > w.top) {
+                w.sum = w.sum * weight_of(w.top, top, cold, two_to);
+                w.top = top;
+            }
+            if (top != -CUDART_INF) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w.sum += weight_of(z[i], top, cold, two_to);
+            }
         }
-        if (pass == 2) {
-            total = running;
-            target = greedy ? 0.0 : a.uniforms[row] * total;
+        for (int off = 16; off > 0; off >>= 1) {
+            const Weights o{__shfl_xor_sync(kAll, w.top, off), __shfl_xor_sync(kAll, w.sum, off)};
+            w = both(w, o, cold, two_to);
         }
+        if (lane == 0) stretches[round * Warps + warp] = w;
+        part.weights = both(part.weights, w, cold, two_to);
     }
-    const uint32_t symbol = greedy ? best_at : found != 0xffffffffu ? found : last;
-    if (threadIdx.x == 0) a.symbols[row] = (int32_t)symbol;
-    if (!a.log_probability) return;
+    // The block's part.
+    for (int off = 16; off > 0; off >>= 1) {
+        const double v = __shfl_xor_sync(kAll, best_value, off);
+        const uint32_t b = __shfl_xor_sync(kAll, part.best, off);
+        if (v > best_value || (v == best_value && b < part.best)) best_value = v, part.best = b;
+        part.bad |= __shfl_xor_sync(kAll, part.bad, off);
+    }
+    if (lane == 0) warp_parts[warp] = part, warp_best[warp] = best_value;
     __syncthreads();
-    const uint32_t first = symbol / kChunk * kChunk;
-    count_history(k, first, min(kChunk, a.vocabulary - first), counts);
     if (threadIdx.x == 0) {
-        const double z = adjusted((double)load(in + symbol), symbol, counts[symbol - first], k);
-        a.log_probability[row] = (float)((z == best ? 0.0 : (z - best) / heat) - log(total));
+        Part p = warp_parts[0];
+        for (int w = 1; w < Warps; ++w) {
+            const Part& o = warp_parts[w];
+            if (warp_best[w] > best_value || (warp_best[w] == best_value && o.best < p.best))
+                best_value = warp_best[w], p.best = o.best;
+            p.bad |= o.bad;
+            p.weights = both(p.weights, o.weights, cold, two_to);
+        }
+        mine = p;
+        block_best = best_value;
+    }
+    if (blocks > 1)
+        cluster.sync();
+    else
+        __syncthreads();
+
+    // The row's, the same in every block.
+    if (warp == 0) {
+        Part p{no_weights(), kAll, 0};
+        double value = -CUDART_INF;
+        if (lane < blocks) {
+            p = *cluster.map_shared_rank(&mine, lane);
+            value = *cluster.map_shared_rank(&block_best, lane);
+        }
+        double top = value;
+        uint32_t best = p.best, bad = p.bad;
+        for (int off = 16; off > 0; off >>= 1) {
+            const double v = __shfl_xor_sync(kAll, top, off);
+            const uint32_t b = __shfl_xor_sync(kAll, best, off);
+            if (v > top || (v == top && b < best)) top = v, best = b;
+            bad |= __shfl_xor_sync(kAll, bad, off);
+        }
+        uint32_t pick = kAll - 1u;  // nothing to walk
+        if (!bad && best != kAll) {
+            const double share = p.weights.sum * (lane < blocks ? weight_of(p.weights.top, top, cold, two_to) : 0.0);
+            double total = 0.0;
+            for (uint32_t j = 0; j < blocks; ++j) total += __shfl_sync(kAll, share, j);
+            if (greedy) {
+                if (rank == 0 && lane == 0) {
+                    a.symbols[at] = (int32_t)best;
+                    if (a.log_probability) a.log_probability[at] = (float)-log(total);
+                }
+            } else {
+                // The block, then its stretch, in which the running sum passes u * total.
+                const double goal = a.uniforms[at] * total;
+                double sum = 0.0, sum_before = 0.0;
+                uint32_t owner = kAll, last = 0;
+                for (uint32_t j = 0; j < blocks; ++j) {
+                    const double s = __shfl_sync(kAll, share, j);
+                    if (owner == kAll && s > 0.0) {
+                        sum_before = sum;
+                        last = j;
+                        if (sum + s > goal) owner = j;
+                    }
+                    sum += s;
+                }
+                if (owner == kAll) owner = last;  // u is nearly 1, and the sums were rounded
+                if (rank == owner) {
+                    double running = sum_before, stretch_before = sum_before;
+                    uint32_t found = kAll, last_stretch = 0;
+                    for (uint32_t base = 0; base < rounds * Warps && found == kAll; base += 32) {
+                        const uint32_t j = base + lane;
+                        Weights w = no_weights();
+                        if (j < rounds * Warps) w = stretches[j];
+                        const double s = w.sum * weight_of(w.top, top, cold, two_to);
+                        for (uint32_t l = 0; l < 32 && found == kAll; ++l) {
+                            const double one = __shfl_sync(kAll, s, l);
+                            if (one > 0.0) {
+                                stretch_before = running;
+                                last_stretch = base + l;
+                                if (running + one > goal) found = base + l;
+                                running += one;
+                            }
+                        }
+                    }
+                    pick = found != kAll ? found : last_stretch;
+                    if (lane == 0) before = stretch_before, target = goal, row_best = top, row_total = total;
+                }
+            }
+        } else if (rank == 0 && lane == 0) {
+            a.symbols[at] = -1;
+            if (a.log_probability) a.log_probability[at] = bad ? CUDART_NAN_F : -CUDART_INF_F;
+        }
+        if (lane == 0) chosen = pick;
+    }
+    // No block leaves, or changes what the others read, before they have read it.
+    if (blocks > 1)
+        cluster.sync();
+    else
+        __syncthreads();
+    if (chosen == kAll - 1u) return;
+
+    // One block walks the stretch.
+    const uint32_t round = chosen / Warps, w = chosen % Warps;
+    const int32_t first = row.first + (int32_t)((rank * rounds + round) * S::kSpan);
+    if (k.length) count_history<S::kSpan>(k, first, counts);
+    if (warp != 0) return;
+    const double top = row_best, total = row_total, goal = target;
+    double running = before;
+    uint32_t symbol = kAll, last = 0;
+    double symbol_z = 0.0, last_z = 0.0;
+    for (int step = 0; step < Steps && symbol == kAll; ++step) {
+        const int32_t v = symbols_at(round, w, step);
+        double z[8], weight[8], sum = 0.0;
+        if (v < (int32_t)a.vocabulary) {
+            float bias[8] = {};
+            read_bias(k, row, v, bias);
+            adjust(row.read(v), bias, v, first, z);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) z[i] = -CUDART_INF;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            weight[i] = weight_of(z[i], top, cold, two_to);
+            sum += weight[i];
+        }
+        double through = sum;  // of the lanes up to this one
+        for (int off = 1; off < 32; off <<= 1) {
+            const double o = __shfl_up_sync(kAll, through, off);
+            if (lane >= (uint32_t)off) through += o;
+        }
+        double mine_before = running + (through - sum);
+        uint32_t here = kAll, here_last = kAll;
+        double here_z = 0.0, here_last_z = 0.0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            mine_before += weight[i];
+            if (weight[i] > 0.0) {
+                here_last = (uint32_t)(v + i), here_last_z = z[i];
+                if (here == kAll && mine_before > goal) here = (uint32_t)(v + i), here_z = z[i];
+            }
+        }
+        const uint32_t hits = __ballot_sync(kAll, here != kAll), some = __ballot_sync(kAll, here_last != kAll);
+        if (hits) {
+            const int from = __ffs(hits) - 1;
+            symbol = __shfl_sync(kAll, here, from);
+            symbol_z = __shfl_sync(kAll, here_z, from);
+        }
+        if (some) {
+            const int from = 31 - __clz(some);
+            last = __shfl_sync(kAll, here_last, from);
+            last_z = __shfl_sync(kAll, here_last_z, from);
+        }
+        running += __shfl_sync(kAll, through, 31);
+    }
+    if (symbol == kAll) symbol = last, symbol_z = last_z;
+    if (lane == 0) {
+        a.symbols[at] = (int32_t)symbol;
+        if (a.log_probability)
+            a.log_probability[at] = (float)((symbol_z == top ? 0.0 : (symbol_z - top) / heat) - log(total));
     }
 }
 
@@ -240,60 +581,176 @@ struct LossArgs {
     int64_t gradient_stride;
 };
 
-__device__ float block_reduce(float v, bool maximum, float* shared) {
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
-    for (int off = 16; off > 0; off >>= 1) {
-        const float o = __shfl_xor_sync(0xffffffffu, v, off);
-        v = maximum ? fmaxf(v, o) : v + o;
-    }
-    __syncthreads();
-    if (lane == 0) shared[warp] = v;
-    __syncthreads();
-    v = shared[0];
-    for (uint32_t w = 1; w < kWarps; ++w) v = maximum ? fmaxf(v, shared[w]) : v + shared[w];
+__device__ __forceinline__ float warp_max(float v) {
+    for (int off = 16; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, off));
+    return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+    for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(kAll, v, off);
     return v;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) cross_entropy_kernel(LossArgs a) {
-    __shared__ float shared[kWarps];
-    const uint32_t row = blockIdx.x;
+// exp(z - top) for a masked place's -inf too.
+__device__ __forceinline__ float weight32(float z, float top) { return z == -CUDART_INF_F ? 0.0f : expf(z - top); }
+
+// Loss of a row with the sum of its weights and the (masked) logit of its target.
+__device__ __forceinline__ float loss_of(float sum, float top, float z) {
+    if (sum != sum) return sum;
+    if (sum == 0.0f || z == -CUDART_INF_F) return CUDART_INF_F;
+    return logf(sum) + (top - z);
+}
+
+// Rows of up to 32 N symbols, a warp each: symbol 32 j + lane is in register j,
+// so the mask's word j is the warp's, and the logits are read once.
+template <typename T, int N>
+__global__ void __launch_bounds__(256) narrow_loss_kernel(const __grid_constant__ LossArgs a) {
+    const uint32_t lane = threadIdx.x & 31u;
+    const uint64_t at = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (at >= a.rows) return;
+    const uint32_t row = (uint32_t)at;
     const T* in = static_cast<const T*>(a.logits) + (int64_t)row * a.logits_stride;
     T* out = static_cast<T*>(a.gradient) + (int64_t)row * a.gradient_stride;
+    float z[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) z[j] = 32 * j + lane < a.vocabulary ? load(in + 32 * j + lane) : -CUDART_INF_F;
     const int32_t target = a.targets[row];
     const MaskRow mask = mask_row(a.allowed, a.allowed_stride, a.states, a.state, row);
     const bool outside = target >= 0 && (uint32_t)target >= a.vocabulary;
     if (target < 0 || outside) {
-        for (uint32_t v = threadIdx.x; v < a.vocabulary; v += kThreads) store(out + v, 0.0f);
-        if (threadIdx.x == 0) a.losses[row] = outside ? CUDART_NAN_F : 0.0f;
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (32 * j + lane < a.vocabulary) store(out + 32 * j + lane, 0.0f);
+        if (lane == 0) a.losses[row] = outside ? CUDART_NAN_F : 0.0f;
         return;
     }
-    float top = -CUDART_INF_F;
-    for (uint32_t v = threadIdx.x; v < a.vocabulary; v += kThreads)
-        if (mask.allows(v)) top = fmaxf(top, load(in + v));
-    top = block_reduce(top, true, shared);
-    float sum = 0.0f;
-    // Nothing left, or only NaN: top stays -inf.  exp(NaN - top) keeps a NaN in the sum.
-    for (uint32_t v = threadIdx.x; v < a.vocabulary; v += kThreads)
-        if (mask.allows(v)) {
-            const float z = load(in + v);
-            sum += z == -CUDART_INF_F ? 0.0f : expf(z - top);
-        }
-    sum = block_reduce(sum, false, shared);
-    const float weight = a.weights ? a.weights[row] : 1.0f;
-    for (uint32_t v = threadIdx.x; v < a.vocabulary; v += kThreads) {
-        float g = 0.0f;
-        if (sum != 0.0f && mask.allows(v)) {
-            const float z = load(in + v);
-            g = (z == -CUDART_INF_F ? 0.0f : expf(z - top)) / sum;
-            g = weight * (g - (v == (uint32_t)target ? 1.0f : 0.0f));
-        }
-        store(out + v, g);
+    uint32_t ok = mask.words || !mask.open ? 0u : kAll;  // bit j: symbol 32 j + lane counts
+    if (mask.words) {
+        const uint32_t words = (a.vocabulary + 31) / 32;
+        const uint32_t word = lane < words ? __ldg(mask.words + lane) : 0u;
+#pragma unroll
+        for (int j = 0; j < N; ++j) ok |= (__shfl_sync(kAll, word, j) >> lane & 1u) << j;
     }
-    if (threadIdx.x == 0) {
-        const float z = mask.allows((uint32_t)target) ? load(in + target) : -CUDART_INF_F;
-        a.losses[row] = sum == 0.0f || z == -CUDART_INF_F ? (sum != sum ? sum : CUDART_INF_F) : logf(sum) + (top - z);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+        if (!(ok >> j & 1u)) z[j] = -CUDART_INF_F;
+    float top = z[0];
+#pragma unroll
+    for (int j = 1; j < N; ++j) top = fmaxf(top, z[j]);
+    top = warp_max(top);
+    float w[N], sum = 0.0f, hit = -CUDART_INF_F;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        w[j] = weight32(z[j], top);
+        sum += w[j];
+        if ((uint32_t)target == 32 * j + lane) hit = z[j];
     }
+    sum = warp_sum(sum);
+    hit = __shfl_sync(kAll, hit, target & 31);
+    const float scale = a.weights ? a.weights[row] : 1.0f, share = 1.0f / sum;
+    if (sum == 0.0f) ok = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const uint32_t v = 32 * j + lane;
+        const float p = w[j] * share - (v == (uint32_t)target ? 1.0f : 0.0f);
+        if (v < a.vocabulary) store(out + v, ok >> j & 1u ? scale * p : 0.0f);
+    }
+    if (lane == 0) a.losses[row] = loss_of(sum, top, hit);
+}
+
+// Wider rows, a block each: up to Held groups a thread stay in registers
+// between the two sweeps; what lies beyond is read again (out of L2).
+template <int Threads>
+__device__ __forceinline__ float block_max(float v, float* shared) {
+    v = warp_max(v);
+    __syncthreads();
+    if ((threadIdx.x & 31u) == 0) shared[threadIdx.x >> 5] = v;
+    __syncthreads();
+    return warp_max(threadIdx.x % 32 < Threads / 32 ? shared[threadIdx.x % 32] : -CUDART_INF_F);
+}
+template <int Threads>
+__device__ __forceinline__ float block_sum(float v, float* shared) {
+    v = warp_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 31u) == 0) shared[threadIdx.x >> 5] = v;
+    __syncthreads();
+    return warp_sum(threadIdx.x % 32 < Threads / 32 ? shared[threadIdx.x % 32] : 0.0f);
+}
+
+template <typename T, int Threads, int Held>
+__global__ void __launch_bounds__(Threads) wide_loss_kernel(const __grid_constant__ LossArgs a) {
+    __shared__ float shared[32];
+    const uint32_t at = blockIdx.x;
+    const Row<T> row(static_cast<const T*>(a.logits) + (int64_t)at * a.logits_stride, a.vocabulary);
+    T* out = static_cast<T*>(a.gradient) + (int64_t)at * a.gradient_stride;
+    const bool aligned = row.alike(out);
+    const int32_t target = a.targets[at];
+    const MaskRow mask = mask_row(a.allowed, a.allowed_stride, a.states, a.state, at);
+    const bool outside = target >= 0 && (uint32_t)target >= a.vocabulary;
+    const auto symbol_of = [&](uint32_t g) { return row.first + (int32_t)g * 8; };
+    if (target < 0 || outside) {
+        Eight<T> zero;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) zero.set(i, 0.0f);
+        for (uint32_t g = threadIdx.x; g < row.groups; g += Threads) row.write(out, aligned, symbol_of(g), zero);
+        if (threadIdx.x == 0) a.losses[at] = outside ? CUDART_NAN_F : 0.0f;
+        return;
+    }
+    // Bit i: symbol v + i counts.
+    const auto counts_at = [&](int32_t v) {
+        uint32_t ok = mask.eight(v, a.vocabulary);
+        if (!row.whole(v))
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (!row.in(v + i)) ok &= ~(1u << i);
+        return ok;
+    };
+    Eight<T> held[Held];
+    const auto each = [&](auto&& body) {
+#pragma unroll
+        for (int j = 0; j < Held; ++j) {
+            const uint32_t g = j * Threads + threadIdx.x;
+            if (g < row.groups) body(held[j], symbol_of(g));
+        }
+        for (uint32_t g = Held * Threads + threadIdx.x; g < row.groups; g += Threads)
+            body(row.read(symbol_of(g)), symbol_of(g));
+    };
+#pragma unroll
+    for (int j = 0; j < Held; ++j) {
+        const uint32_t g = j * Threads + threadIdx.x;
+        if (g < row.groups) held[j] = row.read(symbol_of(g));
+    }
+    // The largest logit and the sum of the weights by it: first by the thread's own, in one sweep.
+    float top = -CUDART_INF_F, sum = 0.0f;
+    each([&](const Eight<T>& e, int32_t v) {
+        const uint32_t ok = counts_at(v);
+        float most = -CUDART_INF_F;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (ok >> i & 1u) most = fmaxf(most, e[i]);
+        if (most > top) {
+            sum *= weight32(top, most);
+            top = most;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (ok >> i & 1u) sum += weight32(e[i], top);
+    });
+    const float own = top;
+    top = block_max<Threads>(top, shared);
+    sum = block_sum<Threads>(own == top ? sum : sum * weight32(own, top), shared);
+    const float scale = a.weights ? a.weights[at] : 1.0f, share = 1.0f / sum;
+    each([&](const Eight<T>& e, int32_t v) {
+        const uint32_t ok = sum == 0.0f ? 0u : counts_at(v);
+        Eight<T> r;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float p = weight32(e[i], top) * share - (v + i == target ? 1.0f : 0.0f);
+            r.set(i, ok >> i & 1u ? scale * p : 0.0f);
+        }
+        row.write(out, aligned, v, r);
+    });
+    if (threadIdx.x == 0)
+        a.losses[at] = loss_of(sum, top, mask.allows((uint32_t)target) ? load(row.p + target) : -CUDART_INF_F);
 }
 
 template <typename Body>
@@ -304,6 +761,41 @@ void dispatch(int dtype, Body&& body) {
         case LEO_B200_F16: body((__half*)nullptr); return;
         default: throw Failure("logits must be float32, bfloat16 or float16");
     }
+}
+
+// A block a row, or a cluster of up to eight while that leaves SMs without work.
+template <typename T, int Warps, int Steps>
+void launch_pick(const LogitArgs& a, cudaStream_t stream) {
+    using S = PickShape<T, Warps, Steps>;
+    const uint32_t all = (a.vocabulary + 7 + S::kSpan - 1) / S::kSpan;
+    uint32_t blocks = 1;
+    while (blocks < 8 && blocks < all && (uint64_t)a.rows * blocks < 512) blocks *= 2;
+    while (blocks < 8 && (all + blocks - 1) / blocks > S::kMaxRounds) blocks *= 2;
+    const uint32_t rounds = (all + blocks - 1) / blocks;
+    require(rounds <= S::kMaxRounds, "the vocabulary is too large for one pick");
+    require((uint64_t)a.rows * blocks < (1ull << 31), "too many rows for one call");
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(a.rows * blocks);
+    config.blockDim = dim3(32 * Warps);
+    config.stream = stream;
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = blocks;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    config.attrs = &cluster;
+    config.numAttrs = 1;
+    check(cudaLaunchKernelEx(&config, pick_kernel<T, Warps, Steps>, a, rounds), "pick_kernel");
+}
+
+// A warp a row while it holds the row in 32 registers a lane, a block above.
+template <typename T>
+void launch_loss(const LossArgs& a, cudaStream_t stream) {
+    const uint32_t v = a.vocabulary, warps = (a.rows + 7) / 8;
+    if (v <= 288) narrow_loss_kernel<T, 9><<<warps, 256, 0, stream>>>(a);
+    else if (v <= 512) narrow_loss_kernel<T, 16><<<warps, 256, 0, stream>>>(a);
+    else if (v <= 1024) narrow_loss_kernel<T, 32><<<warps, 256, 0, stream>>>(a);
+    else if (v <= 8000) wide_loss_kernel<T, 256, 4><<<a.rows, 256, 0, stream>>>(a);
+    else wide_loss_kernel<T, 512, sizeof(T) == 2 ? 8 : 4><<<a.rows, 512, 0, stream>>>(a);
 }
 
 void check_mask(const uint32_t* allowed, int64_t stride, uint32_t states, const int32_t* state, uint32_t rows,
@@ -355,7 +847,10 @@ int leo_b200_adjust_logits(int device, int dtype, const void* logits, int64_t lo
             a.out = out;
             a.out_stride = out_stride;
             DeviceScope scope(device);
-            adjust_kernel<T><<<rows, kThreads, 0, (cudaStream_t)stream>>>(a);
+            // A chunk more than the symbols take, if a row can start off a 16-byte address.
+            const uint32_t chunks = (vocabulary + 7 + kAdjustSpan - 1) / kAdjustSpan;
+            require((uint64_t)rows * chunks < (1ull << 31), "too many rows for one call");
+            adjust_kernel<T><<<rows * chunks, kAdjustThreads, 0, (cudaStream_t)stream>>>(a, chunks);
             check(cudaGetLastError(), "adjust_kernel");
         });
     });
@@ -387,8 +882,10 @@ int leo_b200_pick_symbols(int device, int dtype, const void* logits, int64_t log
             a.symbols = symbols;
             a.log_probability = log_probability;
             DeviceScope scope(device);
-            pick_kernel<T><<<rows, kThreads, 0, (cudaStream_t)stream>>>(a);
-            check(cudaGetLastError(), "pick_kernel");
+            if (vocabulary + 7 <= PickShape<T, 4, 1>::kSpan)
+                launch_pick<T, 4, 1>(a, (cudaStream_t)stream);
+            else
+                launch_pick<T, 8, 4>(a, (cudaStream_t)stream);
         });
     });
 }
@@ -409,7 +906,7 @@ int leo_b200_masked_cross_entropy(int device, int dtype, const void* logits, int
             LossArgs a{logits, logits_stride, rows,    vocabulary, targets, allowed, allowed_stride,
                        states, state,         weights, losses,     gradient, gradient_stride};
             DeviceScope scope(device);
-            cross_entropy_kernel<T><<<rows, kThreads, 0, (cudaStream_t)stream>>>(a);
+            launch_loss<T>(a, (cudaStream_t)stream);
             check(cudaGetLastError(), "cross_entropy_kernel");
         });
     });
