@@ -18,6 +18,7 @@
 #include <type_traits>
 
 #include "../../include/leo_b200.h"
+#include "leo_operator_device.cuh"
 #include "leo_operator_host.h"
 
 namespace {
@@ -26,13 +27,6 @@ using namespace leo_operator;
 namespace cg = cooperative_groups;
 
 constexpr uint32_t kAll = 0xffffffffu;
-
-__device__ __forceinline__ float load(const float* p) { return *p; }
-__device__ __forceinline__ float load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-__device__ __forceinline__ float load(const __half* p) { return __half2float(*p); }
-__device__ __forceinline__ void store(float* p, float v) { *p = v; }
-__device__ __forceinline__ void store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void store(__half* p, float v) { *p = __float2half_rn(v); }
 
 // Eight neighbours of a row as they lie in memory.
 template <typename T> struct Eight {
@@ -45,6 +39,25 @@ template <typename T> struct Eight {
             return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
         } else {
             return __half2float(__ushort_as_half((unsigned short)(w[i / 2] >> 16 * (i & 1))));
+        }
+    }
+    __device__ __forceinline__ const uint32_t* words() const { return reinterpret_cast<const uint32_t*>(raw); }
+    // Elements 2 i and 2 i + 1.
+    __device__ __forceinline__ Pair32 pair(int i) const { return PairOf<T>::unpack(words() + i * (sizeof(T) / 2)); }
+    __device__ __forceinline__ void set_pair(int i, Pair32 v) {
+        PairOf<T>::pack(v, reinterpret_cast<uint32_t*>(raw) + i * (sizeof(T) / 2));
+    }
+    __device__ __forceinline__ float largest() const {
+        if constexpr (std::is_same_v<T, float>) {
+            float m = (*this)[0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) m = fmaxf(m, (*this)[i]);
+            return m;
+        } else {
+            using Two = std::conditional_t<std::is_same_v<T, __nv_bfloat16>, __nv_bfloat162, __half2>;
+            const Two* w = reinterpret_cast<const Two*>(raw);
+            const Two m = __hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3]));
+            return fmaxf(load(&m.x), load(&m.y));
         }
     }
     __device__ __forceinline__ void set(int i, float v) {  // i ascending
@@ -249,8 +262,17 @@ __global__ void __launch_bounds__(kAdjustThreads) adjust_kernel(const __grid_con
             c[0] = x.x, c[1] = x.y, c[2] = x.z, c[3] = x.w, c[4] = y.x, c[5] = y.y, c[6] = y.z, c[7] = y.w;
         }
         Eight<T> r;
+        if (((c[0] | c[1]) | (c[2] | c[3]) | (c[4] | c[5]) | (c[6] | c[7])) == 0 && ok == 0xffu) {
+            // nothing of these was said before, and nothing is masked
+            r = e[j];
+            if (k.bias)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) r.set(i, adjusted(e[j][i], c[i], k, bias[j][i], ok >> i & 1u));
+                for (int i = 0; i < 4; ++i)
+                    r.set_pair(i, add2(e[j].pair(i), pair_of(bias[j][2 * i], bias[j][2 * i + 1])));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) r.set(i, adjusted(e[j][i], c[i], k, bias[j][i], ok >> i & 1u));
+        }
         row.write(out, aligned, v, r);
     }
 }
@@ -269,8 +291,8 @@ __device__ const double kTwoTo[32] = {
     0x1.ae89f995ad3adp+0, 0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0,
     0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0, 0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0};
 __device__ __forceinline__ double exp_down(double x, const double* two_to) {
-    if (!(x > -700.0)) return exp(x);  // subnormal results, -inf and NaN
     const double magic = 0x1.8p52;
+    x = fmax(x, -746.0);  // 0 from there on; NaN becomes 0 too
     const double shifted = fma(x, 0x1.71547652b82fep+5, magic);
     const int32_t n = __double2loint(shifted);
     const double whole = shifted - magic;
@@ -282,8 +304,10 @@ __device__ __forceinline__ double exp_down(double x, const double* two_to) {
     p = fma(p, r, 0.5);
     p = fma(p, r, 1.0);
     const double scale = two_to[n & 31];
-    const double y = fma(scale, p * r, scale);
-    return __hiloint2double(__double2hiint(y) + ((n >> 5) << 20), __double2loint(y));
+    // 2^q in two factors, so that a subnormal result is rounded once
+    const int32_t q = n >> 5, half = q >> 1;
+    return fma(scale, p * r, scale) * __hiloint2double((1023 + half) << 20, 0) *
+           __hiloint2double((1023 + (q - half)) << 20, 0);
 }
 
 // A sum of weights exp((z - top) / heat), by its own top.
@@ -292,12 +316,8 @@ struct Weights {
 };
 __device__ __forceinline__ Weights no_weights() { return {-CUDART_INF, 0.0}; }
 __device__ __forceinline__ double weight_of(double z, double top, double cold, const double* two_to) {
-    return z == top ? 1.0 : z == -CUDART_INF || top == CUDART_INF ? 0.0 : exp_down((z - top) * cold, two_to);
-}
-__device__ __forceinline__ Weights both(const Weights& x, const Weights& y, double cold, const double* two_to) {
-    const double top = fmax(x.top, y.top);
-    if (top == -CUDART_INF) return no_weights();
-    return {top, x.sum * weight_of(x.top, top, cold, two_to) + y.sum * weight_of(y.top, top, cold, two_to)};
+    // A masked place's -inf gives 0 by itself; beside an infinite top only its equals count.
+    return top == CUDART_INF ? (z == top ? 1.0 : 0.0) : exp_down((z - top) * cold, two_to);
 }
 
 // What a part of a row knows: its weights, its largest logit and the lowest
@@ -345,6 +365,13 @@ __global__ void __launch_bounds__(32 * Warps) pick_kernel(const __grid_constant_
     const auto symbols_at = [&](uint32_t round, uint32_t w, int step) {
         return row.first + (int32_t)((rank * rounds + round) * S::kSpan + ((w * Steps + step) * 32 + lane) * 8);
     };
+    // Whether the rules leave a whole group as it is, but for the bias.
+    const auto plain = [&](int32_t v, int32_t first) {
+        if (!row.whole(v) || k.mask.eight(v, a.vocabulary) != 0xffu) return false;
+        if (!k.length) return true;
+        const uint4* c = reinterpret_cast<const uint4*>(counts + (v - first));
+        return ((c[0].x | c[0].y) | (c[0].z | c[0].w) | (c[1].x | c[1].y) | (c[1].z | c[1].w)) == 0;
+    };
     const auto adjust = [&](const Eight<T>& e, const float (&bias)[8], int32_t v, int32_t first, double (&z)[8]) {
         const uint32_t ok = k.mask.eight(v, a.vocabulary);
 #pragma unroll
@@ -375,32 +402,55 @@ __global__ void __launch_bounds__(32 * Warps) pick_kernel(const __grid_constant_
         for (int step = 0; step < Steps; ++step) {
             const int32_t v = symbols_at(round, warp, step);
             if (v >= (int32_t)a.vocabulary) continue;
-            float bias[8] = {};
-            read_bias(k, row, v, bias);
-            double z[8];
-            adjust(e[step], bias, v, first, z);
-            double top = w.top;
+            double z[8], top;
+            const bool as_is = plain(v, first);
+            if (as_is && !k.bias) {
+                // Nothing of these was said before, and nothing is masked: a float's order is the double's.
+                const float most = e[step].largest();
+                top = (double)most;
+                if (top > best_value) {
+                    best_value = top;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (z[i] != z[i]) part.bad = 1;
-                if (z[i] > best_value) best_value = z[i], part.best = (uint32_t)(v + i);
-                top = fmax(top, z[i]);
+                    for (int i = 7; i >= 0; --i)
+                        if (e[step][i] == most) part.best = (uint32_t)(v + i);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    z[i] = (double)e[step][i];
+                    part.bad |= e[step][i] != e[step][i];
+                }
+            } else {
+                float bias[8] = {};
+                read_bias(k, row, v, bias);
+                if (as_is) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) z[i] = (double)e[step][i] + (double)bias[i];
+                } else {
+                    adjust(e[step], bias, v, first, z);
+                }
+                top = -CUDART_INF;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    part.bad |= z[i] != z[i];
+                    if (z[i] > best_value) best_value = z[i], part.best = (uint32_t)(v + i);
+                    top = fmax(top, z[i]);
+                }
             }
             if (top > w.top) {
-                w.sum = w.sum * weight_of(w.top, top, cold, two_to);
+                w.sum = w.top == -CUDART_INF ? 0.0 : w.sum * weight_of(w.top, top, cold, two_to);
                 w.top = top;
             }
-            if (top != -CUDART_INF) {
+            if (w.top != -CUDART_INF) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) w.sum += weight_of(z[i], top, cold, two_to);
+                for (int i = 0; i < 8; ++i) w.sum += weight_of(z[i], w.top, cold, two_to);
             }
         }
-        for (int off = 16; off > 0; off >>= 1) {
-            const Weights o{__shfl_xor_sync(kAll, w.top, off), __shfl_xor_sync(kAll, w.sum, off)};
-            w = both(w, o, cold, two_to);
-        }
-        if (lane == 0) stretches[round * Warps + warp] = w;
-        part.weights = both(part.weights, w, cold, two_to);
+        // The warp's, by its own top.
+        double top = w.top;
+        for (int off = 16; off > 0; off >>= 1) top = fmax(top, __shfl_xor_sync(kAll, top, off));
+        double sum = w.top == -CUDART_INF ? 0.0 : w.sum * weight_of(w.top, top, cold, two_to);
+        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(kAll, sum, off);
+        if (lane == 0) stretches[round * Warps + warp] = {top, sum};
     }
     // The block's part.
     for (int off = 16; off > 0; off >>= 1) {
@@ -411,17 +461,25 @@ __global__ void __launch_bounds__(32 * Warps) pick_kernel(const __grid_constant_
     }
     if (lane == 0) warp_parts[warp] = part, warp_best[warp] = best_value;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        Part p = warp_parts[0];
-        for (int w = 1; w < Warps; ++w) {
-            const Part& o = warp_parts[w];
-            if (warp_best[w] > best_value || (warp_best[w] == best_value && o.best < p.best))
-                best_value = warp_best[w], p.best = o.best;
-            p.bad |= o.bad;
-            p.weights = both(p.weights, o.weights, cold, two_to);
+    if (warp == 0) {
+        Part p = warp_parts[lane < Warps ? lane : 0];
+        best_value = warp_best[lane < Warps ? lane : 0];
+        for (int off = Warps / 2; off > 0; off >>= 1) {
+            const double v = __shfl_xor_sync(kAll, best_value, off);
+            const uint32_t b = __shfl_xor_sync(kAll, p.best, off);
+            if (v > best_value || (v == best_value && b < p.best)) best_value = v, p.best = b;
+            p.bad |= __shfl_xor_sync(kAll, p.bad, off);
         }
-        mine = p;
-        block_best = best_value;
+        // by the block's largest logit, which is the top of one of its stretches
+        best_value = __shfl_sync(kAll, best_value, 0);
+        double sum = 0.0;
+        for (uint32_t j = lane; j < rounds * Warps; j += 32) {
+            const Weights w = stretches[j];
+            if (w.top != -CUDART_INF) sum += w.sum * weight_of(w.top, best_value, cold, two_to);
+        }
+        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(kAll, sum, off);
+        p.weights = {best_value, sum};
+        if (lane == 0) mine = p, block_best = best_value;
     }
     if (blocks > 1)
         cluster.sync();
@@ -446,7 +504,9 @@ __global__ void __launch_bounds__(32 * Warps) pick_kernel(const __grid_constant_
         }
         uint32_t pick = kAll - 1u;  // nothing to walk
         if (!bad && best != kAll) {
-            const double share = p.weights.sum * (lane < blocks ? weight_of(p.weights.top, top, cold, two_to) : 0.0);
+            const double share = lane < blocks && p.weights.top != -CUDART_INF
+                                     ? p.weights.sum * weight_of(p.weights.top, top, cold, two_to)
+                                     : 0.0;
             double total = 0.0;
             for (uint32_t j = 0; j < blocks; ++j) total += __shfl_sync(kAll, share, j);
             if (greedy) {
@@ -476,7 +536,7 @@ __global__ void __launch_bounds__(32 * Warps) pick_kernel(const __grid_constant_
                         const uint32_t j = base + lane;
                         Weights w = no_weights();
                         if (j < rounds * Warps) w = stretches[j];
-                        const double s = w.sum * weight_of(w.top, top, cold, two_to);
+                        const double s = w.top == -CUDART_INF ? 0.0 : w.sum * weight_of(w.top, top, cold, two_to);
                         for (uint32_t l = 0; l < 32 && found == kAll; ++l) {
                             const double one = __shfl_sync(kAll, s, l);
                             if (one > 0.0) {
@@ -590,15 +650,36 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
-// exp(z - top) for a masked place's -inf too.
-__device__ __forceinline__ float weight32(float z, float top) { return z == -CUDART_INF_F ? 0.0f : expf(z - top); }
-
-// Loss of a row with the sum of its weights and the (masked) logit of its target.
-__device__ __forceinline__ float loss_of(float sum, float top, float z) {
-    if (sum != sum) return sum;
-    if (sum == 0.0f || z == -CUDART_INF_F) return CUDART_INF_F;
-    return logf(sum) + (top - z);
+__device__ __forceinline__ float exp2_of(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
+
+// Weights by a row's largest logit as 2^(z c - top c), one multiply-add and one
+// exponential each.  top c is rounded once for the whole row, which scales all
+// weights alike: out of their ratios it falls, and the loss takes it out.  A
+// masked place's -inf gives 0.  Beside logits so large that neighbours are
+// 2^100 apart only equals count, which a c of 2^-20 gives without overflow.
+struct RowScale {
+    float top, c, shift, off;  // weights are 2^off times too large
+    __device__ __forceinline__ explicit RowScale(float top_) : top(top_) {
+        c = fabsf(top) < 1e37f ? 1.44269504f : 0x1p-20f;
+        shift = top == -CUDART_INF_F ? 0.0f : top * c;
+        off = top == -CUDART_INF_F ? 0.0f : fmaf(top, c, -shift);
+    }
+    __device__ __forceinline__ float weight(float z) const { return exp2_of(fmaf(z, c, -shift)); }
+    __device__ __forceinline__ Pair32 weight(Pair32 z) const {
+        const float2 x = parts(fma2(z, pair_of(c, c), pair_of(-shift, -shift)));
+        return pair_of(exp2_of(x.x), exp2_of(x.y));
+    }
+    // Loss of a row with the sum of its weights and the (masked) logit of its target.
+    __device__ __forceinline__ float loss(float sum, float z) const {
+        if (sum != sum) return sum;
+        if (sum == 0.0f || z == -CUDART_INF_F) return CUDART_INF_F;
+        return fmaf(off, -0.693147181f, logf(sum)) + (top - z);
+    }
+};
 
 // Rows of up to 32 N symbols, a warp each: symbol 32 j + lane is in register j,
 // so the mask's word j is the warp's, and the logits are read once.
@@ -608,85 +689,83 @@ __global__ void __launch_bounds__(256) narrow_loss_kernel(const __grid_constant_
     const uint64_t at = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (at >= a.rows) return;
     const uint32_t row = (uint32_t)at;
-    const T* in = static_cast<const T*>(a.logits) + (int64_t)row * a.logits_stride;
-    T* out = static_cast<T*>(a.gradient) + (int64_t)row * a.gradient_stride;
+    const T* in = static_cast<const T*>(a.logits) + (int64_t)row * a.logits_stride + lane;
+    T* out = static_cast<T*>(a.gradient) + (int64_t)row * a.gradient_stride + lane;
+    const uint32_t mine = (a.vocabulary + 31 - lane) / 32;  // symbols of the lane
     float z[N];
 #pragma unroll
-    for (int j = 0; j < N; ++j) z[j] = 32 * j + lane < a.vocabulary ? load(in + 32 * j + lane) : -CUDART_INF_F;
+    for (int j = 0; j < N; ++j) z[j] = j < mine ? load(in + 32 * j) : -CUDART_INF_F;
     const int32_t target = a.targets[row];
     const MaskRow mask = mask_row(a.allowed, a.allowed_stride, a.states, a.state, row);
     const bool outside = target >= 0 && (uint32_t)target >= a.vocabulary;
     if (target < 0 || outside) {
 #pragma unroll
         for (int j = 0; j < N; ++j)
-            if (32 * j + lane < a.vocabulary) store(out + 32 * j + lane, 0.0f);
+            if (j < mine) store(out + 32 * j, 0.0f);
         if (lane == 0) a.losses[row] = outside ? CUDART_NAN_F : 0.0f;
         return;
     }
-    uint32_t ok = mask.words || !mask.open ? 0u : kAll;  // bit j: symbol 32 j + lane counts
+    const uint32_t bit = 1u << lane;
     if (mask.words) {
-        const uint32_t words = (a.vocabulary + 31) / 32;
-        const uint32_t word = lane < words ? __ldg(mask.words + lane) : 0u;
 #pragma unroll
-        for (int j = 0; j < N; ++j) ok |= (__shfl_sync(kAll, word, j) >> lane & 1u) << j;
+        for (int j = 0; j < N; ++j)
+            if (j < mine && !(__ldg(mask.words + j) & bit)) z[j] = -CUDART_INF_F;
+    } else if (!mask.open) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) z[j] = -CUDART_INF_F;
     }
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-        if (!(ok >> j & 1u)) z[j] = -CUDART_INF_F;
     float top = z[0];
 #pragma unroll
     for (int j = 1; j < N; ++j) top = fmaxf(top, z[j]);
-    top = warp_max(top);
-    float w[N], sum = 0.0f, hit = -CUDART_INF_F;
+    const RowScale by(warp_max(top));
+    float w[N], sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-        w[j] = weight32(z[j], top);
+        w[j] = by.weight(z[j]);
         sum += w[j];
-        if ((uint32_t)target == 32 * j + lane) hit = z[j];
     }
     sum = warp_sum(sum);
-    hit = __shfl_sync(kAll, hit, target & 31);
-    const float scale = a.weights ? a.weights[row] : 1.0f, share = 1.0f / sum;
-    if (sum == 0.0f) ok = 0;
+    const float scale = a.weights ? a.weights[row] : 1.0f, gain = sum == 0.0f ? 0.0f : scale / sum;
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-        const uint32_t v = 32 * j + lane;
-        const float p = w[j] * share - (v == (uint32_t)target ? 1.0f : 0.0f);
-        if (v < a.vocabulary) store(out + v, ok >> j & 1u ? scale * p : 0.0f);
+    for (int j = 0; j < N; ++j)
+        if (j < mine) store(out + 32 * j, w[j] * gain);
+    // The target's term, in place of what this lane has written there.
+    if (lane == ((uint32_t)target & 31u)) {
+        const bool counts = mask.allows((uint32_t)target);
+        const float hit = counts ? load(in + (target & ~31)) : -CUDART_INF_F;
+        if (counts && sum != 0.0f) store(out + (target & ~31), fmaf(by.weight(hit), gain, -scale));
+        a.losses[row] = by.loss(sum, hit);
     }
-    if (lane == 0) a.losses[row] = loss_of(sum, top, hit);
 }
 
 // Wider rows, a block each: up to Held groups a thread stay in registers
-// between the two sweeps; what lies beyond is read again (out of L2).
-template <int Threads>
-__device__ __forceinline__ float block_max(float v, float* shared) {
-    v = warp_max(v);
-    __syncthreads();
+// between the sweeps; what lies beyond is read again (out of L2).
+template <int Threads, bool Maximum>
+__device__ __forceinline__ float block_of(float v, float* shared) {
+    v = Maximum ? warp_max(v) : warp_sum(v);
     if ((threadIdx.x & 31u) == 0) shared[threadIdx.x >> 5] = v;
     __syncthreads();
-    return warp_max(threadIdx.x % 32 < Threads / 32 ? shared[threadIdx.x % 32] : -CUDART_INF_F);
-}
-template <int Threads>
-__device__ __forceinline__ float block_sum(float v, float* shared) {
-    v = warp_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 31u) == 0) shared[threadIdx.x >> 5] = v;
-    __syncthreads();
-    return warp_sum(threadIdx.x % 32 < Threads / 32 ? shared[threadIdx.x % 32] : 0.0f);
+    v = threadIdx.x % 32 < Threads / 32 ? shared[threadIdx.x % 32] : Maximum ? -CUDART_INF_F : 0.0f;
+    return Maximum ? warp_max(v) : warp_sum(v);
 }
 
 template <typename T, int Threads, int Held>
 __global__ void __launch_bounds__(Threads) wide_loss_kernel(const __grid_constant__ LossArgs a) {
-    __shared__ float shared[32];
+    __shared__ float shared[2][32];
     const uint32_t at = blockIdx.x;
     const Row<T> row(static_cast<const T*>(a.logits) + (int64_t)at * a.logits_stride, a.vocabulary);
     T* out = static_cast<T*>(a.gradient) + (int64_t)at * a.gradient_stride;
     const bool aligned = row.alike(out);
+    const auto symbol_of = [&](uint32_t g) { return row.first + (int32_t)g * 8; };
+    Eight<T> held[Held];
+#pragma unroll
+    for (int j = 0; j < Held; ++j) {
+        const uint32_t g = j * Threads + threadIdx.x;
+        if (g < row.groups) held[j] = row.read(symbol_of(g));
+    }
     const int32_t target = a.targets[at];
     const MaskRow mask = mask_row(a.allowed, a.allowed_stride, a.states, a.state, at);
     const bool outside = target >= 0 && (uint32_t)target >= a.vocabulary;
-    const auto symbol_of = [&](uint32_t g) { return row.first + (int32_t)g * 8; };
     if (target < 0 || outside) {
         Eight<T> zero;
 #pragma unroll
@@ -704,7 +783,6 @@ __global__ void __launch_bounds__(Threads) wide_loss_kernel(const __grid_constan
                 if (!row.in(v + i)) ok &= ~(1u << i);
         return ok;
     };
-    Eight<T> held[Held];
     const auto each = [&](auto&& body) {
 #pragma unroll
         for (int j = 0; j < Held; ++j) {
@@ -714,43 +792,50 @@ __global__ void __launch_bounds__(Threads) wide_loss_kernel(const __grid_constan
         for (uint32_t g = Held * Threads + threadIdx.x; g < row.groups; g += Threads)
             body(row.read(symbol_of(g)), symbol_of(g));
     };
-#pragma unroll
-    for (int j = 0; j < Held; ++j) {
-        const uint32_t g = j * Threads + threadIdx.x;
-        if (g < row.groups) held[j] = row.read(symbol_of(g));
-    }
-    // The largest logit and the sum of the weights by it: first by the thread's own, in one sweep.
-    float top = -CUDART_INF_F, sum = 0.0f;
+    float top = -CUDART_INF_F;
     each([&](const Eight<T>& e, int32_t v) {
         const uint32_t ok = counts_at(v);
-        float most = -CUDART_INF_F;
+        if (ok == 0xffu) {
+            top = fmaxf(top, e.largest());
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (ok >> i & 1u) most = fmaxf(most, e[i]);
-        if (most > top) {
-            sum *= weight32(top, most);
-            top = most;
+            for (int i = 0; i < 8; ++i)
+                if (ok >> i & 1u) top = fmaxf(top, e[i]);
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (ok >> i & 1u) sum += weight32(e[i], top);
     });
-    const float own = top;
-    top = block_max<Threads>(top, shared);
-    sum = block_sum<Threads>(own == top ? sum : sum * weight32(own, top), shared);
-    const float scale = a.weights ? a.weights[at] : 1.0f, share = 1.0f / sum;
+    const RowScale by(block_of<Threads, true>(top, shared[0]));
+    Pair32 sums = 0;
     each([&](const Eight<T>& e, int32_t v) {
-        const uint32_t ok = sum == 0.0f ? 0u : counts_at(v);
-        Eight<T> r;
+        const uint32_t ok = counts_at(v);
+        if (ok == 0xffu) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float p = weight32(e[i], top) * share - (v + i == target ? 1.0f : 0.0f);
-            r.set(i, ok >> i & 1u ? scale * p : 0.0f);
+            for (int i = 0; i < 4; ++i) sums = add2(sums, by.weight(e.pair(i)));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (ok >> i & 1u) sums = add2(sums, pair_of(by.weight(e[i]), 0.0f));
+        }
+    });
+    const float2 halves = parts(sums);
+    const float sum = block_of<Threads, false>(halves.x + halves.y, shared[1]);
+    const float scale = a.weights ? a.weights[at] : 1.0f, gain = sum == 0.0f ? 0.0f : scale / sum;
+    each([&](const Eight<T>& e, int32_t v) {
+        const uint32_t ok = counts_at(v);
+        Eight<T> r;
+        if (ok == 0xffu && (uint32_t)(target - v) >= 8u) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r.set_pair(i, mul2(by.weight(e.pair(i)), pair_of(gain, gain)));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float g = fmaf(by.weight(e[i]), gain, v + i == target && sum != 0.0f ? -scale : 0.0f);
+                r.set(i, ok >> i & 1u ? g : 0.0f);
+            }
         }
         row.write(out, aligned, v, r);
     });
     if (threadIdx.x == 0)
-        a.losses[at] = loss_of(sum, top, mask.allows((uint32_t)target) ? load(row.p + target) : -CUDART_INF_F);
+        a.losses[at] = by.loss(sum, mask.allows((uint32_t)target) ? load(row.p + target) : -CUDART_INF_F);
 }
 
 template <typename Body>
