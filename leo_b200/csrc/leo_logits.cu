@@ -28,6 +28,15 @@ namespace cg = cooperative_groups;
 
 constexpr uint32_t kAll = 0xffffffffu;
 
+__device__ __forceinline__ float warp_max(float v) {
+    for (int off = 16; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, off));
+    return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+    for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(kAll, v, off);
+    return v;
+}
+
 // Eight neighbours of a row as they lie in memory.
 template <typename T> struct Eight {
     uint4 raw[sizeof(T) / 2];
@@ -166,28 +175,37 @@ __device__ __forceinline__ RowRules row_rules(const LeoB200LogitRules& r, uint32
     return k;
 }
 
-// Counts of the history's symbols in [first, first + Span), by the whole block.
-template <uint32_t Span>
-__device__ __forceinline__ void count_history(const RowRules& k, int32_t first, uint32_t* counts) {
-    for (uint32_t i = threadIdx.x; i < Span / 4; i += blockDim.x)
+// Counts of the history's symbols in [first, first + span), span a multiple of
+// four, by the whole block.
+__device__ __forceinline__ void count_history(const RowRules& k, int32_t first, uint32_t span, uint32_t* counts) {
+    for (uint32_t i = threadIdx.x; i < span / 4; i += blockDim.x)
         reinterpret_cast<uint4*>(counts)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
 #pragma unroll 4
     for (uint32_t i = threadIdx.x; i < k.length; i += blockDim.x) {
         const int32_t symbol = __ldg(k.history + i);
         const uint32_t v = (uint32_t)(symbol - first);
-        if (symbol >= 0 && v < Span) atomicAdd(&counts[v], 1u);
+        if (symbol >= 0 && v < span) atomicAdd(&counts[v], 1u);
     }
     __syncthreads();
 }
 
+__device__ __forceinline__ float quotient(float x, float y, float) { return x / y; }
+// x / y rounded as a division is, from the rounded reciprocal of y (P. W.
+// Markstein, IBM J. Res. Dev. 34, 1990): the remainder of the first quotient
+// is exact, as x and y are floats and nothing leaves the range of double.  An
+// infinite quotient has none.
+__device__ __forceinline__ double quotient(double x, double y, double reciprocal) {
+    const double q = x * reciprocal;
+    return isinf(q) ? q : fma(fma(-q, y, x), reciprocal, q);
+}
+
 // The penalties, the bias and the mask, every operation rounded by itself in F.
 template <typename F>
-__device__ __forceinline__ F adjusted(F z, uint32_t count, const RowRules& k, float bias, bool allowed) {
-    if (count) {
-        z = z > (F)0 ? z / (F)k.repetition : z * (F)k.repetition;
-        z -= (F)k.presence + (F)k.frequency * (F)count;
-    }
+__device__ __forceinline__ F adjusted(F z, uint32_t count, const RowRules& k, F reciprocal, float bias, bool allowed) {
+    const F penalised = (z > (F)0 ? quotient(z, (F)k.repetition, reciprocal) : z * (F)k.repetition) -
+                        ((F)k.presence + (F)k.frequency * (F)count);
+    z = count ? penalised : z;
     if (k.bias) z += (F)bias;
     return allowed ? z : -(F)CUDART_INF;
 }
@@ -248,7 +266,7 @@ __global__ void __launch_bounds__(kAdjustThreads) adjust_kernel(const __grid_con
             read_bias(k, row, v, bias[j]);
         }
     }
-    if (k.length) count_history<kAdjustSpan>(k, first, counts);
+    if (k.length) count_history(k, first, kAdjustSpan, counts);
 #pragma unroll
     for (uint32_t j = 0; j < kAdjustGroups; ++j) {
         const uint32_t within = (j * blockDim.x + threadIdx.x) * 8;
@@ -271,7 +289,7 @@ __global__ void __launch_bounds__(kAdjustThreads) adjust_kernel(const __grid_con
                     r.set_pair(i, add2(e[j].pair(i), pair_of(bias[j][2 * i], bias[j][2 * i + 1])));
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) r.set(i, adjusted(e[j][i], c[i], k, bias[j][i], ok >> i & 1u));
+            for (int i = 0; i < 8; ++i) r.set(i, adjusted(e[j][i], c[i], k, 0.0f, bias[j][i], ok >> i & 1u));
         }
         row.write(out, aligned, v, r);
     }
@@ -292,7 +310,9 @@ __device__ const double kTwoTo[32] = {
     0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0, 0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0};
 __device__ __forceinline__ double exp_down(double x, const double* two_to) {
     const double magic = 0x1.8p52;
-    x = fmax(x, -746.0);  // 0 from there on; NaN becomes 0 too
+    // -746 and below (-inf too, by the bits of its high word): 0
+    const bool none = (uint32_t)__double2hiint(x) >= 0xc0875000u;
+    if (none) x = 0.0;
     const double shifted = fma(x, 0x1.71547652b82fep+5, magic);
     const int32_t n = __double2loint(shifted);
     const double whole = shifted - magic;
@@ -307,7 +327,7 @@ __device__ __forceinline__ double exp_down(double x, const double* two_to) {
     // 2^q in two factors, so that a subnormal result is rounded once
     const int32_t q = n >> 5, half = q >> 1;
     return fma(scale, p * r, scale) * __hiloint2double((1023 + half) << 20, 0) *
-           __hiloint2double((1023 + (q - half)) << 20, 0);
+           __hiloint2double(none ? 0 : (1023 + (q - half)) << 20, 0);
 }
 
 // A sum of weights exp((z - top) / heat), by its own top.
@@ -315,9 +335,19 @@ struct Weights {
     double top, sum;
 };
 __device__ __forceinline__ Weights no_weights() { return {-CUDART_INF, 0.0}; }
+// A masked place's -inf gives 0 by itself; beside an infinite top only its equals count.
 __device__ __forceinline__ double weight_of(double z, double top, double cold, const double* two_to) {
-    // A masked place's -inf gives 0 by itself; beside an infinite top only its equals count.
     return top == CUDART_INF ? (z == top ? 1.0 : 0.0) : exp_down((z - top) * cold, two_to);
+}
+__device__ __forceinline__ void weights_of(const double (&z)[8], double top, double cold, const double* two_to,
+                                           double (&w)[8]) {
+    if (top == CUDART_INF) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = z[i] == top ? 1.0 : 0.0;
+    } else {  // eight at a time: an exponential is a chain of some fifteen operations
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = exp_down((z[i] - top) * cold, two_to);
+    }
 }
 
 // What a part of a row knows: its weights, its largest logit and the lowest
@@ -328,185 +358,167 @@ struct Part {
     uint32_t bad;
 };
 
-// A cluster of blocks takes a row, each block a run of rounds, a warp of it
-// Steps x 32 groups of a round.  One pass over the logits gives each of these
-// stretches its weights (by its own top, so the row's is not needed first); the
+// A cluster of blocks takes a row, each block a run of steps of 256 symbols,
+// a step a warp.  One pass over the logits gives every step its weights (by a
+// value near its own largest logit, so the row's is not needed first); the
 // blocks exchange theirs through distributed shared memory, which says in which
-// stretch the running sum passes u * total, and one warp walks that stretch
-// again.  Everything is in 64 bits: among 131,072 borders between symbols a
-// float32 sum would put one in a hundred draws on the wrong side.
-template <typename T, int Warps, int Steps>
-struct PickShape {
-    static constexpr uint32_t kSpan = Warps * Steps * 256;  // symbols of a round
-    static constexpr uint32_t kMaxRounds = 64;
-};
+// step the running sum passes u * total, and one warp walks that step again.
+// Everything is in 64 bits: among 131,072 borders between symbols a float32 sum
+// would put one in a hundred draws on the wrong side.  What bounds it is the 64-bit
+// exponential, some 16 operations a symbol: 8.4 million symbols take 9 us at the
+// card's rate for them, their logits 3 us at its bandwidth.
+constexpr uint32_t kStepSymbols = 256;
+constexpr uint32_t kPickWindow = 96;  // steps whose counts are in shared memory at a time
 
-template <typename T, int Warps, int Steps>
-__global__ void __launch_bounds__(32 * Warps) pick_kernel(const __grid_constant__ LogitArgs a, uint32_t rounds) {
-    using S = PickShape<T, Warps, Steps>;
-    __shared__ __align__(16) uint32_t counts[S::kSpan];
+template <typename T, int Warps>
+__global__ void __launch_bounds__(32 * Warps) pick_kernel(const __grid_constant__ LogitArgs a, uint32_t steps) {
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    Weights* weights = reinterpret_cast<Weights*>(dynamic);              // [steps]
+    uint32_t* counts = reinterpret_cast<uint32_t*>(weights + steps);     // of a window, if there is a history
     __shared__ double two_to[32];
-    __shared__ Weights stretches[S::kMaxRounds * Warps];
-    __shared__ Part warp_parts[Warps], mine;
-    __shared__ double warp_best[Warps], block_best;
-    __shared__ uint32_t chosen;  // stretch
-    __shared__ double before, target, row_best, row_total;
+    __shared__ double warp_best[Warps];
+    __shared__ uint32_t warp_at[Warps], warp_bad[Warps];
+    __shared__ Part mine;
+    __shared__ double block_best, before, target, row_best, row_total;
+    __shared__ uint32_t chosen;  // step
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t blocks = cluster.num_blocks(), rank = cluster.block_rank();
     const uint32_t at = blockIdx.x / blocks, lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     const Row<T> row(static_cast<const T*>(a.logits) + (int64_t)at * a.logits_stride, a.vocabulary);
+    const int32_t block_first = row.first + (int32_t)(rank * steps * kStepSymbols);
+    const auto symbol_of = [&](uint32_t step) { return block_first + (int32_t)(step * kStepSymbols + lane * 8); };
+    const auto inside = [&](uint32_t step) { return step < steps && symbol_of(step) < (int32_t)a.vocabulary; };
+    Eight<T> next;
+    if (inside(warp)) next = row.read(symbol_of(warp));
     const RowRules k = row_rules(a.rules, at);
     const float temperature = a.temperature ? a.temperature[at] : a.temperature_value;
     const bool greedy = temperature == 0.0f;
     const double heat = greedy ? 1.0 : (double)temperature, cold = 1.0 / heat;
+    const double reciprocal = 1.0 / (double)k.repetition;
     for (uint32_t j = threadIdx.x; j < 32; j += 32 * Warps) two_to[j] = kTwoTo[j];
 
-    // Symbols of a group after the rules; the logits read before.
-    const auto symbols_at = [&](uint32_t round, uint32_t w, int step) {
-        return row.first + (int32_t)((rank * rounds + round) * S::kSpan + ((w * Steps + step) * 32 + lane) * 8);
-    };
-    // Whether the rules leave a whole group as it is, but for the bias.
-    const auto plain = [&](int32_t v, int32_t first) {
-        if (!row.whole(v) || k.mask.eight(v, a.vocabulary) != 0xffu) return false;
-        if (!k.length) return true;
-        const uint4* c = reinterpret_cast<const uint4*>(counts + (v - first));
-        return ((c[0].x | c[0].y) | (c[0].z | c[0].w) | (c[1].x | c[1].y) | (c[1].z | c[1].w)) == 0;
-    };
-    const auto adjust = [&](const Eight<T>& e, const float (&bias)[8], int32_t v, int32_t first, double (&z)[8]) {
-        const uint32_t ok = k.mask.eight(v, a.vocabulary);
+    // Bit i: symbol v + i is in the row and allowed.
+    const auto allowed_at = [&](int32_t v) {
+        uint32_t ok = k.mask.eight(v, a.vocabulary);
+        if (!row.whole(v))
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t count = k.length ? counts[(uint32_t)(v + i - first)] : 0u;
-            z[i] = adjusted((double)e[i], count, k, bias[i], row.in(v + i) && (ok >> i & 1u));
+            for (int i = 0; i < 8; ++i)
+                if (!row.in(v + i)) ok &= ~(1u << i);
+        return ok;
+    };
+    // The logits of a group after the rules; `window`: the first symbol of the counts.
+    const auto adjust = [&](const Eight<T>& e, int32_t v, int32_t window, double (&z)[8]) {
+        float bias[8] = {};
+        read_bias(k, row, v, bias);
+        const uint32_t ok = allowed_at(v);
+        uint4 c[2] = {};
+        if (k.length) {
+            c[0] = *reinterpret_cast<const uint4*>(counts + (v - window));
+            c[1] = *reinterpret_cast<const uint4*>(counts + (v - window) + 4);
+        }
+        const uint32_t count[8] = {c[0].x, c[0].y, c[0].z, c[0].w, c[1].x, c[1].y, c[1].z, c[1].w};
+        if (ok == 0xffu && ((c[0].x | c[0].y) | (c[0].z | c[0].w) | (c[1].x | c[1].y) | (c[1].z | c[1].w)) == 0) {
+            // nothing of these was said before, and nothing is masked
+#pragma unroll
+            for (int i = 0; i < 8; ++i) z[i] = k.bias ? (double)e[i] + (double)bias[i] : (double)e[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                z[i] = adjusted((double)e[i], count[i], k, reciprocal, bias[i], ok >> i & 1u);
         }
     };
 
-    Part part{no_weights(), kAll, !(temperature >= 0.0f)};
     double best_value = -CUDART_INF;
-    for (uint32_t round = 0; round < rounds; ++round) {
-        const int32_t first = row.first + (int32_t)((rank * rounds + round) * S::kSpan);
-        if (first >= (int32_t)a.vocabulary) {
-            if (lane == 0) stretches[round * Warps + warp] = no_weights();
-            continue;
-        }
-        Eight<T> e[Steps];
-#pragma unroll
-        for (int step = 0; step < Steps; ++step) {
-            const int32_t v = symbols_at(round, warp, step);
-            if (v < (int32_t)a.vocabulary) e[step] = row.read(v);
-        }
-        __syncthreads();  // the table, or the counts of the round before
-        if (k.length) count_history<S::kSpan>(k, first, counts);
-        Weights w = no_weights();
-#pragma unroll
-        for (int step = 0; step < Steps; ++step) {
-            const int32_t v = symbols_at(round, warp, step);
-            if (v >= (int32_t)a.vocabulary) continue;
-            double z[8], top;
-            const bool as_is = plain(v, first);
-            if (as_is && !k.bias) {
-                // Nothing of these was said before, and nothing is masked: a float's order is the double's.
-                const float most = e[step].largest();
-                top = (double)most;
-                if (top > best_value) {
-                    best_value = top;
-#pragma unroll
-                    for (int i = 7; i >= 0; --i)
-                        if (e[step][i] == most) part.best = (uint32_t)(v + i);
-                }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    z[i] = (double)e[step][i];
-                    part.bad |= e[step][i] != e[step][i];
-                }
+    float best_rough = -CUDART_INF_F;
+    uint32_t best = kAll, bad = !(temperature >= 0.0f);
+    for (uint32_t first = 0; first < steps; first += kPickWindow) {
+        const int32_t window = block_first + (int32_t)(first * kStepSymbols);
+        const uint32_t past = min(first + kPickWindow, steps);
+        if (first) __syncthreads();  // the counts of the window before are read
+        if (k.length)
+            count_history(k, window, (past - first) * kStepSymbols, counts);
+        else if (first == 0)
+            __syncthreads();  // the table of powers
+        for (uint32_t step = first + warp; step < past; step += Warps) {
+            const Eight<T> e = next;
+            const int32_t v = symbol_of(step);
+            if (inside(step + Warps)) next = row.read(symbol_of(step + Warps));
+            double z[8];
+            if (inside(step)) {
+                adjust(e, v, window, z);
             } else {
-                float bias[8] = {};
-                read_bias(k, row, v, bias);
-                if (as_is) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) z[i] = (double)e[step][i] + (double)bias[i];
-                } else {
-                    adjust(e[step], bias, v, first, z);
-                }
-                top = -CUDART_INF;
+                for (int i = 0; i < 8; ++i) z[i] = -CUDART_INF;
+            }
+            // Rounded to float for the comparisons that need no more.
+            float most = -CUDART_INF_F;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    part.bad |= z[i] != z[i];
-                    if (z[i] > best_value) best_value = z[i], part.best = (uint32_t)(v + i);
-                    top = fmax(top, z[i]);
-                }
+            for (int i = 0; i < 8; ++i) {
+                const float rough = (float)z[i];
+                bad |= rough != rough;
+                most = fmaxf(most, rough);
             }
-            if (top > w.top) {
-                w.sum = w.top == -CUDART_INF ? 0.0 : w.sum * weight_of(w.top, top, cold, two_to);
-                w.top = top;
-            }
-            if (w.top != -CUDART_INF) {
+            if (!(most < best_rough - fabsf(best_rough) * 0x1p-21f)) {  // float's order is double's but for neighbours
 #pragma unroll
-                for (int i = 0; i < 8; ++i) w.sum += weight_of(z[i], w.top, cold, two_to);
+                for (int i = 0; i < 8; ++i)
+                    if (z[i] > best_value) best_value = z[i], best = (uint32_t)(v + i);
+                best_rough = fmaxf(best_rough, most);
             }
+            double top = (double)warp_max(most);
+            if (!(fabs(top) < 1e38)) {  // what float calls infinite may not be
+                top = z[0];
+#pragma unroll
+                for (int i = 1; i < 8; ++i) top = fmax(top, z[i]);
+                for (int off = 16; off > 0; off >>= 1) top = fmax(top, __shfl_xor_sync(kAll, top, off));
+            }
+            double sum = 0.0;
+            if (top != -CUDART_INF) {
+                double w[8];
+                weights_of(z, top, cold, two_to, w);
+                sum = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+                for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(kAll, sum, off);
+            }
+            if (lane == 0) weights[step] = {top, sum};
         }
-        // The warp's, by its own top.
-        double top = w.top;
-        for (int off = 16; off > 0; off >>= 1) top = fmax(top, __shfl_xor_sync(kAll, top, off));
-        double sum = w.top == -CUDART_INF ? 0.0 : w.sum * weight_of(w.top, top, cold, two_to);
-        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(kAll, sum, off);
-        if (lane == 0) stretches[round * Warps + warp] = {top, sum};
     }
-    // The block's part.
-    for (int off = 16; off > 0; off >>= 1) {
-        const double v = __shfl_xor_sync(kAll, best_value, off);
-        const uint32_t b = __shfl_xor_sync(kAll, part.best, off);
-        if (v > best_value || (v == best_value && b < part.best)) best_value = v, part.best = b;
-        part.bad |= __shfl_xor_sync(kAll, part.bad, off);
-    }
-    if (lane == 0) warp_parts[warp] = part, warp_best[warp] = best_value;
-    __syncthreads();
-    if (warp == 0) {
-        Part p = warp_parts[lane < Warps ? lane : 0];
-        best_value = warp_best[lane < Warps ? lane : 0];
-        for (int off = Warps / 2; off > 0; off >>= 1) {
+    // The block's part: its largest logit, and its weights by that.
+    const auto join_best = [&](uint32_t width) {
+        for (uint32_t off = width / 2; off > 0; off >>= 1) {
             const double v = __shfl_xor_sync(kAll, best_value, off);
-            const uint32_t b = __shfl_xor_sync(kAll, p.best, off);
-            if (v > best_value || (v == best_value && b < p.best)) best_value = v, p.best = b;
-            p.bad |= __shfl_xor_sync(kAll, p.bad, off);
-        }
-        // by the block's largest logit, which is the top of one of its stretches
-        best_value = __shfl_sync(kAll, best_value, 0);
-        double sum = 0.0;
-        for (uint32_t j = lane; j < rounds * Warps; j += 32) {
-            const Weights w = stretches[j];
-            if (w.top != -CUDART_INF) sum += w.sum * weight_of(w.top, best_value, cold, two_to);
-        }
-        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(kAll, sum, off);
-        p.weights = {best_value, sum};
-        if (lane == 0) mine = p, block_best = best_value;
-    }
-    if (blocks > 1)
-        cluster.sync();
-    else
-        __syncthreads();
-
-    // The row's, the same in every block.
-    if (warp == 0) {
-        Part p{no_weights(), kAll, 0};
-        double value = -CUDART_INF;
-        if (lane < blocks) {
-            p = *cluster.map_shared_rank(&mine, lane);
-            value = *cluster.map_shared_rank(&block_best, lane);
-        }
-        double top = value;
-        uint32_t best = p.best, bad = p.bad;
-        for (int off = 16; off > 0; off >>= 1) {
-            const double v = __shfl_xor_sync(kAll, top, off);
             const uint32_t b = __shfl_xor_sync(kAll, best, off);
-            if (v > top || (v == top && b < best)) top = v, best = b;
+            if (v > best_value || (v == best_value && b < best)) best_value = v, best = b;
             bad |= __shfl_xor_sync(kAll, bad, off);
         }
-        uint32_t pick = kAll - 1u;  // nothing to walk
+    };
+    // A sum of weights by another value.
+    const auto by = [&](const Weights& w, double top) {
+        return w.top == -CUDART_INF ? 0.0 : w.sum * weight_of(w.top, top, cold, two_to);
+    };
+    join_best(32);
+    if (lane == 0) warp_best[warp] = best_value, warp_at[warp] = best, warp_bad[warp] = bad;
+    __syncthreads();
+    if (warp == 0) {
+        const uint32_t w = lane % Warps;
+        best_value = warp_best[w], best = warp_at[w], bad = warp_bad[w];
+        join_best(Warps);
+        double sum = 0.0;
+        for (uint32_t j = lane; j < steps; j += 32) sum += by(weights[j], best_value);
+        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(kAll, sum, off);
+        if (lane == 0) mine = {{best_value, sum}, best, bad}, block_best = best_value;
+        __syncwarp();
+    }
+    if (blocks > 1) cluster.sync();
+
+    // The row's, the same in every block; its first warp goes on.
+    if (warp == 0) {
+        const Part part = lane < blocks ? (blocks > 1 ? *cluster.map_shared_rank(&mine, lane) : mine)
+                                        : Part{no_weights(), kAll, 0};
+        best_value = lane < blocks ? part.weights.top : -CUDART_INF;
+        best = part.best, bad = part.bad;
+        join_best(32);
+        uint32_t pick = kAll;  // nothing to walk
         if (!bad && best != kAll) {
-            const double share = lane < blocks && p.weights.top != -CUDART_INF
-                                     ? p.weights.sum * weight_of(p.weights.top, top, cold, two_to)
-                                     : 0.0;
+            const double share = blocks == 1 && lane == 0 ? part.weights.sum : by(part.weights, best_value);
             double total = 0.0;
             for (uint32_t j = 0; j < blocks; ++j) total += __shfl_sync(kAll, share, j);
             if (greedy) {
@@ -515,7 +527,7 @@ __global__ void __launch_bounds__(32 * Warps) pick_kernel(const __grid_constant_
                     if (a.log_probability) a.log_probability[at] = (float)-log(total);
                 }
             } else {
-                // The block, then its stretch, in which the running sum passes u * total.
+                // The block, then its step, in which the running sum passes u * total.
                 const double goal = a.uniforms[at] * total;
                 double sum = 0.0, sum_before = 0.0;
                 uint32_t owner = kAll, last = 0;
@@ -530,25 +542,28 @@ __global__ void __launch_bounds__(32 * Warps) pick_kernel(const __grid_constant_
                 }
                 if (owner == kAll) owner = last;  // u is nearly 1, and the sums were rounded
                 if (rank == owner) {
-                    double running = sum_before, stretch_before = sum_before;
-                    uint32_t found = kAll, last_stretch = 0;
-                    for (uint32_t base = 0; base < rounds * Warps && found == kAll; base += 32) {
+                    double running = sum_before, step_before = sum_before;
+                    uint32_t found = kAll, last_step = 0;
+                    for (uint32_t base = 0; base < steps && found == kAll; base += 32) {
                         const uint32_t j = base + lane;
-                        Weights w = no_weights();
-                        if (j < rounds * Warps) w = stretches[j];
-                        const double s = w.top == -CUDART_INF ? 0.0 : w.sum * weight_of(w.top, top, cold, two_to);
-                        for (uint32_t l = 0; l < 32 && found == kAll; ++l) {
-                            const double one = __shfl_sync(kAll, s, l);
-                            if (one > 0.0) {
-                                stretch_before = running;
-                                last_stretch = base + l;
-                                if (running + one > goal) found = base + l;
-                                running += one;
-                            }
+                        const double s = j < steps ? by(weights[j], best_value) : 0.0;
+                        double through = s;
+                        for (int off = 1; off < 32; off <<= 1) {
+                            const double o = __shfl_up_sync(kAll, through, off);
+                            if (lane >= (uint32_t)off) through += o;
                         }
+                        const uint32_t some = __ballot_sync(kAll, s > 0.0);
+                        const uint32_t hits = __ballot_sync(kAll, s > 0.0 && running + through > goal);
+                        if (some) {
+                            const int from = hits ? __ffs(hits) - 1 : 31 - __clz(some);
+                            last_step = base + from;
+                            if (hits) found = last_step;
+                            step_before = running + __shfl_sync(kAll, through - s, from);
+                        }
+                        running += __shfl_sync(kAll, through, 31);
                     }
-                    pick = found != kAll ? found : last_stretch;
-                    if (lane == 0) before = stretch_before, target = goal, row_best = top, row_total = total;
+                    pick = found != kAll ? found : last_step;
+                    if (lane == 0) before = step_before, target = goal, row_best = best_value, row_total = total;
                 }
             }
         } else if (rank == 0 && lane == 0) {
@@ -557,72 +572,53 @@ __global__ void __launch_bounds__(32 * Warps) pick_kernel(const __grid_constant_
         }
         if (lane == 0) chosen = pick;
     }
-    // No block leaves, or changes what the others read, before they have read it.
+    // No block leaves before the others have read its part.
     if (blocks > 1)
         cluster.sync();
     else
         __syncthreads();
-    if (chosen == kAll - 1u) return;
+    if (chosen == kAll) return;
 
-    // One block walks the stretch.
-    const uint32_t round = chosen / Warps, w = chosen % Warps;
-    const int32_t first = row.first + (int32_t)((rank * rounds + round) * S::kSpan);
-    if (k.length) count_history<S::kSpan>(k, first, counts);
+    // The step's counts are there, unless it lies in an earlier window.
+    const uint32_t first = chosen / kPickWindow * kPickWindow;
+    const int32_t window = block_first + (int32_t)(first * kStepSymbols);
+    if (k.length && steps - first > kPickWindow) count_history(k, window, kPickWindow * kStepSymbols, counts);
     if (warp != 0) return;
-    const double top = row_best, total = row_total, goal = target;
-    double running = before;
-    uint32_t symbol = kAll, last = 0;
-    double symbol_z = 0.0, last_z = 0.0;
-    for (int step = 0; step < Steps && symbol == kAll; ++step) {
-        const int32_t v = symbols_at(round, w, step);
-        double z[8], weight[8], sum = 0.0;
-        if (v < (int32_t)a.vocabulary) {
-            float bias[8] = {};
-            read_bias(k, row, v, bias);
-            adjust(row.read(v), bias, v, first, z);
-        } else {
+    const double top = row_best, goal = target;
+    const int32_t v = symbol_of(chosen);
+    double z[8], w[8], sum = 0.0;
+    if (v < (int32_t)a.vocabulary) {
+        adjust(row.read(v), v, window, z);
+    } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) z[i] = -CUDART_INF;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            weight[i] = weight_of(z[i], top, cold, two_to);
-            sum += weight[i];
-        }
-        double through = sum;  // of the lanes up to this one
-        for (int off = 1; off < 32; off <<= 1) {
-            const double o = __shfl_up_sync(kAll, through, off);
-            if (lane >= (uint32_t)off) through += o;
-        }
-        double mine_before = running + (through - sum);
-        uint32_t here = kAll, here_last = kAll;
-        double here_z = 0.0, here_last_z = 0.0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            mine_before += weight[i];
-            if (weight[i] > 0.0) {
-                here_last = (uint32_t)(v + i), here_last_z = z[i];
-                if (here == kAll && mine_before > goal) here = (uint32_t)(v + i), here_z = z[i];
-            }
-        }
-        const uint32_t hits = __ballot_sync(kAll, here != kAll), some = __ballot_sync(kAll, here_last != kAll);
-        if (hits) {
-            const int from = __ffs(hits) - 1;
-            symbol = __shfl_sync(kAll, here, from);
-            symbol_z = __shfl_sync(kAll, here_z, from);
-        }
-        if (some) {
-            const int from = 31 - __clz(some);
-            last = __shfl_sync(kAll, here_last, from);
-            last_z = __shfl_sync(kAll, here_last_z, from);
-        }
-        running += __shfl_sync(kAll, through, 31);
+        for (int i = 0; i < 8; ++i) z[i] = -CUDART_INF;
     }
-    if (symbol == kAll) symbol = last, symbol_z = last_z;
-    if (lane == 0) {
-        a.symbols[at] = (int32_t)symbol;
+    weights_of(z, top, cold, two_to, w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += w[i];
+    double through = sum;  // of the lanes up to this one
+    for (int off = 1; off < 32; off <<= 1) {
+        const double o = __shfl_up_sync(kAll, through, off);
+        if (lane >= (uint32_t)off) through += o;
+    }
+    double running = before + (through - sum);
+    uint32_t hit = kAll, last = kAll;
+    double hit_z = 0.0, last_z = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        running += w[i];
+        if (w[i] > 0.0) {
+            last = (uint32_t)(v + i), last_z = z[i];
+            if (hit == kAll && running > goal) hit = last, hit_z = z[i];
+        }
+    }
+    // The first lane with a hit, or, the sums having been rounded, the last with any weight.
+    const uint32_t hits = __ballot_sync(kAll, hit != kAll), some = __ballot_sync(kAll, last != kAll);
+    if (hits ? lane == (uint32_t)__ffs(hits) - 1u : lane == 31u - __clz(some)) {
+        const double logit = hits ? hit_z : last_z;
+        a.symbols[at] = (int32_t)(hits ? hit : last);
         if (a.log_probability)
-            a.log_probability[at] = (float)((symbol_z == top ? 0.0 : (symbol_z - top) / heat) - log(total));
+            a.log_probability[at] = (float)((logit == top ? 0.0 : (logit - top) / heat) - log(row_total));
     }
 }
 
@@ -640,15 +636,6 @@ struct LossArgs {
     void* gradient;
     int64_t gradient_stride;
 };
-
-__device__ __forceinline__ float warp_max(float v) {
-    for (int off = 16; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, off));
-    return v;
-}
-__device__ __forceinline__ float warp_sum(float v) {
-    for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(kAll, v, off);
-    return v;
-}
 
 __device__ __forceinline__ float exp2_of(float x) {
     float y;
@@ -849,19 +836,25 @@ void dispatch(int dtype, Body&& body) {
 }
 
 // A block a row, or a cluster of up to eight while that leaves SMs without work.
-template <typename T, int Warps, int Steps>
+template <typename T, int Warps>
 void launch_pick(const LogitArgs& a, cudaStream_t stream) {
-    using S = PickShape<T, Warps, Steps>;
-    const uint32_t all = (a.vocabulary + 7 + S::kSpan - 1) / S::kSpan;
+    const uint32_t all = (a.vocabulary + 7 + kStepSymbols - 1) / kStepSymbols;
     uint32_t blocks = 1;
-    while (blocks < 8 && blocks < all && (uint64_t)a.rows * blocks < 512) blocks *= 2;
-    while (blocks < 8 && (all + blocks - 1) / blocks > S::kMaxRounds) blocks *= 2;
-    const uint32_t rounds = (all + blocks - 1) / blocks;
-    require(rounds <= S::kMaxRounds, "the vocabulary is too large for one pick");
+    while (blocks < 8 && blocks * 2 * Warps <= all && (uint64_t)a.rows * blocks < 512) blocks *= 2;
+    if (all > 2048) blocks = 8;
+    const uint32_t steps = (all + blocks - 1) / blocks;
+    require(steps <= 4096, "the vocabulary is too large for one pick");
     require((uint64_t)a.rows * blocks < (1ull << 31), "too many rows for one call");
+    const auto kernel = pick_kernel<T, Warps>;
+    const size_t shared = steps * sizeof(Weights) +
+                          (a.rules.history ? std::min(steps, kPickWindow) * kStepSymbols * sizeof(uint32_t) : 0);
+    check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               (int)(4096 * sizeof(Weights) + kPickWindow * kStepSymbols * sizeof(uint32_t))),
+          "shared memory");
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(a.rows * blocks);
     config.blockDim = dim3(32 * Warps);
+    config.dynamicSmemBytes = shared;
     config.stream = stream;
     cudaLaunchAttribute cluster{};
     cluster.id = cudaLaunchAttributeClusterDimension;
@@ -869,7 +862,7 @@ void launch_pick(const LogitArgs& a, cudaStream_t stream) {
     cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
     config.attrs = &cluster;
     config.numAttrs = 1;
-    check(cudaLaunchKernelEx(&config, pick_kernel<T, Warps, Steps>, a, rounds), "pick_kernel");
+    check(cudaLaunchKernelEx(&config, kernel, a, steps), "pick_kernel");
 }
 
 // A warp a row while it holds the row in 32 registers a lane, a block above.
@@ -967,10 +960,10 @@ int leo_b200_pick_symbols(int device, int dtype, const void* logits, int64_t log
             a.symbols = symbols;
             a.log_probability = log_probability;
             DeviceScope scope(device);
-            if (vocabulary + 7 <= PickShape<T, 4, 1>::kSpan)
-                launch_pick<T, 4, 1>(a, (cudaStream_t)stream);
+            if (vocabulary + 7 <= 4 * kStepSymbols)
+                launch_pick<T, 4>(a, (cudaStream_t)stream);
             else
-                launch_pick<T, 8, 4>(a, (cudaStream_t)stream);
+                launch_pick<T, 8>(a, (cudaStream_t)stream);
         });
     });
 }
