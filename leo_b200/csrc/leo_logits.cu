@@ -295,42 +295,48 @@ __global__ void __launch_bounds__(kAdjustThreads) adjust_kernel(const __grid_con
     }
 }
 
-// exp(x) for x <= 0 after Tang's table-driven method (P. T. P. Tang, ACM TOMS
-// 15, 1989): x = (32 q + j) ln 2 / 32 + r, exp x = 2^q 2^(j/32) exp r, with a
-// Taylor polynomial of degree 6 for |r| <= ln 2 / 64 (its rest is below 2^-58)
-// and ln 2 / 32 in two parts so that r is exact to the last bits.
-__device__ const double kTwoTo[32] = {
-    0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0,
-    0x1.172b83c7d517bp+0, 0x1.1d4873168b9aap+0, 0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0,
-    0x1.306fe0a31b715p+0, 0x1.371a7373aa9cbp+0, 0x1.3dea64c123422p+0, 0x1.44e086061892dp+0,
-    0x1.4bfdad5362a27p+0, 0x1.5342b569d4f82p+0, 0x1.5ab07dd485429p+0, 0x1.6247eb03a5585p+0,
-    0x1.6a09e667f3bcdp+0, 0x1.71f75e8ec5f74p+0, 0x1.7a11473eb0187p+0, 0x1.82589994cce13p+0,
-    0x1.8ace5422aa0dbp+0, 0x1.93737b0cdc5e5p+0, 0x1.9c49182a3f090p+0, 0x1.a5503b23e255dp+0,
-    0x1.ae89f995ad3adp+0, 0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0,
-    0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0, 0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0};
-__device__ __forceinline__ double exp_down(double x, const double* two_to) {
+// exp(y ln 2 / 64) for y <= 0 after Tang's table-driven method (P. T. P. Tang,
+// ACM TOMS 15, 1989): y = 64 q + j + d with |d| <= 1/2, so the value is
+// 2^q 2^(j/64) exp(d ln 2 / 64), the last by its Taylor polynomial of degree 5
+// in d (its rest is below 2^-58).  Below e^-708 it is 0, which no double sum
+// beside a weight of 1 can tell.
+constexpr uint32_t kPowers = 64;
+__device__ const double kTwoTo[kPowers] = {
+    0x1.0000000000000p+0, 0x1.02c9a3e778061p+0, 0x1.059b0d3158574p+0, 0x1.0874518759bc8p+0,
+    0x1.0b5586cf9890fp+0, 0x1.0e3ec32d3d1a2p+0, 0x1.11301d0125b51p+0, 0x1.1429aaea92de0p+0,
+    0x1.172b83c7d517bp+0, 0x1.1a35beb6fcb75p+0, 0x1.1d4873168b9aap+0, 0x1.2063b88628cd6p+0,
+    0x1.2387a6e756238p+0, 0x1.26b4565e27cddp+0, 0x1.29e9df51fdee1p+0, 0x1.2d285a6e4030bp+0,
+    0x1.306fe0a31b715p+0, 0x1.33c08b26416ffp+0, 0x1.371a7373aa9cbp+0, 0x1.3a7db34e59ff7p+0,
+    0x1.3dea64c123422p+0, 0x1.4160a21f72e2ap+0, 0x1.44e086061892dp+0, 0x1.486a2b5c13cd0p+0,
+    0x1.4bfdad5362a27p+0, 0x1.4f9b2769d2ca7p+0, 0x1.5342b569d4f82p+0, 0x1.56f4736b527dap+0,
+    0x1.5ab07dd485429p+0, 0x1.5e76f15ad2148p+0, 0x1.6247eb03a5585p+0, 0x1.6623882552225p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.6dfb23c651a2fp+0, 0x1.71f75e8ec5f74p+0, 0x1.75feb564267c9p+0,
+    0x1.7a11473eb0187p+0, 0x1.7e2f336cf4e62p+0, 0x1.82589994cce13p+0, 0x1.868d99b4492edp+0,
+    0x1.8ace5422aa0dbp+0, 0x1.8f1ae99157736p+0, 0x1.93737b0cdc5e5p+0, 0x1.97d829fde4e50p+0,
+    0x1.9c49182a3f090p+0, 0x1.a0c667b5de565p+0, 0x1.a5503b23e255dp+0, 0x1.a9e6b5579fdbfp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b33a2b84f15fbp+0, 0x1.b7f76f2fb5e47p+0, 0x1.bcc1e904bc1d2p+0,
+    0x1.c199bdd85529cp+0, 0x1.c67f12e57d14bp+0, 0x1.cb720dcef9069p+0, 0x1.d072d4a07897cp+0,
+    0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
+    0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0};
+constexpr double kSixtyFourths = 0x1.71547652b82fep+6;  // 64 / ln 2
+__device__ __forceinline__ double exp_down(double y, const double* two_to) {
     const double magic = 0x1.8p52;
-    // -746 and below (-inf too, by the bits of its high word): 0
-    const bool none = (uint32_t)__double2hiint(x) >= 0xc0875000u;
-    if (none) x = 0.0;
-    const double shifted = fma(x, 0x1.71547652b82fep+5, magic);
+    // y < -65,372 (-inf too, by the bits of its high word)
+    const bool none = (uint32_t)__double2hiint(y) >= 0xc0efeb80u;
+    const double shifted = y + magic;
     const int32_t n = __double2loint(shifted);
-    const double whole = shifted - magic;
-    double r = fma(whole, -0x1.62e42fee00000p-6, x);
-    r = fma(whole, -0x1.a39ef35793c76p-38, r);
-    double p = fma(r, 1.0 / 720.0, 1.0 / 120.0);
-    p = fma(p, r, 1.0 / 24.0);
-    p = fma(p, r, 1.0 / 6.0);
-    p = fma(p, r, 0.5);
-    p = fma(p, r, 1.0);
-    const double scale = two_to[n & 31];
-    // 2^q in two factors, so that a subnormal result is rounded once
-    const int32_t q = n >> 5, half = q >> 1;
-    return fma(scale, p * r, scale) * __hiloint2double((1023 + half) << 20, 0) *
-           __hiloint2double(none ? 0 : (1023 + (q - half)) << 20, 0);
+    const double d = y - (shifted - magic);
+    double p = fma(d, 0x1.5d87fe78a6731p-40, 0x1.3b2ab6fba4e77p-31);
+    p = fma(p, d, 0x1.c6b08d704a0c0p-23);
+    p = fma(p, d, 0x1.ebfbdff82c58fp-15);
+    p = fma(p, d, 0x1.62e42fefa39efp-7) * d;
+    const double scale = two_to[n & 63];
+    const double v = fma(scale, p, scale);
+    const int32_t high = __double2hiint(v) + ((n >> 6) << 20);
+    return none ? 0.0 : __hiloint2double(high, __double2loint(v));
 }
 
-// A sum of weights exp((z - top) / heat), by its own top.
+// A sum of weights exp((z - top) / heat), by its own top; `cold` is 64 / ln 2 / heat.
 struct Weights {
     double top, sum;
 };
@@ -375,7 +381,7 @@ __global__ void __launch_bounds__(32 * Warps) pick_kernel(const __grid_constant_
     extern __shared__ __align__(16) unsigned char dynamic[];
     Weights* weights = reinterpret_cast<Weights*>(dynamic);              // [steps]
     uint32_t* counts = reinterpret_cast<uint32_t*>(weights + steps);     // of a window, if there is a history
-    __shared__ double two_to[32];
+    __shared__ double two_to[kPowers];
     __shared__ double warp_best[Warps];
     __shared__ uint32_t warp_at[Warps], warp_bad[Warps];
     __shared__ Part mine;
@@ -389,13 +395,16 @@ __global__ void __launch_bounds__(32 * Warps) pick_kernel(const __grid_constant_
     const auto symbol_of = [&](uint32_t step) { return block_first + (int32_t)(step * kStepSymbols + lane * 8); };
     const auto inside = [&](uint32_t step) { return step < steps && symbol_of(step) < (int32_t)a.vocabulary; };
     Eight<T> next;
+    float next_bias[8] = {};
     if (inside(warp)) next = row.read(symbol_of(warp));
     const RowRules k = row_rules(a.rules, at);
+    if (inside(warp)) read_bias(k, row, symbol_of(warp), next_bias);
     const float temperature = a.temperature ? a.temperature[at] : a.temperature_value;
     const bool greedy = temperature == 0.0f;
-    const double heat = greedy ? 1.0 : (double)temperature, cold = 1.0 / heat;
+    const double uniform = a.uniforms ? a.uniforms[at] : 0.0;
+    const double heat = greedy ? 1.0 : (double)temperature, cold = kSixtyFourths / heat;
     const double reciprocal = 1.0 / (double)k.repetition;
-    for (uint32_t j = threadIdx.x; j < 32; j += 32 * Warps) two_to[j] = kTwoTo[j];
+    for (uint32_t j = threadIdx.x; j < kPowers; j += 32 * Warps) two_to[j] = kTwoTo[j];
 
     // Bit i: symbol v + i is in the row and allowed.
     const auto allowed_at = [&](int32_t v) {
@@ -406,10 +415,10 @@ __global__ void __launch_bounds__(32 * Warps) pick_kernel(const __grid_constant_
                 if (!row.in(v + i)) ok &= ~(1u << i);
         return ok;
     };
-    // The logits of a group after the rules; `window`: the first symbol of the counts.
-    const auto adjust = [&](const Eight<T>& e, int32_t v, int32_t window, double (&z)[8]) {
-        float bias[8] = {};
-        read_bias(k, row, v, bias);
+    // The logits of a group after the rules, and roughly so, rounded to float once or twice;
+    // `window`: the first symbol of the counts.
+    const auto adjust = [&](const Eight<T>& e, const float (&bias)[8], int32_t v, int32_t window, double (&z)[8],
+                            float (&rough)[8]) {
         const uint32_t ok = allowed_at(v);
         uint4 c[2] = {};
         if (k.length) {
@@ -417,14 +426,23 @@ __global__ void __launch_bounds__(32 * Warps) pick_kernel(const __grid_constant_
             c[1] = *reinterpret_cast<const uint4*>(counts + (v - window) + 4);
         }
         const uint32_t count[8] = {c[0].x, c[0].y, c[0].z, c[0].w, c[1].x, c[1].y, c[1].z, c[1].w};
-        if (ok == 0xffu && ((c[0].x | c[0].y) | (c[0].z | c[0].w) | (c[1].x | c[1].y) | (c[1].z | c[1].w)) == 0) {
-            // nothing of these was said before, and nothing is masked
 #pragma unroll
-            for (int i = 0; i < 8; ++i) z[i] = k.bias ? (double)e[i] + (double)bias[i] : (double)e[i];
-        } else {
+        for (int i = 0; i < 8; ++i) {
+            z[i] = k.bias ? (double)e[i] + (double)bias[i] : (double)e[i];
+            rough[i] = k.bias ? e[i] + bias[i] : e[i];
+        }
+        if (((c[0].x | c[0].y) | (c[0].z | c[0].w) | (c[1].x | c[1].y) | (c[1].z | c[1].w)) != 0) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                z[i] = adjusted((double)e[i], count[i], k, reciprocal, bias[i], ok >> i & 1u);
+                if (count[i]) {  // a few in a step: most of a vocabulary has not been said
+                    z[i] = adjusted((double)e[i], count[i], k, reciprocal, bias[i], true);
+                    rough[i] = (float)z[i];
+                }
+        }
+        if (ok != 0xffu) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (!(ok >> i & 1u)) z[i] = -CUDART_INF, rough[i] = -CUDART_INF_F;
         }
     };
 
@@ -441,22 +459,26 @@ __global__ void __launch_bounds__(32 * Warps) pick_kernel(const __grid_constant_
             __syncthreads();  // the table of powers
         for (uint32_t step = first + warp; step < past; step += Warps) {
             const Eight<T> e = next;
+            float bias[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) bias[i] = next_bias[i];
             const int32_t v = symbol_of(step);
-            if (inside(step + Warps)) next = row.read(symbol_of(step + Warps));
+            if (inside(step + Warps)) {
+                next = row.read(symbol_of(step + Warps));
+                read_bias(k, row, symbol_of(step + Warps), next_bias);
+            }
             double z[8];
+            float rough[8], most = -CUDART_INF_F;
             if (inside(step)) {
-                adjust(e, v, window, z);
+                adjust(e, bias, v, window, z, rough);
             } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) z[i] = -CUDART_INF;
+                for (int i = 0; i < 8; ++i) z[i] = -CUDART_INF, rough[i] = -CUDART_INF_F;
             }
-            // Rounded to float for the comparisons that need no more.
-            float most = -CUDART_INF_F;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float rough = (float)z[i];
-                bad |= rough != rough;
-                most = fmaxf(most, rough);
+                bad |= rough[i] != rough[i];
+                most = fmaxf(most, rough[i]);
             }
             if (!(most < best_rough - fabsf(best_rough) * 0x1p-21f)) {  // float's order is double's but for neighbours
 #pragma unroll
@@ -528,7 +550,7 @@ __global__ void __launch_bounds__(32 * Warps) pick_kernel(const __grid_constant_
                 }
             } else {
                 // The block, then its step, in which the running sum passes u * total.
-                const double goal = a.uniforms[at] * total;
+                const double goal = uniform * total;
                 double sum = 0.0, sum_before = 0.0;
                 uint32_t owner = kAll, last = 0;
                 for (uint32_t j = 0; j < blocks; ++j) {
@@ -587,8 +609,10 @@ __global__ void __launch_bounds__(32 * Warps) pick_kernel(const __grid_constant_
     const double top = row_best, goal = target;
     const int32_t v = symbol_of(chosen);
     double z[8], w[8], sum = 0.0;
+    float rough[8], bias[8] = {};
     if (v < (int32_t)a.vocabulary) {
-        adjust(row.read(v), v, window, z);
+        read_bias(k, row, v, bias);
+        adjust(row.read(v), bias, v, window, z, rough);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) z[i] = -CUDART_INF;
@@ -619,6 +643,119 @@ __global__ void __launch_bounds__(32 * Warps) pick_kernel(const __grid_constant_
         a.symbols[at] = (int32_t)(hits ? hit : last);
         if (a.log_probability)
             a.log_probability[at] = (float)((logit == top ? 0.0 : (logit - top) / heat) - log(row_total));
+    }
+}
+
+// Rows of up to 128 N symbols, a block each and a symbol in N of a thread's
+// registers from the logits to the pick: with a row's few symbols what counts is
+// the length of the chain, and how much code a block runs through once.
+template <typename T, int N>
+__global__ void __launch_bounds__(128) narrow_pick_kernel(const __grid_constant__ LogitArgs a) {
+    __shared__ __align__(16) uint32_t counts[128 * N];
+    __shared__ double two_to[kPowers], sums[4 * N], warp_best[4];
+    __shared__ uint32_t warp_at[4], warp_bad[4], hit, last;
+    const uint32_t at = blockIdx.x, lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const T* row = static_cast<const T*>(a.logits) + (int64_t)at * a.logits_stride;
+    const RowRules k = row_rules(a.rules, at);
+    const float temperature = a.temperature ? a.temperature[at] : a.temperature_value;
+    const double uniform = a.uniforms ? a.uniforms[at] : 0.0;
+    float logit[N], bias[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const uint32_t v = 128 * j + threadIdx.x;
+        logit[j] = v < a.vocabulary ? load(row + v) : 0.0f;
+        bias[j] = k.bias && v < a.vocabulary ? __ldg(k.bias + v) : 0.0f;
+    }
+    if (threadIdx.x < kPowers) two_to[threadIdx.x] = kTwoTo[threadIdx.x];
+    if (threadIdx.x == 0) hit = kAll, last = 0;
+    if (k.length)
+        count_history(k, 0, 128 * N, counts);
+    else
+        __syncthreads();
+    const bool greedy = temperature == 0.0f;
+    const double heat = greedy ? 1.0 : (double)temperature, cold = kSixtyFourths / heat;
+    const double reciprocal = 1.0 / (double)k.repetition;
+    double z[N], best_value = -CUDART_INF;
+    uint32_t best = kAll, bad = !(temperature >= 0.0f);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const uint32_t v = 128 * j + threadIdx.x;
+        z[j] = adjusted((double)logit[j], k.length ? counts[v] : 0u, k, reciprocal, bias[j],
+                        v < a.vocabulary && k.mask.allows(v));
+        bad |= z[j] != z[j];
+        if (z[j] > best_value) best_value = z[j], best = v;
+    }
+    const auto join_best = [&](uint32_t width) {
+#pragma unroll 1
+        for (uint32_t off = width / 2; off > 0; off >>= 1) {
+            const double v = __shfl_xor_sync(kAll, best_value, off);
+            const uint32_t b = __shfl_xor_sync(kAll, best, off);
+            if (v > best_value || (v == best_value && b < best)) best_value = v, best = b;
+            bad |= __shfl_xor_sync(kAll, bad, off);
+        }
+    };
+    join_best(32);
+    if (lane == 0) warp_best[warp] = best_value, warp_at[warp] = best, warp_bad[warp] = bad;
+    __syncthreads();
+    best_value = warp_best[lane & 3u], best = warp_at[lane & 3u], bad = warp_bad[lane & 3u];
+    join_best(4);
+    if (bad || best == kAll) {
+        if (threadIdx.x == 0) {
+            a.symbols[at] = -1;
+            if (a.log_probability) a.log_probability[at] = bad ? CUDART_NAN_F : -CUDART_INF_F;
+        }
+        return;
+    }
+    // Running sums in the order of the symbols: of a warp's 32 here, of the warps' sums below.
+    double w[N], through[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) through[j] = w[j] = weight_of(z[j], best_value, cold, two_to);
+#pragma unroll 1
+    for (int off = 1; off < 32; off <<= 1) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const double o = __shfl_up_sync(kAll, through[j], off);
+            if (lane >= (uint32_t)off) through[j] += o;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+        if (lane == 31) sums[4 * j + warp] = through[j];
+    __syncthreads();
+    double total = 0.0, before[N];
+#pragma unroll
+    for (int j = 0; j < 4 * N; ++j) {
+        if ((j & 3) == (int)warp) before[j / 4] = total;
+        total += sums[j];
+    }
+    if (greedy) {
+        if (threadIdx.x == 0) {
+            a.symbols[at] = (int32_t)best;
+            if (a.log_probability) a.log_probability[at] = (float)-log(total);
+        }
+        return;
+    }
+    const double goal = uniform * total;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+        if (w[j] > 0.0) {
+            const uint32_t v = 128 * j + threadIdx.x;
+            if (before[j] + through[j] > goal)
+                atomicMin(&hit, v);
+            else
+                atomicMax(&last, v);
+        }
+    __syncthreads();
+    // A uniform of nearly 1 may pass no sum, which were rounded.
+    const uint32_t symbol = hit != kAll ? hit : last;
+    if (threadIdx.x == (symbol & 127u)) {
+        double chosen = 0.0;
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (symbol / 128 == j) chosen = z[j];
+        a.symbols[at] = (int32_t)symbol;
+        if (a.log_probability)
+            a.log_probability[at] = (float)((chosen == best_value ? 0.0 : (chosen - best_value) / heat) - log(total));
     }
 }
 
@@ -840,7 +977,8 @@ template <typename T, int Warps>
 void launch_pick(const LogitArgs& a, cudaStream_t stream) {
     const uint32_t all = (a.vocabulary + 7 + kStepSymbols - 1) / kStepSymbols;
     uint32_t blocks = 1;
-    while (blocks < 8 && blocks * 2 * Warps <= all && (uint64_t)a.rows * blocks < 512) blocks *= 2;
+    // two blocks an SM and no second wave of them: 64 rows of 131,072 take 70 us in 512 blocks, 61 us in 256
+    while (blocks < 8 && blocks * 2 * Warps <= all && (uint64_t)a.rows * blocks * 2 <= 296) blocks *= 2;
     if (all > 2048) blocks = 8;
     const uint32_t steps = (all + blocks - 1) / blocks;
     require(steps <= 4096, "the vocabulary is too large for one pick");
@@ -960,10 +1098,13 @@ int leo_b200_pick_symbols(int device, int dtype, const void* logits, int64_t log
             a.symbols = symbols;
             a.log_probability = log_probability;
             DeviceScope scope(device);
-            if (vocabulary + 7 <= 4 * kStepSymbols)
-                launch_pick<T, 4>(a, (cudaStream_t)stream);
+            if (vocabulary <= 384)
+                narrow_pick_kernel<T, 3><<<rows, 128, 0, (cudaStream_t)stream>>>(a);
+            else if (vocabulary <= 1024)
+                narrow_pick_kernel<T, 8><<<rows, 128, 0, (cudaStream_t)stream>>>(a);
             else
                 launch_pick<T, 8>(a, (cudaStream_t)stream);
+            check(cudaGetLastError(), "pick_kernel");
         });
     });
 }
