@@ -10,6 +10,17 @@ import torch
 from .ctypes_types import BF16, F16, F32
 
 DTYPE_CODES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+
+
+def device_of(name: str, tensor) -> int:
+    """The device index of a call's first tensor, which has to be a CUDA tensor."""
+    index = tensor.get_device() if isinstance(tensor, torch.Tensor) else -1
+    if index < 0 or not tensor.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if tensor.requires_grad:
+        _refuse_gradient(name)
+    return index
 
 
 def dtype_code(name: str, tensor) -> int:
@@ -19,28 +30,34 @@ def dtype_code(name: str, tensor) -> int:
     return code
 
 
-def check_tensor(name: str, tensor, device, dtype=None, shape=None) -> None:
-    """A tensor of the call: a CUDA tensor on ``device`` that asks for no gradient."""
+def _refuse_gradient(name: str) -> None:
+    if torch.is_grad_enabled():
+        raise ValueError(f"{name} asks for a gradient, which this call does not record: detach it and use the "
+                         "gradients that the operators return")
+
+
+def check_tensor(name: str, tensor, device: int, dtype=None, shape=None) -> None:
+    """A tensor of the call: on CUDA device ``device``, asking for no gradient."""
     if not isinstance(tensor, torch.Tensor) or not tensor.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
-    if tensor.device != device:
-        raise ValueError(f"{name} is on {tensor.device}, not on {device}")
+    if tensor.get_device() != device:
+        raise ValueError(f"{name} is on {tensor.device}, not on cuda:{device}")
     if dtype is not None and tensor.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, not {tensor.dtype}")
     if shape is not None and tensor.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(tensor.shape)}")
-    if tensor.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} asks for a gradient, which this call does not record: detach it and use the "
-                         "gradients that the operators return")
+    if tensor.requires_grad:
+        _refuse_gradient(name)
 
 
 def row_stride(name: str, tensor) -> int:
     """Elements between the rows of a 2-D tensor whose rows are adjacent elements."""
     if tensor.dim() != 2:
         raise ValueError(f"{name} must have two dimensions, not {tensor.dim()}")
-    if tensor.shape[1] > 1 and tensor.stride(1) != 1:
+    stride = tensor.stride()
+    if stride[1] != 1 and tensor.shape[1] > 1:
         raise ValueError(f"the elements of a row of {name} must be adjacent")
-    return tensor.stride(0)
+    return stride[0]
 
 
 def check_contiguous(name: str, tensor) -> None:
@@ -61,15 +78,30 @@ def _other_stream(stream, tensors):
             t.record_stream(stream)
 
 
-def on_stream(device, stream, tensors):
+class _CurrentStream:
+    """The raw current stream of a device, as a context that does nothing."""
+
+    __slots__ = ("raw",)
+
+    def __init__(self, raw: int):
+        self.raw = raw
+
+    def __enter__(self) -> int:
+        return self.raw
+
+    def __exit__(self, *exc) -> None:
+        return None
+
+
+def on_stream(device: int, stream, tensors):
     """The raw stream of a call: the current one of ``device``, or ``stream``.
 
     Outputs and scratch are to be allocated inside the context, so that they
     belong to the stream that writes them; with a ``stream`` other than the
     current one, ``tensors`` (the call's inputs) are marked as used on it."""
-    current = torch.cuda.current_stream(device)
-    if stream is None or stream == current:
-        return contextlib.nullcontext(current.cuda_stream)
-    if stream.device != device:
-        raise ValueError(f"the stream is on {stream.device}, not on {device}")
+    if stream is None:
+        raw = _raw_stream(device) if _raw_stream else torch.cuda.current_stream(device).cuda_stream
+        return _CurrentStream(raw)
+    if stream.device.index != device:
+        raise ValueError(f"the stream is on {stream.device}, not on cuda:{device}")
     return _other_stream(stream, tensors)

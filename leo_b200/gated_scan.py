@@ -29,7 +29,7 @@ import torch
 
 from . import native
 from .ctypes_types import LeoB200StoryTables
-from .device_tensors import check_contiguous, check_tensor, dtype_code, on_stream, pointer, row_stride
+from .device_tensors import check_contiguous, check_tensor, device_of, dtype_code, on_stream, pointer, row_stride
 
 
 class StoryLayout:
@@ -55,6 +55,7 @@ class StoryLayout:
         if device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
         self.device = device
+        self.index = device.index
         self.stories = stories
         self.tokens = int(offsets[-1])
         host = torch.empty(size, dtype=torch.uint8)
@@ -95,11 +96,11 @@ class GatedScanGradients(NamedTuple):
     initial: torch.Tensor | None
 
 
-def _check_decay(decay, drive) -> tuple[int, int, int]:
+def _check_decay(decay, drive, device: int) -> tuple[int, int, int]:
     """(type code, row stride, one row for all tokens or lanes)."""
-    check_tensor("decay", decay, drive.device)
+    check_tensor("decay", decay, device)
     code = dtype_code("decay", decay)
-    if decay.dtype != drive.dtype and decay.dtype != torch.float32:
+    if decay.dtype != torch.float32 and decay.dtype != drive.dtype:
         raise ValueError(f"decay must be of the drive's type or float32, not {decay.dtype}")
     if decay.dim() == 1:
         if decay.shape[0] != drive.shape[1] or (decay.shape[0] > 1 and decay.stride(0) != 1):
@@ -112,18 +113,18 @@ def _check_decay(decay, drive) -> tuple[int, int, int]:
 
 
 def _check_scan(drive, decay, layout, initial):
-    if not isinstance(drive, torch.Tensor) or not drive.is_cuda:
-        raise ValueError("drive must be a CUDA tensor")
-    check_tensor("drive", drive, drive.device)
-    stride = row_stride("drive", drive)
-    if layout.device != drive.device:
+    """(device, type code and row stride of the drive, the decay's)."""
+    device = device_of("drive", drive)
+    code, stride = dtype_code("drive", drive), row_stride("drive", drive)
+    if layout.index != device:
         raise ValueError(f"the layout is on {layout.device}, not on {drive.device}")
-    if drive.shape[0] != layout.tokens or drive.shape[1] == 0:
+    tokens, channels = drive.shape
+    if tokens != layout.tokens or channels == 0:
         raise ValueError(f"drive must have {layout.tokens} tokens of at least one channel, not {tuple(drive.shape)}")
     if initial is not None:
-        check_tensor("initial", initial, drive.device, torch.float32, (layout.stories, drive.shape[1]))
+        check_tensor("initial", initial, device, torch.float32, (layout.stories, channels))
         check_contiguous("initial", initial)
-    return dtype_code("drive", drive), stride, _check_decay(decay, drive)
+    return device, code, stride, _check_decay(decay, drive, device)
 
 
 def gated_scan(drive, decay, layout: StoryLayout, initial=None, keep_carries: bool = False,
@@ -135,21 +136,20 @@ def gated_scan(drive, decay, layout: StoryLayout, initial=None, keep_carries: bo
     distance, so a slice of a wider projection will do).  ``initial``: float32
     [stories, channels], zero if ``None``.  ``keep_carries``: keep what
     :func:`gated_scan_backward` needs."""
-    code, stride, (decay_code, decay_stride, shared) = _check_scan(drive, decay, layout, initial)
+    device, code, stride, (decay_code, decay_stride, shared) = _check_scan(drive, decay, layout, initial)
     tokens, channels = drive.shape
     L = native.lib()
     size, kept = layout._needs(channels)
-    with on_stream(drive.device, stream, (drive, decay, initial)) as raw:
-        states = torch.empty((tokens, channels), dtype=drive.dtype, device=drive.device)
-        final = torch.empty((layout.stories, channels), dtype=torch.float32, device=drive.device)
-        carries = None
-        if keep_carries:
-            carries = torch.empty(kept, dtype=torch.float32, device=drive.device)
-        scratch = torch.empty(size, dtype=torch.uint8, device=drive.device) if size else None
+    where = layout.device
+    with on_stream(device, stream, (drive, decay, initial)) as raw:
+        states = torch.empty((tokens, channels), dtype=drive.dtype, device=where)
+        final = torch.empty((layout.stories, channels), dtype=torch.float32, device=where)
+        carries = torch.empty(kept, dtype=torch.float32, device=where) if keep_carries else None
+        scratch = torch.empty(size, dtype=torch.uint8, device=where) if size else None
         native.check(L.leo_b200_gated_scan(
-            drive.device.index, layout._ref, channels, code, drive.data_ptr(), stride, decay_code, decay.data_ptr(),
-            decay_stride, shared, pointer(initial), states.data_ptr(), final.data_ptr(), pointer(carries),
-            pointer(scratch), size, raw))
+            device, layout._ref, channels, code, drive.data_ptr(), stride, decay_code, decay.data_ptr(), decay_stride,
+            shared, pointer(initial), states.data_ptr(), final.data_ptr(), pointer(carries), pointer(scratch), size,
+            raw))
     return GatedScan(states, final, carries)
 
 
@@ -160,9 +160,8 @@ def gated_scan_backward(grad_states, drive, decay, layout: StoryLayout, carries,
     ``grad_states``: of the drive's shape and type; ``grad_final``: float32
     [stories, channels], zero if ``None``.  The gradient of a [channels] decay
     is summed over all tokens in a fixed order."""
-    code, stride, (decay_code, decay_stride, shared) = _check_scan(drive, decay, layout, initial)
+    device, code, stride, (decay_code, decay_stride, shared) = _check_scan(drive, decay, layout, initial)
     tokens, channels = drive.shape
-    device = drive.device
     check_tensor("grad_states", grad_states, device, drive.dtype, drive.shape)
     grad_stride = row_stride("grad_states", grad_states)
     if grad_final is not None:
@@ -174,15 +173,16 @@ def gated_scan_backward(grad_states, drive, decay, layout: StoryLayout, carries,
     size, kept = layout._needs(channels)
     check_tensor("carries", carries, device, torch.float32, (kept,))
     check_contiguous("carries", carries)
+    where = layout.device
     with on_stream(device, stream, (grad_states, drive, decay, carries, initial, grad_final)) as raw:
-        grad_drive = torch.empty((tokens, channels), dtype=drive.dtype, device=device)
-        grad_decay = torch.empty(decay.shape, dtype=decay.dtype, device=device)
+        grad_drive = torch.empty((tokens, channels), dtype=drive.dtype, device=where)
+        grad_decay = torch.empty(decay.shape, dtype=decay.dtype, device=where)
         grad_initial = None
         if initial is not None:
-            grad_initial = torch.empty((layout.stories, channels), dtype=torch.float32, device=device)
-        scratch = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+            grad_initial = torch.empty((layout.stories, channels), dtype=torch.float32, device=where)
+        scratch = torch.empty(size, dtype=torch.uint8, device=where) if size else None
         native.check(L.leo_b200_gated_scan_backward(
-            device.index, layout._ref, channels, code, grad_states.data_ptr(), grad_stride, drive.data_ptr(), stride,
+            device, layout._ref, channels, code, grad_states.data_ptr(), grad_stride, drive.data_ptr(), stride,
             decay_code, decay.data_ptr(), decay_stride, shared, pointer(initial), pointer(grad_final),
             carries.data_ptr(), grad_drive.data_ptr(), grad_decay.data_ptr(), pointer(grad_initial),
             pointer(scratch), size, raw))
@@ -201,23 +201,19 @@ def gated_step(drive, decay, state, stream=None):
     """One token for each lane: ``state`` (float32 [lanes, channels]) becomes
     ``decay * state + drive`` in place; returns it in the drive's type.
     ``drive``: [lanes, channels]; ``decay``: the same shape, or [channels]."""
-    if not isinstance(drive, torch.Tensor) or not drive.is_cuda:
-        raise ValueError("drive must be a CUDA tensor")
-    device = drive.device
-    check_tensor("drive", drive, device)
-    stride = row_stride("drive", drive)
-    code = dtype_code("drive", drive)
+    device = device_of("drive", drive)
+    code, stride = dtype_code("drive", drive), row_stride("drive", drive)
     lanes, channels = drive.shape
     if channels == 0:
         raise ValueError("drive must have at least one channel")
-    decay_code, decay_stride, shared = _check_decay(decay, drive)
+    decay_code, decay_stride, shared = _check_decay(decay, drive, device)
     check_tensor("state", state, device, torch.float32, drive.shape)
     state_stride = row_stride("state", state)
-    if lanes > 1 and state_stride < channels:
+    if state_stride < channels and lanes > 1:
         raise ValueError("the rows of state overlap")
     with on_stream(device, stream, (drive, decay, state)) as raw:
-        output = torch.empty((lanes, channels), dtype=drive.dtype, device=device)
+        output = torch.empty((lanes, channels), dtype=drive.dtype, device=drive.device)
         native.check(native.lib().leo_b200_gated_step(
-            device.index, lanes, channels, code, drive.data_ptr(), stride, decay_code, decay.data_ptr(), decay_stride,
-            shared, state.data_ptr(), state_stride, output.data_ptr(), raw))
+            device, lanes, channels, code, drive.data_ptr(), stride, decay_code, decay.data_ptr(), decay_stride, shared,
+            state.data_ptr(), state_stride, output.data_ptr(), raw))
     return output

@@ -25,7 +25,7 @@ import torch
 
 from . import native
 from .ctypes_types import LeoB200LogitRules
-from .device_tensors import check_contiguous, check_tensor, dtype_code, on_stream, pointer, row_stride
+from .device_tensors import check_contiguous, check_tensor, device_of, dtype_code, on_stream, pointer, row_stride
 
 
 def pack_allowed(allowed) -> torch.Tensor:
@@ -42,23 +42,22 @@ def pack_allowed(allowed) -> torch.Tensor:
 
 
 def _check_logits(logits):
-    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
-        raise ValueError("logits must be a CUDA tensor")
-    check_tensor("logits", logits, logits.device)
+    """(device, type code, row stride)."""
+    device = device_of("logits", logits)
     stride = row_stride("logits", logits)
     if logits.shape[1] == 0:
         raise ValueError("logits must have at least one symbol")
-    return dtype_code("logits", logits), stride
+    return device, dtype_code("logits", logits), stride
 
 
-def _check_mask(logits, allowed, state):
+def _check_mask(logits, device, allowed, state):
     """(row stride, states) of the mask table."""
     rows, vocabulary = logits.shape
     if allowed is None:
         if state is not None:
             raise ValueError("state needs a mask table in allowed")
         return 0, 0
-    check_tensor("allowed", allowed, logits.device, torch.int32)
+    check_tensor("allowed", allowed, device, torch.int32)
     stride = row_stride("allowed", allowed)
     states, words = allowed.shape
     if words < (vocabulary + 31) // 32:
@@ -66,17 +65,17 @@ def _check_mask(logits, allowed, state):
     if states == 0:
         raise ValueError("allowed must have at least one state")
     if state is not None:
-        check_tensor("state", state, logits.device, torch.int32, (rows,))
+        check_tensor("state", state, device, torch.int32, (rows,))
         check_contiguous("state", state)
     elif states not in (1, rows):
         raise ValueError(f"without state, allowed must have 1 or {rows} rows, not {states}")
     return stride, states
 
 
-def _scalar_or_rows(name: str, value, logits):
+def _scalar_or_rows(name: str, value, logits, device):
     """(tensor or None, number)."""
     if isinstance(value, torch.Tensor):
-        check_tensor(name, value, logits.device, torch.float32, (logits.shape[0],))
+        check_tensor(name, value, device, torch.float32, (logits.shape[0],))
         check_contiguous(name, value)
         return value, 0.0
     return None, float(value)
@@ -85,9 +84,8 @@ def _scalar_or_rows(name: str, value, logits):
 class _Rules:
     """The checked rules of a call, and the tensors that they point at."""
 
-    def __init__(self, logits, history, lengths, repetition, presence, frequency, bias, allowed, state):
+    def __init__(self, logits, device, history, lengths, repetition, presence, frequency, bias, allowed, state):
         rows, vocabulary = logits.shape
-        device = logits.device
         history_stride = capacity = bias_stride = 0
         if history is not None:
             check_tensor("history", history, device, torch.int32)
@@ -100,9 +98,9 @@ class _Rules:
                 check_contiguous("lengths", lengths)
         elif lengths is not None:
             raise ValueError("lengths needs a history")
-        repetition_rows, repetition = _scalar_or_rows("repetition", repetition, logits)
-        presence_rows, presence = _scalar_or_rows("presence", presence, logits)
-        frequency_rows, frequency = _scalar_or_rows("frequency", frequency, logits)
+        repetition_rows, repetition = _scalar_or_rows("repetition", repetition, logits, device)
+        presence_rows, presence = _scalar_or_rows("presence", presence, logits, device)
+        frequency_rows, frequency = _scalar_or_rows("frequency", frequency, logits, device)
         if repetition_rows is not None:
             repetition = 1.0
         if bias is not None:
@@ -115,7 +113,7 @@ class _Rules:
                     raise ValueError(f"bias must have shape {tuple(logits.shape)} or ({vocabulary},), "
                                      f"not {tuple(bias.shape)}")
                 bias_stride = row_stride("bias", bias)
-        allowed_stride, states = _check_mask(logits, allowed, state)
+        allowed_stride, states = _check_mask(logits, device, allowed, state)
         self.tensors = (logits, history, lengths, repetition_rows, presence_rows, frequency_rows, bias, allowed, state)
         self.c = LeoB200LogitRules(
             pointer(history), history_stride, capacity, pointer(lengths), pointer(repetition_rows),
@@ -134,18 +132,18 @@ def adjust_logits(logits, *, history=None, lengths=None, repetition=1.0, presenc
     taken off.  ``bias`` (float32 ``[vocabulary]`` or ``[rows, vocabulary]``)
     is added, and what the mask forbids becomes -inf.  ``out`` may be
     ``logits`` itself; another one must not overlap it."""
-    code, stride = _check_logits(logits)
-    rules = _Rules(logits, history, lengths, repetition, presence, frequency, bias, allowed, state)
+    device, code, stride = _check_logits(logits)
+    rules = _Rules(logits, device, history, lengths, repetition, presence, frequency, bias, allowed, state)
     rows, vocabulary = logits.shape
     if out is not None:
-        check_tensor("out", out, logits.device, logits.dtype, logits.shape)
+        check_tensor("out", out, device, logits.dtype, logits.shape)
         if row_stride("out", out) < vocabulary and rows > 1:
             raise ValueError("the rows of out overlap")
-    with on_stream(logits.device, stream, rules.tensors + (out,)) as raw:
+    with on_stream(device, stream, rules.tensors + (out,)) as raw:
         if out is None:
             out = torch.empty((rows, vocabulary), dtype=logits.dtype, device=logits.device)
         native.check(native.lib().leo_b200_adjust_logits(
-            logits.device.index, code, logits.data_ptr(), stride, rows, vocabulary, C.byref(rules.c), out.data_ptr(),
+            device, code, logits.data_ptr(), stride, rows, vocabulary, C.byref(rules.c), out.data_ptr(),
             out.stride(0), raw))
     return out
 
@@ -163,18 +161,18 @@ def pick_symbols(logits, *, temperature=0.0, uniforms=None, history=None, length
     and -inf; one with a NaN that is not masked (or a temperature that is
     negative or NaN) -1 and NaN.  Everything is computed in 64 bits from the
     inputs as they are."""
-    code, stride = _check_logits(logits)
-    rules = _Rules(logits, history, lengths, repetition, presence, frequency, bias, allowed, state)
+    device, code, stride = _check_logits(logits)
+    rules = _Rules(logits, device, history, lengths, repetition, presence, frequency, bias, allowed, state)
     rows, vocabulary = logits.shape
-    temperature_rows, temperature = _scalar_or_rows("temperature", temperature, logits)
+    temperature_rows, temperature = _scalar_or_rows("temperature", temperature, logits, device)
     if uniforms is not None:
-        check_tensor("uniforms", uniforms, logits.device, torch.float64, (rows,))
+        check_tensor("uniforms", uniforms, device, torch.float64, (rows,))
         check_contiguous("uniforms", uniforms)
-    with on_stream(logits.device, stream, rules.tensors + (temperature_rows, uniforms)) as raw:
+    with on_stream(device, stream, rules.tensors + (temperature_rows, uniforms)) as raw:
         symbols = torch.empty(rows, dtype=torch.int32, device=logits.device)
         log_probability = torch.empty(rows, dtype=torch.float32, device=logits.device)
         native.check(native.lib().leo_b200_pick_symbols(
-            logits.device.index, code, logits.data_ptr(), stride, rows, vocabulary, C.byref(rules.c),
+            device, code, logits.data_ptr(), stride, rows, vocabulary, C.byref(rules.c),
             pointer(temperature_rows), temperature, pointer(uniforms), symbols.data_ptr(),
             log_probability.data_ptr(), raw))
     return symbols, log_probability
@@ -192,19 +190,19 @@ def masked_cross_entropy(logits, targets, *, allowed=None, state=None, weights=N
     0), one of ``vocabulary`` or more gives loss NaN and gradient 0.  A
     masked target, or a row with nothing left, has loss +inf; the gradient
     stays finite."""
-    code, stride = _check_logits(logits)
+    device, code, stride = _check_logits(logits)
     rows, vocabulary = logits.shape
-    check_tensor("targets", targets, logits.device, torch.int32, (rows,))
+    check_tensor("targets", targets, device, torch.int32, (rows,))
     check_contiguous("targets", targets)
-    allowed_stride, states = _check_mask(logits, allowed, state)
+    allowed_stride, states = _check_mask(logits, device, allowed, state)
     if weights is not None:
-        check_tensor("weights", weights, logits.device, torch.float32, (rows,))
+        check_tensor("weights", weights, device, torch.float32, (rows,))
         check_contiguous("weights", weights)
-    with on_stream(logits.device, stream, (logits, targets, allowed, state, weights)) as raw:
+    with on_stream(device, stream, (logits, targets, allowed, state, weights)) as raw:
         losses = torch.empty(rows, dtype=torch.float32, device=logits.device)
         gradient = torch.empty((rows, vocabulary), dtype=logits.dtype, device=logits.device)
         native.check(native.lib().leo_b200_masked_cross_entropy(
-            logits.device.index, code, logits.data_ptr(), stride, rows, vocabulary, targets.data_ptr(),
+            device, code, logits.data_ptr(), stride, rows, vocabulary, targets.data_ptr(),
             pointer(allowed), allowed_stride, states, pointer(state), pointer(weights), losses.data_ptr(),
             gradient.data_ptr(), vocabulary, raw))
     return losses, gradient
