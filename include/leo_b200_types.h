@@ -385,6 +385,7 @@ typedef struct LeoB200StoryTables {
     const uint32_t* order;                  /* the stories with a token in order, then those without */
     const LeoB200StoryTile* schedule[2][2]; /* tiles of 128, of 64 tokens; forward, backward */
     uint32_t tiles[2];                      /* how many of 128, of 64 tokens or fewer */
+    uint32_t longest[2];                    /* how many of them depend on one another in a row, at most */
     uint32_t tokens;
     uint32_t stories;
     uint32_t full;                          /* stories with a token */

@@ -304,6 +304,7 @@ class LeoB200StoryTables(C.Structure):
         ("order", C.c_void_p),
         ("schedule", (C.c_void_p * 2) * 2),
         ("tiles", C.c_uint32 * 2),
+        ("longest", C.c_uint32 * 2),
         ("tokens", C.c_uint32),
         ("stories", C.c_uint32),
         ("full", C.c_uint32),

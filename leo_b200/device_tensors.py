@@ -38,6 +38,9 @@ def _refuse_gradient(name: str) -> None:
 
 def check_tensor(name: str, tensor, device: int, dtype=None, shape=None) -> None:
     """A tensor of the call: on CUDA device ``device``, asking for no gradient."""
+    if (isinstance(tensor, torch.Tensor) and tensor.get_device() == device and (dtype is None or tensor.dtype == dtype)
+            and (shape is None or tensor.shape == shape) and not tensor.requires_grad):
+        return
     if not isinstance(tensor, torch.Tensor) or not tensor.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
     if tensor.get_device() != device:
@@ -46,8 +49,7 @@ def check_tensor(name: str, tensor, device: int, dtype=None, shape=None) -> None
         raise ValueError(f"{name} must be {dtype}, not {tensor.dtype}")
     if shape is not None and tensor.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(tensor.shape)}")
-    if tensor.requires_grad:
-        _refuse_gradient(name)
+    _refuse_gradient(name)
 
 
 def row_stride(name: str, tensor) -> int:

@@ -127,7 +127,8 @@ def test_story_table(native_lib, lengths):
         assert starts == sum(1 << (b - 32 * w) for b in begins if b // 32 == w)
         assert rank == sum(1 for b in begins if b < 32 * w)
     for k, longest in enumerate((128, 64)):
-        for d in range(2):
+        tiles = []
+        for d in reversed(range(2)):
             listed = [LeoB200StoryTile.from_buffer_copy(raw, (t.schedule[k][d] or 0) + 32 * i)
                       for i in range(t.tiles[k])]
             turn = {x.tile: i for i, x in enumerate(listed)}
@@ -147,6 +148,10 @@ def test_story_table(native_lib, lengths):
                 assert x.onward == int(not x.first <= far <= last)
                 step = 1 if holder <= x.tile else -1
                 assert all(turn[y] < turn[x.tile] for y in range(holder, x.tile, step))
+        rank = [0] * t.tiles[k]
+        for x in tiles if tokens else []:
+            rank[x.tile] = rank[x.tile - 1] + 1 if x.tile and x.first not in begins else 0
+        assert t.longest[k] == max(rank) + 1
     halves = {x.tile: x for x in (LeoB200StoryTile.from_buffer_copy(raw, (t.schedule[1][0] or 0) + 32 * i)
                                   for i in range(t.tiles[1]))}
     for i in range(t.tiles[0]):
@@ -211,7 +216,7 @@ def test_entry_point_refuses_before_device_work(native_lib, bad):
     from leo_b200.ctypes_types import LeoB200StoryTables
 
     p = 256
-    t = LeoB200StoryTables(p, p, ((p, p), (p, p)), (8, 16), 1000, 3, 3)
+    t = LeoB200StoryTables(p, p, ((p, p), (p, p)), (8, 16), (3, 6), 1000, 3, 3)
     args = dict(channels=70, dtype=1, decay_dtype=0, drive=p, final=p)  # and no workspace
     if bad == "stories":
         t.stories = 0
