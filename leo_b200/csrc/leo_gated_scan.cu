@@ -52,13 +52,11 @@ using namespace leo_operator;
 
 constexpr uint32_t kThreads = 128;  // of the reduction
 
-constexpr int kWarps = 8;                        // that map and write a tile
+constexpr int kWarps = 8;                        // of a team, which maps and writes a tile
 constexpr int kSegments = 2 * kWarps;            // of a tile, half a warp each
 constexpr int kColumns = 64;                     // channels of a tile, four a thread
 constexpr int kComposeWarps = kColumns / 16;     // that compose it, two lanes a channel
 constexpr int kScoutWarps = kColumns / 16;       // that find the state before it, two lanes a channel
-constexpr uint32_t kTileThreads = 32 * (kWarps + kComposeWarps + kScoutWarps);
-constexpr int kStages = 3;
 constexpr uint32_t kNone = 0xffffffffu;
 constexpr size_t kSharedLimit = 227 * 1024;
 constexpr uint32_t kKept = LEO_B200_TILE_TOKENS / 2;  // tokens between the states kept for the backward pass
@@ -265,14 +263,25 @@ struct Shape {
         float sums[Backward && Shared ? 2 : 1][Backward && Shared ? kSegments : 1][kColumns];
         Work ring[8];  // the block's work; an entry is rewritten when no warp reads it any more
         float scouted[2][Backward ? 2 : 1][kColumns];  // the value before the tile; the kept state before it
-        uint64_t landed[kStages][kWarps];  // barriers of the tiled loads
+        uint64_t landed[4][kWarps];  // barriers of the tiled loads
     };
-    // 8 tokens a thread, or 4 where three stages of them would not fit.
-    static constexpr size_t kStageOf8 = (size_t)8 * kSegments * kRow;
-    static constexpr int kSegment = kStages * kStageOf8 + sizeof(Control) <= kSharedLimit ? 8 : 4;
+    static constexpr bool fits(int segment, int stages) {
+        return (size_t)stages * segment * kSegments * kRow + sizeof(Control) <= kSharedLimit;
+    }
+    // Two teams with two stages each where they fit shared memory, one with three
+    // where not; 8 tokens a thread, or 4 where not even those would.
+    static constexpr int kTeams = fits(8, 4) || !fits(8, 3) ? 2 : 1;
+    static constexpr int kStages = kTeams == 2 ? 4 : 3;
+    static constexpr int kSegment = fits(8, kStages) ? 8 : 4;
     static constexpr uint32_t kTile = kSegment * kSegments;
     static constexpr size_t kStage = (size_t)kTile * kRow;
     static constexpr size_t kBytes = kStages * kStage + sizeof(Control);
+    // Tickets are drawn so far ahead that a team finds the one whose loads it issues:
+    // its own last turn is the newest that it knows to be over.
+    static constexpr int kAhead = 2 + kTeams;
+    static constexpr int kFirstComposer = kWarps * kTeams;
+    static constexpr int kFirstScout = kFirstComposer + kComposeWarps;
+    static constexpr uint32_t kThreads = 32 * (kFirstScout + kScoutWarps);
 };
 
 // Named barriers of a block, one of each kind for even and one for odd tiles.
@@ -498,14 +507,15 @@ __device__ __forceinline__ void copy_empty(const LeoB200StoryTables& t, uint32_t
 }
 
 template <typename T, typename G, int Unit, bool Shared, bool Backward>
-__global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_constant__ ScanArgs a) {
+__global__ void __launch_bounds__(Shape<T, G, Shared, Backward>::kThreads, 1) scan_kernel(const __grid_constant__ ScanArgs a) {
     using S = Shape<T, G, Shared, Backward>;
     constexpr int Length = S::kSegment;
     constexpr uint32_t kTile = S::kTile;
     constexpr bool Tiled = Unit == 4;
+    constexpr int kStages = S::kStages, kTeams = S::kTeams;
     extern __shared__ __align__(128) unsigned char dynamic[];
     typename S::Control& control = *reinterpret_cast<typename S::Control*>(dynamic + kStages * S::kStage);
-    const uint32_t warp = threadIdx.x >> 5;
+    const uint32_t block_warp = threadIdx.x >> 5;
     const uint32_t total = a.tiles * a.groups;
     const auto work_of = [&](uint32_t ticket) {
         Work w{0, kNone, 0, 0, 0, 0, 0, 0};
@@ -515,7 +525,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
         const uint4 x = __ldg(entry), y = __ldg(entry + 1);  // first, count, tile, kept; holder, onward
         return Work{x.x, x.y, x.z, ticket - place * a.groups, y.x, x.w, y.y, 0};
     };
-    // The first tickets: one if there is a block for each, or three, drawn one
+    // The first tickets: one if there is a block for each, or a few, drawn one
     // after the other so that the blocks take turns: a block that held the next
     // three in a row would keep its neighbours waiting for its third.
     const bool one_each = gridDim.x == total;
@@ -523,12 +533,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
         uint32_t t = a.tiles == 1 ? blockIdx.x : atomicAdd(a.scratch.ticket, 1u) + 1u;
         control.ring[0] = work_of(t);
 #pragma unroll
-        for (int j = 1; j < 3; ++j) {
+        for (int j = 1; j < S::kAhead; ++j) {
             if (!one_each) t = atomicAdd(a.scratch.ticket + (t == kNone), 1u) + 1u;  // after the one before
             control.ring[j] = work_of(one_each ? total : t);
         }
         if constexpr (Tiled) {
-            for (int j = 0; j < kStages * kWarps; ++j)
+            for (int j = 0; j < 4 * kWarps; ++j)
                 asm volatile("mbarrier.init.shared.b64 [%0], 1;" ::"r"(
                     (uint32_t)__cvta_generic_to_shared(&control.landed[0][0] + j))
                              : "memory");
@@ -538,8 +548,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
     __syncthreads();
     const auto work_at = [&](uint32_t i) -> const Work& { return control.ring[i & 7u]; };
 
-    if (warp < kWarps) {
-        // ------------------------------------------------ the threads that map and write
+    if (block_warp < S::kFirstComposer) {
+        // ------------------------------------------------ the teams that map and write, tiles in turn
+        const uint32_t team = block_warp / kWarps, warp = block_warp % kWarps;
         const uint32_t lane = threadIdx.x & 31u, segment = warp * 2 + (lane >> 4);
         const auto stage = [&](uint32_t i) { return dynamic + (i % kStages) * S::kStage; };
         const auto stage_x = [&](uint32_t i, uint32_t seg) {
@@ -575,7 +586,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
         const auto issue = [&](uint32_t i) -> StoryBits {
             StoryBits bits{};
             const Work& work = work_at(i);
-            if (Pends && i > 0) settle(i - 1);
+            if (Pends && i >= kTeams) settle(i - kTeams);
             if (work.count != kNone) {
                 const uint32_t first = work.first + segment * Length, group = work.group;
                 const int count = tokens_of(work);
@@ -768,18 +779,31 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
             }
         };
 
-        StoryBits bits0 = issue(0), bits1 = issue(1);
-        if (work_at(0).count != kNone) map(0, bits0);
-        for (uint32_t i = 0; work_at(i).count != kNone; ++i) {
-            const StoryBits bits2 = issue(i + 2);
-            if (work_at(i + 1).count != kNone) map(i + 1, bits1);
-            sync_of<kComposed>(i & 1u);
-            write(i, bits0);
-            bits0 = bits1;
-            bits1 = bits2;
+        if constexpr (kTeams == 1) {
+            // What is done between the maps of a tile and its writing is the map of the next one.
+            StoryBits bits0 = issue(0), bits1 = issue(1);
+            if (work_at(0).count != kNone) map(0, bits0);
+            for (uint32_t i = 0; work_at(i).count != kNone; ++i) {
+                const StoryBits bits2 = issue(i + 2);
+                if (work_at(i + 1).count != kNone) map(i + 1, bits1);
+                sync_of<kComposed>(i & 1u);
+                write(i, bits0);
+                bits0 = bits1;
+                bits1 = bits2;
+            }
+        } else {
+            // The other team's work fills the time between.
+            StoryBits bits = issue(team);
+            for (uint32_t i = team; work_at(i).count != kNone; i += 2) {
+                const StoryBits bits_next = issue(i + 2);
+                map(i, bits);
+                sync_of<kComposed>(i & 1u);
+                write(i, bits);
+                bits = bits_next;
+            }
         }
-        if constexpr (Backward && Shared) arrive_at<kMapped>(0);  // the last sums are written
-    } else if (warp >= kWarps + kComposeWarps) {
+        if constexpr (Backward && Shared) arrive_at<kMapped>(team);  // the last sums are written
+    } else if (block_warp >= S::kFirstScout) {
         // ------------------------------------------------ the warps that scout
         // Everything that is read from memory between tiles is read here, up to two
         // tiles ahead: beside a load in flight the warps that compose would wait for
@@ -787,8 +811,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
         // channel; its partner is 16 lanes away.
         constexpr int Direction = Backward ? -1 : 1;
         const uint32_t lane = threadIdx.x & 31u, half = lane >> 4;
-        const uint32_t k = (warp - kWarps - kComposeWarps) * 16 + (lane & 15u);
-        const bool leader = threadIdx.x == 32 * (kWarps + kComposeWarps);
+        const uint32_t k = (block_warp - S::kFirstScout) * 16 + (lane & 15u);
+        const bool leader = threadIdx.x == 32 * S::kFirstScout;
         for (uint32_t i = 0;; ++i) {
             const Work work = work_at(i);
             if (work.count == kNone) break;
@@ -829,7 +853,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
                 control.scouted[i & 1u][0][k] = carry;
                 if constexpr (Backward) control.scouted[i & 1u][1][k] = kept;
             }
-            if (leader) control.ring[(i + 3) & 7u] = later;
+            if (leader) control.ring[(i + S::kAhead) & 7u] = later;
             arrive_at<kScouted>(i & 1u);
         }
     } else {
@@ -837,7 +861,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
         // A lane takes half the segments of a channel, the nearer ones in the
         // direction of the scan first; its partner is 16 lanes away.
         constexpr int kHalf = kSegments / 2;
-        const uint32_t lane = threadIdx.x & 31u, half = lane >> 4, k = (warp - kWarps) * 16 + (lane & 15u);
+        const uint32_t lane = threadIdx.x & 31u, half = lane >> 4, k = (block_warp - S::kFirstComposer) * 16 + (lane & 15u);
         // A shared gate's product over a segment's tokens.
         const auto power = [&](uint32_t channel, int count) {
             float2 product = make_float2(1.0f, 0.0f);
@@ -893,14 +917,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
                 }
             };
             float2 product = make_float2(1.0f, 0.0f);
-            float sum = 0.0f;
+            float sum = 0.0f, A[kHalf], v[kHalf];
 #pragma unroll
             for (int j = 0; j < kHalf; ++j) {
                 const int w = segment(j);
-                const float2 A = product_at(w);
-                const float v = Backward ? m.M[Backward ? w : 0][k] : m.H[w][k];
-                sum = cut_at(j) ? v : fmaf(value_of(A), sum, v);
-                product = product_of(product, A);
+                const float2 p = product_at(w);
+                A[j] = value_of(p);
+                v[j] = Backward ? m.M[Backward ? w : 0][k] : m.H[w][k];
+                sum = cut_at(j) ? v[j] : fmaf(A[j], sum, v[j]);
+                product = product_of(product, p);
             }
             const bool cut = (cut_bytes.x | cut_bytes.y) != 0;
             const bool other_cut = __shfl_xor_sync(kNone, cut, 16);
@@ -926,13 +951,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
 
             // The value before each segment, in place of its map.
             float before = half ? (near_cut ? near_sum : fmaf(near_A, carry, near_sum)) : carry;
-            float A[kHalf], v[kHalf];
-#pragma unroll
-            for (int j = 0; j < kHalf; ++j) {
-                const int w = segment(j);
-                A[j] = value_of(product_at(w));
-                v[j] = Backward ? m.M[Backward ? w : 0][k] : m.H[w][k];
-            }
 #pragma unroll
             for (int j = 0; j < kHalf; ++j) {
                 const int w = segment(j);
@@ -982,6 +1000,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) scan_kernel(const __grid_cons
         }
         if constexpr (Backward && Shared) {
             sync_of<kMapped>(0);
+            if constexpr (kTeams == 2) sync_of<kMapped>(1);
             if (before2.x != kNone) add_sums(i, before2);
             if (before1.x != kNone) add_sums(i + 1, before1);
         }
@@ -1382,7 +1401,7 @@ void launch_scan(ScanArgs& a, void* workspace, size_t workspace_bytes, cudaStrea
         check(cudaMemsetAsync(workspace, 0xff, 256 + (size_t)a.tiles * a.channels * sizeof(Slot), stream), "clear scan slots");
     }
     const uint32_t blocks = a.tiles == 1 || total <= 2u * (uint32_t)sms ? (uint32_t)total : (uint32_t)sms;
-    kernel<<<blocks, kTileThreads, S::kBytes, stream>>>(a);
+    kernel<<<blocks, S::kThreads, S::kBytes, stream>>>(a);
     check(cudaGetLastError(), "scan_kernel");
 }
 
