@@ -50,7 +50,7 @@ namespace {
 
 using namespace leo_operator;
 
-constexpr uint32_t kThreads = 128;  // of the reduction
+constexpr uint32_t kReduceThreads = 1024;
 
 constexpr int kWarps = 8;                        // of a team, which maps and writes a tile
 constexpr int kSegments = 2 * kWarps;            // of a tile, half a warp each
@@ -61,7 +61,10 @@ constexpr uint32_t kNone = 0xffffffffu;
 constexpr size_t kSharedLimit = 227 * 1024;
 constexpr uint32_t kKept = LEO_B200_TILE_TOKENS / 2;  // tokens between the states kept for the backward pass
 constexpr int kGroup = 16;                       // tiles between published states
-constexpr uint32_t kAbreast = 12;                // fewer independent tiles than these are mapped in a pass of their own
+// Fewer independent tiles than these are mapped in a pass of their own.  One story
+// of 65,536 tokens: 512 channels (8 abreast) forward 108 us so and 127 us in one
+// pass, backward 137 and 143 us; 1,024 channels (16) 184 and 207 us, 248 and 229 us.
+constexpr uint32_t kAbreast[2] = {20, 12};  // forward, backward
 constexpr uint32_t kSpinLimit = 1u << 21;        // polls of a wait, a memory round trip and more apart
 
 __device__ uint32_t g_gave_up;
@@ -813,9 +816,21 @@ __global__ void __launch_bounds__(Shape<T, G, Shared, Backward>::kThreads, 1) sc
         const uint32_t lane = threadIdx.x & 31u, half = lane >> 4;
         const uint32_t k = (block_warp - S::kFirstScout) * 16 + (lane & 15u);
         const bool leader = threadIdx.x == 32 * S::kFirstScout;
+        const auto draw = [&] {
+            uint32_t t = kNone - 1u;
+            if (leader && !one_each)  // no use of the answer here, so that nothing waits for it
+                asm volatile("atom.relaxed.gpu.global.add.u32 %0, [%1], 1;" : "=r"(t) : "l"(a.scratch.ticket) : "memory");
+            return t;
+        };
+        uint32_t drawn = draw();
         for (uint32_t i = 0;; ++i) {
             const Work work = work_at(i);
             if (work.count == kNone) break;
+            // The schedule's entry of the ticket drawn a turn ago, and another ticket.
+            const uint32_t ticket = drawn + 1u, place = min(ticket / a.groups, a.tiles - 1u);
+            const uint4* entry = reinterpret_cast<const uint4*>(a.schedule + place);
+            const uint4 x = __ldg(entry), y = __ldg(entry + 1);  // first, count, tile, kept; holder, onward
+            drawn = draw();
             const uint32_t c = work.group * kColumns + k;
             const bool active = c < a.channels;
             const Lookback<Direction> back(work.tile, work.holder, a.ready);
@@ -824,8 +839,6 @@ __global__ void __launch_bounds__(Shape<T, G, Shared, Backward>::kThreads, 1) sc
             float kept = 0.0f;
             if (Backward && active && half == 0 && work.count > 0)
                 kept = __ldcs(a.carries + (size_t)work.kept * a.channels + c);
-            Work later{0, kNone, 0, 0, 0, 0, 0, 0};
-            if (leader && !one_each) later = work_of(atomicAdd(a.scratch.ticket, 1u) + 1u);
             float carry = 0.0f;
             if (back.maps >= 0) {
                 float A = 1.0f, H = 0.0f;
@@ -853,7 +866,9 @@ __global__ void __launch_bounds__(Shape<T, G, Shared, Backward>::kThreads, 1) sc
                 control.scouted[i & 1u][0][k] = carry;
                 if constexpr (Backward) control.scouted[i & 1u][1][k] = kept;
             }
-            if (leader) control.ring[(i + S::kAhead) & 7u] = later;
+            if (leader)
+                control.ring[(i + S::kAhead) & 7u] =
+                    Work{x.x, !one_each && ticket < total ? x.y : kNone, x.z, ticket - place * a.groups, y.x, x.w, y.y, 0};
             arrive_at<kScouted>(i & 1u);
         }
     } else {
@@ -1101,14 +1116,21 @@ __global__ void __launch_bounds__(1024) scan_join_kernel(const __grid_constant__
     float A = 1.0f, H = 0.0f;
     bool cut = false;
     if (active)
-#pragma unroll 8
-        for (uint32_t i = begin; i < end; ++i) {
-            const Slot s = *slot(i);
-            const float value = __uint_as_float((uint32_t)(s >> 32)), product = __uint_as_float((uint32_t)s);
-            const bool here = (uint32_t)s == kNone;
-            H = here ? value : fmaf(product, H, value);
-            A *= product;
-            cut |= here;
+        for (uint32_t from = begin; from < end; from += 8) {
+            Slot s[8];
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j)
+                if (from + j < end) s[j] = *slot(from + j);
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j)
+                if (from + j < end) {
+                    const float value = __uint_as_float((uint32_t)(s[j] >> 32));
+                    const float product = __uint_as_float((uint32_t)s[j]);
+                    const bool here = (uint32_t)s[j] == kNone;
+                    H = here ? value : fmaf(product, H, value);
+                    A *= product;
+                    cut |= here;
+                }
         }
     products[warp][lane] = A, values[warp][lane] = H, cuts[warp][lane] = cut;
     __syncthreads();
@@ -1116,32 +1138,37 @@ __global__ void __launch_bounds__(1024) scan_join_kernel(const __grid_constant__
     for (uint32_t w = 0; w < warp; ++w)
         state = cuts[w][lane] ? values[w][lane] : fmaf(products[w][lane], state, values[w][lane]);
     if (active)
-#pragma unroll 8
-        for (uint32_t i = begin; i < end; ++i) {
-            Slot* p = slot(i);
-            const Slot s = *p;
-            const float value = __uint_as_float((uint32_t)(s >> 32));
-            state = (uint32_t)s == kNone ? value : fmaf(__uint_as_float((uint32_t)s), state, value);
-            *p = (Slot)__float_as_uint(state) << 32;
+        for (uint32_t from = begin; from < end; from += 8) {
+            Slot s[8];  // read together, before the first of them is written
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j)
+                if (from + j < end) s[j] = *slot(from + j);
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j)
+                if (from + j < end) {
+                    const float value = __uint_as_float((uint32_t)(s[j] >> 32));
+                    state = (uint32_t)s[j] == kNone ? value : fmaf(__uint_as_float((uint32_t)s[j]), state, value);
+                    *slot(from + j) = (Slot)__float_as_uint(state) << 32;
+                }
         }
     if (blockIdx.x == 0 && threadIdx.x == 0) *a.scratch.ticket = kNone;  // the next one is 0
 }
 
 // The gradient of a shared row of gates: the tiles' sums in double, a column of
-// 32 channels a block, every fourth tile a warp.
+// 32 channels a block, every 32nd tile a warp.
 template <typename G>
-__global__ void __launch_bounds__(kThreads) shared_decay_kernel(const float* partials, uint32_t tiles,
+__global__ void __launch_bounds__(kReduceThreads) shared_decay_kernel(const float* partials, uint32_t tiles,
                                                                 uint32_t channels, G* out) {
-    __shared__ double sums[kThreads / 32][32];
+    __shared__ double sums[kReduceThreads / 32][32];
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     double sum = 0.0;
     if (c < channels)
 #pragma unroll 8
-        for (uint32_t t = warp; t < tiles; t += kThreads / 32) sum += (double)partials[(size_t)t * channels + c];
+        for (uint32_t t = warp; t < tiles; t += kReduceThreads / 32) sum += (double)partials[(size_t)t * channels + c];
     sums[warp][lane] = sum;
     __syncthreads();
     if (warp || c >= channels) return;
-    for (uint32_t w = 1; w < kThreads / 32; ++w) sum += sums[w][lane];
+    for (uint32_t w = 1; w < kReduceThreads / 32; ++w) sum += sums[w][lane];
     store(out + c, (float)sum);
 }
 
@@ -1390,7 +1417,7 @@ void launch_scan(ScanArgs& a, void* workspace, size_t workspace_bytes, cudaStrea
     }
     // Tiles that may be worked on side by side without waiting for one another, of those in the longest row.
     const uint64_t abreast = total / a.tables.longest[halves];
-    a.ready = a.tables.longest[halves] > kGroup && abreast < kAbreast;
+    a.ready = a.tables.longest[halves] > kGroup && abreast < kAbreast[Backward];
     if (a.ready) {
         scan_map_kernel<T, G, Unit, Shared, Backward, S::kSegment>
             <<<(uint32_t)total, 16 * kSegments, 0, stream>>>(a);
@@ -1599,7 +1626,7 @@ int leo_b200_gated_scan_backward(int device, const LeoB200StoryTables* tables, u
             dispatch_shape(unit, shared, [&](auto u, auto is_shared) {
                 launch_scan<T, G, u(), is_shared(), true>(a, workspace, workspace_bytes, (cudaStream_t)stream);
                 if (decay_shared && a.tiles > 1) {
-                    shared_decay_kernel<G><<<(channels + 31) / 32, kThreads, 0, (cudaStream_t)stream>>>(
+                    shared_decay_kernel<G><<<(channels + 31) / 32, kReduceThreads, 0, (cudaStream_t)stream>>>(
                         a.scratch.partials, a.tiles, channels, static_cast<G*>(grad_decay));
                     check(cudaGetLastError(), "shared_decay_kernel");
                 }
