@@ -9,6 +9,8 @@ the same names and argument meaning:
   batch-end mean merge and the serial canonical replay, fused;
 * ``training_story_batch`` / ``training_story_batch_deltas`` --
   backend.rs:457-474 (no replay; the second keeps each story's delta);
+* ``next_symbol`` -- a frozen step of the open document and the pick of the
+  symbol that follows, under penalties, biases and a grammar mask;
 * ``begin_document`` / ``reset_transient_state`` / ``training_step_batch`` /
   ``advance_frozen_batch`` -- the canonical runtime step by step
   (backend.rs:391-431);
@@ -32,6 +34,7 @@ from .configs import Config
 from .ctypes_types import (
     CHANGE_LISTS,
     DELTA_TENSORS,
+    END_DOCUMENT,
     FROZEN,
     OUTPUT_CLASSES,
     TRAINING,
@@ -500,6 +503,47 @@ class GpuBackend:
         symbols, targets = self._steps(steps)
         native.check(native.lib().leo_b200_advance_frozen_batch(self.handle, symbols.ctypes.data,
                                                                  targets.ctypes.data, len(steps)))
+
+    def next_symbol(self, symbol: int, *, temperature: float = 0.0, uniform: float = 0.0, history=(),
+                    repetition: float = 1.0, presence: float = 0.0, frequency: float = 0.0, bias=None,
+                    allowed=None) -> tuple[int, float]:
+        """Reads ``symbol`` in the open document -- a frozen step, nothing is
+        learned -- and picks the symbol that follows it: (symbol, log
+        probability), 257 being the end of the document.
+
+        The step's 257 log-probabilities pass through the rules of
+        :func:`leo_b200.logits.pick_symbols`: penalties for the symbols of
+        ``history`` (bytes or symbol numbers), ``bias`` and ``allowed`` (257
+        numbers and truth values, the last for the end of the document), then
+        the largest at ``temperature`` 0, or the one that ``uniform`` in [0, 1)
+        falls on."""
+        import torch
+
+        from .logits import pack_allowed, pick_symbols
+
+        spoken = [OUTPUT_CLASSES - 1 if s == END_DOCUMENT else s if s < OUTPUT_CLASSES - 1 else -1 for s in history]
+        if not 0.0 <= uniform < 1.0:
+            raise ValueError("uniform must lie in [0, 1)")
+        if bias is not None and len(bias) != OUTPUT_CLASSES or allowed is not None and len(allowed) != OUTPUT_CLASSES:
+            raise ValueError(f"bias and allowed have {OUTPUT_CLASSES} entries, one a class")
+        # A target makes the step form its probabilities; a frozen one neither learns from it nor counts it.
+        self.training_step_batch([(symbol, 0)], FROZEN)
+        p = self.lane_array(self.CANONICAL_LANE, "probabilities", capacity=4 * OUTPUT_CLASSES)
+        where = torch.device("cuda", self.device)
+        rules = {"repetition": repetition, "presence": presence, "frequency": frequency}
+        if spoken:
+            rules["history"] = torch.tensor([spoken], dtype=torch.int32, device=where)
+        if bias is not None:
+            rules["bias"] = torch.as_tensor(bias, dtype=torch.float32).to(where)
+        if allowed is not None:
+            rules["allowed"] = pack_allowed(torch.as_tensor(allowed, dtype=torch.bool)[None]).to(where)
+        logits = torch.log(torch.from_numpy(p)).to(where)[None]
+        symbols, chance = pick_symbols(logits, temperature=temperature,
+                                       uniforms=torch.full((1,), uniform, dtype=torch.float64, device=where), **rules)
+        picked = int(symbols[0])
+        if picked < 0:
+            raise native.LeoError("no symbol is left to pick from")
+        return END_DOCUMENT if picked == OUTPUT_CLASSES - 1 else picked, float(chance[0])
 
     def enable_parameter_tracking(self) -> None:
         """RuntimeBackend::enable_parameter_tracking (backend.rs:358)."""
