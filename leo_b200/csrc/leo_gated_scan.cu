@@ -1403,11 +1403,10 @@ void launch_scan(ScanArgs& a, void* workspace, size_t workspace_bytes, cudaStrea
         require(workspace != nullptr && workspace_bytes >= size, "the workspace is too small");
         require(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "the workspace must be aligned to 16 bytes");
     }
-    int device = 0, sms = 0;
-    check(cudaGetDevice(&device), "cudaGetDevice");
-    check(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device), "SM count");
+    const int sms = sm_count();
     const auto kernel = scan_kernel<T, G, Unit, Shared, Backward>;
-    check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kBytes), "shared memory");
+    static std::atomic<uint64_t> allowed{0};
+    allow_shared(kernel, S::kBytes, allowed);
     if constexpr (Unit == 4) {
         const uint32_t rows = 2 * S::kSegment;
         describe<T>(&a.drive_map, a.drive, a.drive_stride, a.tables.tokens, a.channels, rows);

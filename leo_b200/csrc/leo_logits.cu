@@ -986,9 +986,8 @@ void launch_pick(const LogitArgs& a, cudaStream_t stream) {
     const auto kernel = pick_kernel<T, Warps>;
     const size_t shared = steps * sizeof(Weights) +
                           (a.rules.history ? std::min(steps, kPickWindow) * kStepSymbols * sizeof(uint32_t) : 0);
-    check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)(4096 * sizeof(Weights) + kPickWindow * kStepSymbols * sizeof(uint32_t))),
-          "shared memory");
+    static std::atomic<uint64_t> allowed{0};
+    allow_shared(kernel, 4096 * sizeof(Weights) + kPickWindow * kStepSymbols * sizeof(uint32_t), allowed);
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(a.rows * blocks);
     config.blockDim = dim3(32 * Warps);

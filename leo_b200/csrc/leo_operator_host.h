@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <exception>
 #include <stdexcept>
 #include <string>
@@ -47,6 +48,29 @@ class DeviceScope {
     int previous_ = 0;
     bool switched_ = false;
 };
+
+// SMs of the current device, asked for once a device.
+inline int sm_count() {
+    static std::atomic<int> known[64];
+    int device = 0, sms = 0;
+    check(cudaGetDevice(&device), "cudaGetDevice");
+    if (device < 64 && (sms = known[device].load(std::memory_order_relaxed)) > 0) return sms;
+    check(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device), "SM count");
+    if (device < 64) known[device].store(sms, std::memory_order_relaxed);
+    return sms;
+}
+
+// Lets `kernel` have `bytes` of dynamic shared memory on the current device;
+// `done` remembers for which devices that has been said.
+template <typename Kernel>
+void allow_shared(Kernel kernel, size_t bytes, std::atomic<uint64_t>& done) {
+    int device = 0;
+    check(cudaGetDevice(&device), "cudaGetDevice");
+    const uint64_t bit = device < 64 ? 1ull << device : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return;
+    check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), "shared memory");
+    done.fetch_or(bit, std::memory_order_relaxed);
+}
 
 template <typename Body>
 int guarded(Body&& body) noexcept {

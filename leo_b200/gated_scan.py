@@ -140,12 +140,11 @@ def gated_scan(drive, decay, layout: StoryLayout, initial=None, keep_carries: bo
     tokens, channels = drive.shape
     L = native.lib()
     size, kept = layout._needs(channels)
-    where = layout.device
     with on_stream(device, stream, (drive, decay, initial)) as raw:
-        states = torch.empty((tokens, channels), dtype=drive.dtype, device=where)
-        final = torch.empty((layout.stories, channels), dtype=torch.float32, device=where)
-        carries = torch.empty(kept, dtype=torch.float32, device=where) if keep_carries else None
-        scratch = torch.empty(size, dtype=torch.uint8, device=where) if size else None
+        states = drive.new_empty((tokens, channels))
+        final = drive.new_empty((layout.stories, channels), dtype=torch.float32)
+        carries = drive.new_empty(kept, dtype=torch.float32) if keep_carries else None
+        scratch = drive.new_empty(size, dtype=torch.uint8) if size else None
         native.check(L.leo_b200_gated_scan(
             device, layout._ref, channels, code, drive.data_ptr(), stride, decay_code, decay.data_ptr(), decay_stride,
             shared, pointer(initial), states.data_ptr(), final.data_ptr(), pointer(carries), pointer(scratch), size,
@@ -173,14 +172,13 @@ def gated_scan_backward(grad_states, drive, decay, layout: StoryLayout, carries,
     size, kept = layout._needs(channels)
     check_tensor("carries", carries, device, torch.float32, (kept,))
     check_contiguous("carries", carries)
-    where = layout.device
     with on_stream(device, stream, (grad_states, drive, decay, carries, initial, grad_final)) as raw:
-        grad_drive = torch.empty((tokens, channels), dtype=drive.dtype, device=where)
-        grad_decay = torch.empty(decay.shape, dtype=decay.dtype, device=where)
+        grad_drive = drive.new_empty((tokens, channels))
+        grad_decay = decay.new_empty(decay.shape)
         grad_initial = None
         if initial is not None:
-            grad_initial = torch.empty((layout.stories, channels), dtype=torch.float32, device=where)
-        scratch = torch.empty(size, dtype=torch.uint8, device=where) if size else None
+            grad_initial = initial.new_empty((layout.stories, channels))
+        scratch = drive.new_empty(size, dtype=torch.uint8) if size else None
         native.check(L.leo_b200_gated_scan_backward(
             device, layout._ref, channels, code, grad_states.data_ptr(), grad_stride, drive.data_ptr(), stride,
             decay_code, decay.data_ptr(), decay_stride, shared, pointer(initial), pointer(grad_final),
@@ -212,7 +210,7 @@ def gated_step(drive, decay, state, stream=None):
     if state_stride < channels and lanes > 1:
         raise ValueError("the rows of state overlap")
     with on_stream(device, stream, (drive, decay, state)) as raw:
-        output = torch.empty((lanes, channels), dtype=drive.dtype, device=drive.device)
+        output = drive.new_empty((lanes, channels))
         native.check(native.lib().leo_b200_gated_step(
             device, lanes, channels, code, drive.data_ptr(), stride, decay_code, decay.data_ptr(), decay_stride, shared,
             state.data_ptr(), state_stride, output.data_ptr(), raw))

@@ -20,6 +20,7 @@ float32 CUDA tensors ``[rows]`` (whose values are then not checked).
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
@@ -81,8 +82,15 @@ def _scalar_or_rows(name: str, value, logits, device):
     return None, float(value)
 
 
+# LeoB200LogitRules as bytes, which are made faster than a structure of ctypes.
+_RULES = struct.Struct("@PqIPPPPfffPqPqIP")
+assert _RULES.size == C.sizeof(LeoB200LogitRules)
+
+
 class _Rules:
     """The checked rules of a call, and the tensors that they point at."""
+
+    __slots__ = ("tensors", "packed")
 
     def __init__(self, logits, device, history, lengths, repetition, presence, frequency, bias, allowed, state):
         rows, vocabulary = logits.shape
@@ -115,10 +123,10 @@ class _Rules:
                 bias_stride = row_stride("bias", bias)
         allowed_stride, states = _check_mask(logits, device, allowed, state)
         self.tensors = (logits, history, lengths, repetition_rows, presence_rows, frequency_rows, bias, allowed, state)
-        self.c = LeoB200LogitRules(
-            pointer(history), history_stride, capacity, pointer(lengths), pointer(repetition_rows),
-            pointer(presence_rows), pointer(frequency_rows), repetition, presence, frequency, pointer(bias),
-            bias_stride, pointer(allowed), allowed_stride, states, pointer(state))
+        address = [0 if x is None else x.data_ptr() for x in self.tensors]
+        self.packed = _RULES.pack(address[1], history_stride, capacity, address[2], address[3], address[4], address[5],
+                                  repetition, presence, frequency, address[6], bias_stride, address[7],
+                                  allowed_stride, states, address[8])
 
 
 def adjust_logits(logits, *, history=None, lengths=None, repetition=1.0, presence=0.0, frequency=0.0, bias=None,
@@ -141,9 +149,9 @@ def adjust_logits(logits, *, history=None, lengths=None, repetition=1.0, presenc
             raise ValueError("the rows of out overlap")
     with on_stream(device, stream, rules.tensors + (out,)) as raw:
         if out is None:
-            out = torch.empty((rows, vocabulary), dtype=logits.dtype, device=logits.device)
+            out = logits.new_empty((rows, vocabulary))
         native.check(native.lib().leo_b200_adjust_logits(
-            device, code, logits.data_ptr(), stride, rows, vocabulary, C.byref(rules.c), out.data_ptr(),
+            device, code, logits.data_ptr(), stride, rows, vocabulary, rules.packed, out.data_ptr(),
             out.stride(0), raw))
     return out
 
@@ -169,10 +177,10 @@ def pick_symbols(logits, *, temperature=0.0, uniforms=None, history=None, length
         check_tensor("uniforms", uniforms, device, torch.float64, (rows,))
         check_contiguous("uniforms", uniforms)
     with on_stream(device, stream, rules.tensors + (temperature_rows, uniforms)) as raw:
-        symbols = torch.empty(rows, dtype=torch.int32, device=logits.device)
-        log_probability = torch.empty(rows, dtype=torch.float32, device=logits.device)
+        symbols = logits.new_empty(rows, dtype=torch.int32)
+        log_probability = logits.new_empty(rows, dtype=torch.float32)
         native.check(native.lib().leo_b200_pick_symbols(
-            device, code, logits.data_ptr(), stride, rows, vocabulary, C.byref(rules.c),
+            device, code, logits.data_ptr(), stride, rows, vocabulary, rules.packed,
             pointer(temperature_rows), temperature, pointer(uniforms), symbols.data_ptr(),
             log_probability.data_ptr(), raw))
     return symbols, log_probability
@@ -199,8 +207,8 @@ def masked_cross_entropy(logits, targets, *, allowed=None, state=None, weights=N
         check_tensor("weights", weights, device, torch.float32, (rows,))
         check_contiguous("weights", weights)
     with on_stream(device, stream, (logits, targets, allowed, state, weights)) as raw:
-        losses = torch.empty(rows, dtype=torch.float32, device=logits.device)
-        gradient = torch.empty((rows, vocabulary), dtype=logits.dtype, device=logits.device)
+        losses = logits.new_empty(rows, dtype=torch.float32)
+        gradient = logits.new_empty((rows, vocabulary))
         native.check(native.lib().leo_b200_masked_cross_entropy(
             device, code, logits.data_ptr(), stride, rows, vocabulary, targets.data_ptr(),
             pointer(allowed), allowed_stride, states, pointer(state), pointer(weights), losses.data_ptr(),

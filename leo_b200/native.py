@@ -12,7 +12,6 @@ from .ctypes_types import (
     LeoB200BatchReport,
     LeoB200Config,
     LeoB200HostModel,
-    LeoB200LogitRules,
     LeoB200PackedUpdate,
     LeoB200ParameterChanges,
     LeoB200ParameterChangeSizes,
@@ -125,8 +124,8 @@ def lib() -> C.CDLL:
                                                i32, vp, vp, vp, vp, vp, vp, vp, sz, vp]
     L.leo_b200_gated_scan_status.argtypes = [i32, P(u32)]
     L.leo_b200_gated_step.argtypes = [i32, u32, u32, i32, vp, i64, i32, vp, i64, i32, vp, i64, vp, vp]
-    L.leo_b200_adjust_logits.argtypes = [i32, i32, vp, i64, u32, u32, P(LeoB200LogitRules), vp, i64, vp]
-    L.leo_b200_pick_symbols.argtypes = [i32, i32, vp, i64, u32, u32, P(LeoB200LogitRules), vp, f32, vp, vp, vp, vp]
+    L.leo_b200_adjust_logits.argtypes = [i32, i32, vp, i64, u32, u32, vp, vp, i64, vp]  # rules: their bytes
+    L.leo_b200_pick_symbols.argtypes = [i32, i32, vp, i64, u32, u32, vp, vp, f32, vp, vp, vp, vp]
     L.leo_b200_masked_cross_entropy.argtypes = [i32, i32, vp, i64, u32, u32, vp, vp, i64, u32, vp, vp, vp, vp, i64, vp]
     _lib = L
     return L
