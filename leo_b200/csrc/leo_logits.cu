@@ -240,57 +240,68 @@ __device__ __forceinline__ void read_bias(const RowRules& k, const Row<T>& row, 
     }
 }
 
-// A block takes a chunk of a row, two groups a thread, which it reads before it
-// counts the history's symbols of the chunk in shared memory: any vocabulary
-// and history fit, and the chunks of a long row run side by side.
+// A block takes a run of a row, of up to kAdjustRun symbols: it counts the
+// history's symbols in it once, in shared memory, then goes through it with the
+// groups of the next turn in flight.  Any vocabulary and history fit, and the runs
+// of a long row go side by side.  (256 x 50,001 with 1,000 symbols of history: 33 us
+// in runs of 4,096 symbols, whose counts then take longer than their logits.)
 constexpr uint32_t kAdjustThreads = 256;
-constexpr uint32_t kAdjustGroups = 2;
-constexpr uint32_t kAdjustSpan = kAdjustThreads * kAdjustGroups * 8;
+constexpr uint32_t kAdjustTurn = kAdjustThreads * 8;   // symbols of a turn
+constexpr uint32_t kAdjustRun = 4 * kAdjustTurn;
 
 template <typename T>
-__global__ void __launch_bounds__(kAdjustThreads) adjust_kernel(const __grid_constant__ LogitArgs a, uint32_t chunks) {
-    __shared__ __align__(16) uint32_t counts[kAdjustSpan];
-    const uint32_t at = blockIdx.x / chunks, chunk = blockIdx.x - at * chunks;
+__global__ void __launch_bounds__(kAdjustThreads) adjust_kernel(const __grid_constant__ LogitArgs a, uint32_t runs,
+                                                                uint32_t turns) {
+    extern __shared__ __align__(16) uint32_t run_counts[];
+    const uint32_t at = blockIdx.x / runs, run = blockIdx.x - at * runs;
     const Row<T> row(static_cast<const T*>(a.logits) + (int64_t)at * a.logits_stride, a.vocabulary);
     T* out = static_cast<T*>(a.out) + (int64_t)at * a.out_stride;
     const RowRules k = row_rules(a.rules, at);
     const bool aligned = row.alike(out);
-    const int32_t first = row.first + (int32_t)(chunk * kAdjustSpan);
-    Eight<T> e[kAdjustGroups];
-    float bias[kAdjustGroups][8] = {};
-#pragma unroll
-    for (uint32_t j = 0; j < kAdjustGroups; ++j) {
-        const int32_t v = first + (int32_t)(j * blockDim.x + threadIdx.x) * 8;
-        if (v < (int32_t)a.vocabulary) {
-            e[j] = row.read(v);
-            read_bias(k, row, v, bias[j]);
+    const int32_t first = row.first + (int32_t)(run * turns * kAdjustTurn);
+    const auto symbol_of = [&](uint32_t turn) { return first + (int32_t)(turn * kAdjustTurn + threadIdx.x * 8); };
+    Eight<T> next;
+    float next_bias[8] = {};
+    const auto ask = [&](uint32_t turn) {
+        const int32_t v = symbol_of(turn);
+        if (turn < turns && v < (int32_t)a.vocabulary) {
+            next = row.read(v);
+            read_bias(k, row, v, next_bias);
         }
-    }
-    if (k.length) count_history(k, first, kAdjustSpan, counts);
+    };
+    ask(0);
+    if (k.length) count_history(k, first, turns * kAdjustTurn, run_counts);
+    for (uint32_t turn = 0; turn < turns; ++turn) {
+        const int32_t v = symbol_of(turn);
+        if (v >= (int32_t)a.vocabulary) return;
+        const Eight<T> e = next;
+        float bias[8];
 #pragma unroll
-    for (uint32_t j = 0; j < kAdjustGroups; ++j) {
-        const uint32_t within = (j * blockDim.x + threadIdx.x) * 8;
-        const int32_t v = first + (int32_t)within;
-        if (v >= (int32_t)a.vocabulary) continue;
+        for (int i = 0; i < 8; ++i) bias[i] = next_bias[i];
+        ask(turn + 1);
         const uint32_t ok = k.mask.eight(v, a.vocabulary);
-        uint32_t c[8] = {};
+        uint4 c[2] = {};
         if (k.length) {
-            const uint4 x = *reinterpret_cast<const uint4*>(counts + within),
-                        y = *reinterpret_cast<const uint4*>(counts + within + 4);
-            c[0] = x.x, c[1] = x.y, c[2] = x.z, c[3] = x.w, c[4] = y.x, c[5] = y.y, c[6] = y.z, c[7] = y.w;
+            c[0] = *reinterpret_cast<const uint4*>(run_counts + (v - first));
+            c[1] = *reinterpret_cast<const uint4*>(run_counts + (v - first) + 4);
+        }
+        float z[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] = k.bias ? e[i] + bias[i] : e[i];
+        if (((c[0].x | c[0].y) | (c[0].z | c[0].w) | (c[1].x | c[1].y) | (c[1].z | c[1].w)) != 0) {
+            const uint32_t count[8] = {c[0].x, c[0].y, c[0].z, c[0].w, c[1].x, c[1].y, c[1].z, c[1].w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (count[i]) z[i] = adjusted(e[i], count[i], k, 0.0f, bias[i], true);
+        }
+        if (ok != 0xffu) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (!(ok >> i & 1u)) z[i] = -CUDART_INF_F;
         }
         Eight<T> r;
-        if (((c[0] | c[1]) | (c[2] | c[3]) | (c[4] | c[5]) | (c[6] | c[7])) == 0 && ok == 0xffu) {
-            // nothing of these was said before, and nothing is masked
-            r = e[j];
-            if (k.bias)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    r.set_pair(i, add2(e[j].pair(i), pair_of(bias[j][2 * i], bias[j][2 * i + 1])));
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) r.set(i, adjusted(e[j][i], c[i], k, 0.0f, bias[j][i], ok >> i & 1u));
-        }
+        for (int i = 0; i < 4; ++i) r.set_pair(i, pair_of(z[2 * i], z[2 * i + 1]));
         row.write(out, aligned, v, r);
     }
 }
@@ -862,8 +873,12 @@ __global__ void __launch_bounds__(256) narrow_loss_kernel(const __grid_constant_
     }
 }
 
-// Wider rows, a block each: up to Held groups a thread stay in registers
-// between the sweeps; what lies beyond is read again (out of L2).
+// Wider rows, a block each, in three sweeps: the largest logit, the sum of the
+// weights, the gradient.  A row that fits is copied into shared memory first,
+// each thread the groups that it will sweep, so that it comes from memory once
+// and three blocks an SM overlap their copies with the others' sweeps (2,048 x
+// 32,001 bfloat16: 87 us with the row in registers and two blocks); a larger one
+// is read in every sweep, the last two times out of L2.
 template <int Threads, bool Maximum>
 __device__ __forceinline__ float block_of(float v, float* shared) {
     v = Maximum ? warp_max(v) : warp_sum(v);
@@ -873,23 +888,37 @@ __device__ __forceinline__ float block_of(float v, float* shared) {
     return Maximum ? warp_max(v) : warp_sum(v);
 }
 
-template <typename T, int Threads, int Held>
-__global__ void __launch_bounds__(Threads) wide_loss_kernel(const __grid_constant__ LossArgs a) {
+template <typename T, int Threads, bool Held>
+__global__ void __launch_bounds__(Threads, Held ? 3 : 2) wide_loss_kernel(const __grid_constant__ LossArgs a) {
+    extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ float shared[2][32];
     const uint32_t at = blockIdx.x;
     const Row<T> row(static_cast<const T*>(a.logits) + (int64_t)at * a.logits_stride, a.vocabulary);
     T* out = static_cast<T*>(a.gradient) + (int64_t)at * a.gradient_stride;
     const bool aligned = row.alike(out);
     const auto symbol_of = [&](uint32_t g) { return row.first + (int32_t)g * 8; };
-    Eight<T> held[Held];
+    Eight<T>* held = reinterpret_cast<Eight<T>*>(dynamic);
+    if constexpr (Held) {
+        for (uint32_t g = threadIdx.x; g < row.groups; g += Threads) {
+            const int32_t v = symbol_of(g);
+            if (row.whole(v)) {
+                const uint32_t to = (uint32_t)__cvta_generic_to_shared(held + g);
 #pragma unroll
-    for (int j = 0; j < Held; ++j) {
-        const uint32_t g = j * Threads + threadIdx.x;
-        if (g < row.groups) held[j] = row.read(symbol_of(g));
+                for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 16 * i),
+                                 "l"(reinterpret_cast<const uint4*>(row.p + v) + i)
+                                 : "memory");
+            } else {
+                held[g] = row.read(v);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     }
     const int32_t target = a.targets[at];
     const MaskRow mask = mask_row(a.allowed, a.allowed_stride, a.states, a.state, at);
+    const float scale = a.weights ? a.weights[at] : 1.0f;
     const bool outside = target >= 0 && (uint32_t)target >= a.vocabulary;
+    if constexpr (Held) asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (target < 0 || outside) {
         Eight<T> zero;
 #pragma unroll
@@ -908,13 +937,13 @@ __global__ void __launch_bounds__(Threads) wide_loss_kernel(const __grid_constan
         return ok;
     };
     const auto each = [&](auto&& body) {
-#pragma unroll
-        for (int j = 0; j < Held; ++j) {
-            const uint32_t g = j * Threads + threadIdx.x;
-            if (g < row.groups) body(held[j], symbol_of(g));
+#pragma unroll 2
+        for (uint32_t g = threadIdx.x; g < row.groups; g += Threads) {
+            if constexpr (Held)
+                body(held[g], symbol_of(g));
+            else
+                body(row.read(symbol_of(g)), symbol_of(g));
         }
-        for (uint32_t g = Held * Threads + threadIdx.x; g < row.groups; g += Threads)
-            body(row.read(symbol_of(g)), symbol_of(g));
     };
     float top = -CUDART_INF_F;
     each([&](const Eight<T>& e, int32_t v) {
@@ -942,7 +971,7 @@ __global__ void __launch_bounds__(Threads) wide_loss_kernel(const __grid_constan
     });
     const float2 halves = parts(sums);
     const float sum = block_of<Threads, false>(halves.x + halves.y, shared[1]);
-    const float scale = a.weights ? a.weights[at] : 1.0f, gain = sum == 0.0f ? 0.0f : scale / sum;
+    const float gain = sum == 0.0f ? 0.0f : scale / sum;
     each([&](const Eight<T>& e, int32_t v) {
         const uint32_t ok = counts_at(v);
         Eight<T> r;
@@ -1009,8 +1038,16 @@ void launch_loss(const LossArgs& a, cudaStream_t stream) {
     if (v <= 288) narrow_loss_kernel<T, 9><<<warps, 256, 0, stream>>>(a);
     else if (v <= 512) narrow_loss_kernel<T, 16><<<warps, 256, 0, stream>>>(a);
     else if (v <= 1024) narrow_loss_kernel<T, 32><<<warps, 256, 0, stream>>>(a);
-    else if (v <= 8000) wide_loss_kernel<T, 256, 4><<<a.rows, 256, 0, stream>>>(a);
-    else wide_loss_kernel<T, 512, sizeof(T) == 2 ? 8 : 4><<<a.rows, 512, 0, stream>>>(a);
+    else if (const size_t held = ((size_t)v + 14) / 8 * sizeof(Eight<T>); held <= 110 * 1024) {
+        // three blocks an SM up to 75 KB a row, two up to 110 KB
+        const bool small = v <= 8192;
+        const auto kernel = small ? wide_loss_kernel<T, 256, true> : wide_loss_kernel<T, 512, true>;
+        static std::atomic<uint64_t> allowed[2];
+        allow_shared(kernel, 110 * 1024, allowed[small]);
+        kernel<<<a.rows, small ? 256 : 512, held, stream>>>(a);
+    } else {
+        wide_loss_kernel<T, 512, false><<<a.rows, 512, 0, stream>>>(a);
+    }
 }
 
 void check_mask(const uint32_t* allowed, int64_t stride, uint32_t states, const int32_t* state, uint32_t rows,
@@ -1062,10 +1099,12 @@ int leo_b200_adjust_logits(int device, int dtype, const void* logits, int64_t lo
             a.out = out;
             a.out_stride = out_stride;
             DeviceScope scope(device);
-            // A chunk more than the symbols take, if a row can start off a 16-byte address.
-            const uint32_t chunks = (vocabulary + 7 + kAdjustSpan - 1) / kAdjustSpan;
-            require((uint64_t)rows * chunks < (1ull << 31), "too many rows for one call");
-            adjust_kernel<T><<<rows * chunks, kAdjustThreads, 0, (cudaStream_t)stream>>>(a, chunks);
+            // A turn more than the symbols take, if a row can start off a 16-byte address.
+            const uint32_t all = (vocabulary + 7 + kAdjustTurn - 1) / kAdjustTurn;
+            const uint32_t turns = std::min(all, kAdjustRun / kAdjustTurn), runs = (all + turns - 1) / turns;
+            require((uint64_t)rows * runs < (1ull << 31), "too many rows for one call");
+            const size_t shared = rules->history ? turns * kAdjustTurn * sizeof(uint32_t) : 0;
+            adjust_kernel<T><<<rows * runs, kAdjustThreads, shared, (cudaStream_t)stream>>>(a, runs, turns);
             check(cudaGetLastError(), "adjust_kernel");
         });
     });
