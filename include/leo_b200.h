@@ -381,14 +381,15 @@ int leo_b200_gated_scan_backward(int device, const LeoB200StoryTables* tables, u
                                  const float* carries, void* grad_drive, void* grad_decay, float* grad_initial,
                                  void* workspace, size_t workspace_bytes, void* stream);
 
-/* A wait between the thread blocks of one scan gave up (it never should: a
-   block only waits for blocks that started before it): the states after it
-   are NaN.  Stores whether that happened on `device` since the library was
+/* Every wait inside a scan has a limit, after which it gives up.  None should
+   ever reach it (a thread block only waits for its own copies and for blocks
+   that started before it); a scan in which one did leaves NaN or unfinished
+   states.  Stores whether that happened on `device` since the library was
    loaded; waits for the device. */
 int leo_b200_gated_scan_status(int device, uint32_t* gave_up);
 
 /* One token for each of `lanes` lanes: state = decay * state + drive in place
-   (float, [lanes] rows), output = the state in `dtype` (rows adjacent). */
+   (float, [lanes] rows that do not overlap), output = the state in `dtype` (rows adjacent). */
 int leo_b200_gated_step(int device, uint32_t lanes, uint32_t channels, int dtype, const void* drive,
                         int64_t drive_stride, int decay_dtype, const void* decay, int64_t decay_stride,
                         int decay_shared, float* state, int64_t state_stride, void* output, void* stream);
@@ -398,7 +399,8 @@ int leo_b200_gated_step(int device, uint32_t lanes, uint32_t channels, int dtype
        c > 0:  l = l > 0 ? l / repetition : l * repetition;  l -= presence + frequency * c
        l += bias[v]
        l = -inf where the mask forbids v, whatever it was before (NaN too).
-   Computed in float, rounded once to `dtype`. */
+   Computed in float, rounded once to `dtype`.  `out` may be `logits` itself
+   with the same stride. */
 int leo_b200_adjust_logits(int device, int dtype, const void* logits, int64_t logits_stride, uint32_t rows,
                            uint32_t vocabulary, const LeoB200LogitRules* rules, void* out, int64_t out_stride,
                            void* stream);
@@ -411,8 +413,9 @@ int leo_b200_adjust_logits(int device, int dtype, const void* logits, int64_t lo
    not wanted) receives log p[v], at temperature 1 for a greedy row.  A row
    in which nothing is left (everything masked or -inf) gives symbol -1 and
    -inf; a row with a NaN logit that is not masked, or whose temperature is
-   negative or NaN, gives -1 and NaN.  `temperature` is [rows] or NULL
-   (temperature_value in every row); `uniforms` may be NULL only if that is 0. */
+   negative or NaN, gives -1 and NaN.  Weights below e^-708 of the largest
+   count as 0.  `temperature` is [rows] or NULL (temperature_value in every
+   row); `uniforms` may be NULL only if that is 0.  Up to 8,388,600 symbols. */
 int leo_b200_pick_symbols(int device, int dtype, const void* logits, int64_t logits_stride, uint32_t rows,
                           uint32_t vocabulary, const LeoB200LogitRules* rules, const float* temperature,
                           float temperature_value, const double* uniforms, int32_t* symbols, float* log_probability,

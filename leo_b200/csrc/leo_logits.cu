@@ -1069,7 +1069,8 @@ void check_rules(const LeoB200LogitRules* r, uint32_t rows, uint32_t vocabulary)
 }
 
 void check_rows(const void* logits, int64_t stride, uint32_t rows, uint32_t vocabulary) {
-    require(vocabulary > 0 && vocabulary < (1u << 31), "the vocabulary must not be empty");
+    require(vocabulary > 0, "the vocabulary must not be empty");
+    require(vocabulary <= (1u << 30), "the vocabulary is too large");
     require(rows < (1u << 31), "too many rows for one call");
     require(rows == 0 || logits != nullptr, "logits are null");
     require(rows <= 1 || stride >= 0, "the row stride must not be negative");

@@ -10,7 +10,6 @@ import torch
 from .ctypes_types import BF16, F16, F32
 
 DTYPE_CODES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
-_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 
 
 def device_of(name: str, tensor) -> int:
@@ -71,6 +70,11 @@ def pointer(tensor) -> int | None:
     return None if tensor is None else tensor.data_ptr()
 
 
+def current_stream(device: int) -> int:
+    """The raw current stream of a device."""
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
 @contextlib.contextmanager
 def _other_stream(stream, tensors):
     with torch.cuda.stream(stream):
@@ -102,8 +106,7 @@ def on_stream(device: int, stream, tensors):
     belong to the stream that writes them; with a ``stream`` other than the
     current one, ``tensors`` (the call's inputs) are marked as used on it."""
     if stream is None:
-        raw = _raw_stream(device) if _raw_stream else torch.cuda.current_stream(device).cuda_stream
-        return _CurrentStream(raw)
+        return _CurrentStream(current_stream(device))
     if stream.device.index != device:
         raise ValueError(f"the stream is on {stream.device}, not on cuda:{device}")
     return _other_stream(stream, tensors)

@@ -29,7 +29,16 @@ import torch
 
 from . import native
 from .ctypes_types import LeoB200StoryTables
-from .device_tensors import check_contiguous, check_tensor, device_of, dtype_code, on_stream, pointer, row_stride
+from .device_tensors import (
+    check_contiguous,
+    check_tensor,
+    current_stream,
+    device_of,
+    dtype_code,
+    on_stream,
+    pointer,
+    row_stride,
+)
 
 
 class StoryLayout:
@@ -65,8 +74,15 @@ class StoryLayout:
         native.check(L.leo_b200_story_table(offsets.ctypes.data, stories, host.data_ptr(), size,
                                             self._table.data_ptr(), self._ref))
         self._table.copy_(host)  # waits for the copy
+        self._home = current_stream(device.index)
         # (scratch bytes, carries) by channels: what every call asks for
         self._sizes: dict[int, tuple[int, int]] = {}
+
+    def _used_on(self, raw: int, stream) -> None:
+        """Keeps the table from other uses of its memory until a call on a
+        stream other than its own has read it."""
+        if raw != self._home:
+            self._table.record_stream(stream or torch.cuda.current_stream(self.device))
 
     def _needs(self, channels: int) -> tuple[int, int]:
         needs = self._sizes.get(channels)
@@ -149,6 +165,7 @@ def gated_scan(drive, decay, layout: StoryLayout, initial=None, keep_carries: bo
             device, layout._ref, channels, code, drive.data_ptr(), stride, decay_code, decay.data_ptr(), decay_stride,
             shared, pointer(initial), states.data_ptr(), final.data_ptr(), pointer(carries), pointer(scratch), size,
             raw))
+        layout._used_on(raw, stream)
     return GatedScan(states, final, carries)
 
 
@@ -184,12 +201,13 @@ def gated_scan_backward(grad_states, drive, decay, layout: StoryLayout, carries,
             decay_code, decay.data_ptr(), decay_stride, shared, pointer(initial), pointer(grad_final),
             carries.data_ptr(), grad_drive.data_ptr(), grad_decay.data_ptr(), pointer(grad_initial),
             pointer(scratch), size, raw))
+        layout._used_on(raw, stream)
     return GatedScanGradients(grad_drive, grad_decay, grad_initial)
 
 
 def gated_scan_gave_up(device: int = 0) -> bool:
-    """Whether a wait inside a scan on ``device`` ever gave up (its states are
-    then NaN from there on).  Waits for the device."""
+    """Whether a wait inside a scan on ``device`` ever gave up, which it should
+    never do; that scan's results are not to be used.  Waits for the device."""
     flag = C.c_uint32()
     native.check(native.lib().leo_b200_gated_scan_status(device, C.byref(flag)))
     return bool(flag.value)

@@ -164,11 +164,13 @@ def pick_symbols(logits, *, temperature=0.0, uniforms=None, history=None, length
     Rows of ``temperature`` 0 take the largest adjusted logit, the lowest
     symbol of equal ones.  Others take the first symbol at which the running
     sum of the softmax of ``adjusted / temperature`` passes ``uniforms[row]``
-    (float64, in [0, 1)).  ``log_probability`` is that of the symbol, at
+    (float64, in [0, 1); it may be ``None`` only if ``temperature`` is the number 0).
+    ``log_probability`` is that of the symbol, at
     temperature 1 for a greedy row.  A row with nothing left gives symbol -1
     and -inf; one with a NaN that is not masked (or a temperature that is
     negative or NaN) -1 and NaN.  Everything is computed in 64 bits from the
-    inputs as they are."""
+    inputs as they are, weights below e^-708 of the largest counting as 0; up to
+    8,388,600 symbols."""
     device, code, stride = _check_logits(logits)
     rules = _Rules(logits, device, history, lengths, repetition, presence, frequency, bias, allowed, state)
     rows, vocabulary = logits.shape

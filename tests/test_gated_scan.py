@@ -321,6 +321,17 @@ def test_scan_and_gradients(native_lib, lengths, channels, dtype, decay):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lengths,channels,dtype,decay", [
+    ([3000, 600], 1600, "bf16", "f32"), ([2300], 1537, "f32", "f32"), ([5000], 768, "f16", "channel"),
+    ([40, 3500, 100, 2700], 648, "f32", "channel"), ([2500, 7], 1282, "bf16", "bf16")])
+def test_long_stories_of_many_channels(native_lib, lengths, channels, dtype, decay):
+    """States handed from tile to tile in one pass, over more tiles than a tile looks back."""
+    s = make(31, lengths, channels, DTYPES[dtype], decay, True, "cuda")
+    scan, grad = run_all(s, lengths)
+    check_all(s, lengths, scan, grad)
+
+
+@pytest.mark.gpu
 def test_one_story_over_many_blocks(native_lib):
     """A story long enough that partial states of distant blocks meet, gates near 1."""
     lengths = [20_011]
@@ -375,8 +386,13 @@ def test_rows_of_wider_tensors(native_lib):
 
 @pytest.mark.gpu
 def test_a_story_never_reaches_another(native_lib):
-    """NaN and infinities of one story stay in it, in both directions."""
-    lengths, channels = [90, 200, 61], 64
+    """NaN and infinities of one story stay in it, in both directions: in one
+    tile, over many tiles mapped ahead, and over many in one pass."""
+    for lengths, channels in (([90, 200, 61], 64), ([90, 200, 2600, 61], 64), ([90, 200, 2600, 61], 1540)):
+        check_isolation(lengths, channels)
+
+
+def check_isolation(lengths, channels):
     s = make(13, lengths, channels, torch.float32, "f32", True, "cuda")
     clean, clean_grad = run_all(s, lengths)
     for bad in (float("nan"), float("inf")):
@@ -388,7 +404,7 @@ def test_a_story_never_reaches_another(native_lib):
             assert torch.equal(a[:90], b[:90]) and torch.equal(a[290:], b[290:])
             assert not torch.isfinite(a[90:290]).all()
         for a, b in ((scan.final, clean.final), (grad.initial, clean_grad.initial)):
-            assert torch.equal(a[0], b[0]) and torch.equal(a[2], b[2])
+            assert torch.equal(a[0], b[0]) and torch.equal(a[2:], b[2:])
 
 
 @pytest.mark.gpu
@@ -482,6 +498,14 @@ def test_other_streams(native_lib):
     for scan, grad in got:
         assert torch.equal(scan.states, want.states) and torch.equal(scan.final, want.final)
         assert torch.equal(grad.drive, want_grad.drive) and torch.equal(grad.decay, want_grad.decay)
+    # a layout that goes away while another stream still reads it
+    for st in streams:
+        with torch.cuda.stream(st):
+            torch.cuda._sleep(2_000_000)
+            got = run_all(s, lengths, layout_of(lengths))
+        torch.full((1 << 16,), 7, dtype=torch.uint8, device="cuda")
+        st.synchronize()
+        assert torch.equal(got[0].states, want.states)
 
 
 @pytest.mark.gpu
