@@ -808,6 +808,11 @@ struct RowScale {
         const float2 x = parts(fma2(z, pair_of(c, c), pair_of(-shift, -shift)));
         return pair_of(exp2_of(x.x), exp2_of(x.y));
     }
+    // What makes weights by `part`, of some of the row's symbols, weights by this one.  Where
+    // the two differ in c they are so far apart that nothing of the part is left.
+    __device__ __forceinline__ float of(const RowScale& part) const {
+        return part.top == -CUDART_INF_F || part.c != c ? 0.0f : part.top == top ? 1.0f : exp2_of(part.shift - shift);
+    }
     // Loss of a row with the sum of its weights and the (masked) logit of its target.
     __device__ __forceinline__ float loss(float sum, float z) const {
         if (sum != sum) return sum;
@@ -874,20 +879,12 @@ __global__ void __launch_bounds__(256) narrow_loss_kernel(const __grid_constant_
 }
 
 // Wider rows, a block each, in three sweeps: the largest logit, the sum of the
-// weights, the gradient.  A row that fits is copied into shared memory first,
+// weights, the gradient.  The first two are a warp's own, by its own largest
+// logit, so that the warps meet once.  A row that fits is copied into shared memory first,
 // each thread the groups that it will sweep, so that it comes from memory once
 // and three blocks an SM overlap their copies with the others' sweeps (2,048 x
 // 32,001 bfloat16: 87 us with the row in registers and two blocks); a larger one
 // is read in every sweep, the last two times out of L2.
-template <int Threads, bool Maximum>
-__device__ __forceinline__ float block_of(float v, float* shared) {
-    v = Maximum ? warp_max(v) : warp_sum(v);
-    if ((threadIdx.x & 31u) == 0) shared[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = threadIdx.x % 32 < Threads / 32 ? shared[threadIdx.x % 32] : Maximum ? -CUDART_INF_F : 0.0f;
-    return Maximum ? warp_max(v) : warp_sum(v);
-}
-
 template <typename T, int Threads, bool Held>
 __global__ void __launch_bounds__(Threads, Held ? 3 : 2) wide_loss_kernel(const __grid_constant__ LossArgs a) {
     extern __shared__ __align__(16) unsigned char dynamic[];
@@ -956,21 +953,26 @@ __global__ void __launch_bounds__(Threads, Held ? 3 : 2) wide_loss_kernel(const 
                 if (ok >> i & 1u) top = fmaxf(top, e[i]);
         }
     });
-    const RowScale by(block_of<Threads, true>(top, shared[0]));
+    const RowScale here(warp_max(top));  // this warp's
     Pair32 sums = 0;
     each([&](const Eight<T>& e, int32_t v) {
         const uint32_t ok = counts_at(v);
         if (ok == 0xffu) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sums = add2(sums, by.weight(e.pair(i)));
+            for (int i = 0; i < 4; ++i) sums = add2(sums, here.weight(e.pair(i)));
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (ok >> i & 1u) sums = add2(sums, pair_of(by.weight(e[i]), 0.0f));
+                if (ok >> i & 1u) sums = add2(sums, pair_of(here.weight(e[i]), 0.0f));
         }
     });
     const float2 halves = parts(sums);
-    const float sum = block_of<Threads, false>(halves.x + halves.y, shared[1]);
+    const float mine = warp_sum(halves.x + halves.y);
+    if ((threadIdx.x & 31u) == 0) shared[0][threadIdx.x >> 5] = here.top, shared[1][threadIdx.x >> 5] = mine;
+    __syncthreads();
+    const bool warp_of = threadIdx.x % 32 < Threads / 32;
+    const RowScale part(warp_of ? shared[0][threadIdx.x % 32] : -CUDART_INF_F), by(warp_max(part.top));
+    const float sum = warp_sum(warp_of ? shared[1][threadIdx.x % 32] * by.of(part) : 0.0f);
     const float gain = sum == 0.0f ? 0.0f : scale / sum;
     each([&](const Eight<T>& e, int32_t v) {
         const uint32_t ok = counts_at(v);
