@@ -385,7 +385,8 @@ struct Columns {
         }
         return q;
     }
-    // A thread's channels of a row in global memory, as they lie there; `row` at its first channel.
+    // A thread's channels of a row in global memory, as they lie there; `row` at its first
+    // channel.  Loaded to stay in L2, for it will be read again.
     template <typename E>
     struct Rows {
         alignas(16) uint32_t words[sizeof(E) == 4 || Unit == 1 ? 4 : 2];
@@ -398,13 +399,13 @@ struct Columns {
             if (in(u)) {
                 if constexpr (Unit == 1) {
                     if constexpr (sizeof(E) == 4)
-                        r.words[u] = __ldcs(reinterpret_cast<const uint32_t*>(row + step(u)));
+                        r.words[u] = __ldg(reinterpret_cast<const uint32_t*>(row + step(u)));
                     else
-                        r.words[u] = __ldcs(reinterpret_cast<const unsigned short*>(row + step(u)));
+                        r.words[u] = __ldg(reinterpret_cast<const unsigned short*>(row + step(u)));
                 } else {
                     using Raw = typename Packed<E, Unit>::Raw;
                     *reinterpret_cast<Raw*>(r.words + u * (Unit * sizeof(E) / 4)) =
-                        __ldcs(reinterpret_cast<const Raw*>(row + step(u)));
+                        __ldg(reinterpret_cast<const Raw*>(row + step(u)));
                 }
             }
         return r;
@@ -1101,56 +1102,84 @@ __global__ void __launch_bounds__(16 * kSegments) scan_map_kernel(const __grid_c
     a.scratch.slots[(size_t)tile.tile * a.channels + c] = (Slot)__float_as_uint(sum) << 32 | low;
 }
 
-// The states after all tiles out of their maps: a lane a channel, a warp a run
-// of tiles, composed first and then walked from the state before it.
+// The states after all tiles out of their maps: a lane a run of tiles of a
+// channel, its maps composed first and then walked from the state before it.  The
+// time is that of the trips to memory, so runs are short, and the first eight
+// maps are read at once and kept.
+constexpr uint32_t kJoinChannels = 8, kJoinRuns = 4;  // of a warp
 template <bool Backward>
 __global__ void __launch_bounds__(1024) scan_join_kernel(const __grid_constant__ ScanArgs a) {
-    __shared__ float products[32][33], values[32][33];
-    __shared__ uint32_t cuts[32][33];
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
-    const uint32_t run = (a.tiles + 31) / 32, begin = min(warp * run, a.tiles), end = min(begin + run, a.tiles);
-    const bool active = c < a.channels;
+    struct Map {
+        float A = 1.0f, H = 0.0f;
+        bool cut = false;  // a story starts inside: H is the state after it
+        __device__ __forceinline__ void then(Slot s) {
+            const float value = __uint_as_float((uint32_t)(s >> 32)), product = __uint_as_float((uint32_t)s);
+            const bool here = (uint32_t)s == kNone;
+            H = here ? value : fmaf(product, H, value);
+            A *= product;
+            cut |= here;
+        }
+        __device__ __forceinline__ float of(float state) const { return cut ? H : fmaf(A, state, H); }
+    };
+    __shared__ float products[32][kJoinChannels], values[32][kJoinChannels];
+    __shared__ bool cuts[32][kJoinChannels];
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, k = lane % kJoinChannels, sub = lane / kJoinChannels;
+    const uint32_t c = blockIdx.x * kJoinChannels + k, runs = 32 * kJoinRuns;
+    const uint32_t run = (a.tiles + runs - 1) / runs, begin = min((warp * kJoinRuns + sub) * run, a.tiles);
+    const uint32_t end = c < a.channels ? min(begin + run, a.tiles) : begin;
     const auto slot = [&](uint32_t i) {
         return a.scratch.slots + (size_t)(Backward ? a.tiles - 1 - i : i) * a.channels + c;
     };
-    float A = 1.0f, H = 0.0f;
-    bool cut = false;
-    if (active)
-        for (uint32_t from = begin; from < end; from += 8) {
-            Slot s[8];
+    const auto read = [&](uint32_t from, Slot (&s)[8]) {
 #pragma unroll
-            for (uint32_t j = 0; j < 8; ++j)
-                if (from + j < end) s[j] = *slot(from + j);
+        for (uint32_t j = 0; j < 8; ++j)
+            if (from + j < end) s[j] = *slot(from + j);
+    };
+    Slot held[8], more[8];
+    read(begin, held);
+    Map mine;
 #pragma unroll
-            for (uint32_t j = 0; j < 8; ++j)
-                if (from + j < end) {
-                    const float value = __uint_as_float((uint32_t)(s[j] >> 32));
-                    const float product = __uint_as_float((uint32_t)s[j]);
-                    const bool here = (uint32_t)s[j] == kNone;
-                    H = here ? value : fmaf(product, H, value);
-                    A *= product;
-                    cut |= here;
-                }
-        }
-    products[warp][lane] = A, values[warp][lane] = H, cuts[warp][lane] = cut;
+    for (uint32_t j = 0; j < 8; ++j)
+        if (begin + j < end) mine.then(held[j]);
+    for (uint32_t from = begin + 8; from < end; from += 8) {
+        read(from, more);
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j)
+            if (from + j < end) mine.then(more[j]);
+    }
+    // The maps of the warp's runs before this one, and of all of them.
+    Map before, all;
+#pragma unroll
+    for (uint32_t r = 0; r < kJoinRuns; ++r) {
+        const uint32_t from = r * kJoinChannels + k;
+        const float A = __shfl_sync(kNone, mine.A, from), H = __shfl_sync(kNone, mine.H, from);
+        const bool cut = __shfl_sync(kNone, mine.cut, from);
+        if (r == sub) before = all;
+        all.H = cut ? H : fmaf(A, all.H, H);
+        all.A *= A;
+        all.cut |= cut;
+    }
+    if (sub == 0) products[warp][k] = all.A, values[warp][k] = all.H, cuts[warp][k] = all.cut;
     __syncthreads();
     float state = 0.0f;
-    for (uint32_t w = 0; w < warp; ++w)
-        state = cuts[w][lane] ? values[w][lane] : fmaf(products[w][lane], state, values[w][lane]);
-    if (active)
-        for (uint32_t from = begin; from < end; from += 8) {
-            Slot s[8];  // read together, before the first of them is written
+#pragma unroll 4
+    for (uint32_t w = 0; w < warp; ++w) state = cuts[w][k] ? values[w][k] : fmaf(products[w][k], state, values[w][k]);
+    if (sub) state = before.of(state);
+    const auto walk = [&](uint32_t from, const Slot (&s)[8]) {
 #pragma unroll
-            for (uint32_t j = 0; j < 8; ++j)
-                if (from + j < end) s[j] = *slot(from + j);
-#pragma unroll
-            for (uint32_t j = 0; j < 8; ++j)
-                if (from + j < end) {
-                    const float value = __uint_as_float((uint32_t)(s[j] >> 32));
-                    state = (uint32_t)s[j] == kNone ? value : fmaf(__uint_as_float((uint32_t)s[j]), state, value);
-                    *slot(from + j) = (Slot)__float_as_uint(state) << 32;
-                }
-        }
+        for (uint32_t j = 0; j < 8; ++j)
+            if (from + j < end) {
+                Map m;
+                m.then(s[j]);
+                state = m.of(state);
+                *slot(from + j) = (Slot)__float_as_uint(state) << 32;
+            }
+    };
+    walk(begin, held);
+    for (uint32_t from = begin + 8; from < end; from += 8) {
+        read(from, more);
+        walk(from, more);
+    }
     if (blockIdx.x == 0 && threadIdx.x == 0) *a.scratch.ticket = kNone;  // the next one is 0
 }
 
@@ -1421,7 +1450,7 @@ void launch_scan(ScanArgs& a, void* workspace, size_t workspace_bytes, cudaStrea
         scan_map_kernel<T, G, Unit, Shared, Backward, S::kSegment>
             <<<(uint32_t)total, 16 * kSegments, 0, stream>>>(a);
         check(cudaGetLastError(), "scan_map_kernel");
-        scan_join_kernel<Backward><<<(a.channels + 31) / 32, 1024, 0, stream>>>(a);
+        scan_join_kernel<Backward><<<(a.channels + kJoinChannels - 1) / kJoinChannels, 1024, 0, stream>>>(a);
         check(cudaGetLastError(), "scan_join_kernel");
     } else if (a.tiles > 1) {
         check(cudaMemsetAsync(workspace, 0xff, 256 + (size_t)a.tiles * a.channels * sizeof(Slot), stream), "clear scan slots");
