@@ -106,7 +106,6 @@ struct ScanArgs {
     CUtensorMap drive_map, decay_map, grad_map;  // of the tiled loads
     LeoB200StoryTables tables;
     const LeoB200StoryTile* schedule;  // the tiles in the order of their tickets
-    bool ready;                        // the slots hold the states after the tiles before the launch
     uint32_t channels, tiles, groups;  // groups: of 64 channels
     const void* drive;
     int64_t drive_stride;
@@ -190,15 +189,10 @@ template <int Direction>
 struct Lookback {
     uint32_t from;  // tile whose slot is a state
     int maps;       // tiles between it and this one; -1: no story crosses in
-    __device__ __forceinline__ Lookback(uint32_t tile, uint32_t holder, bool ready) {
+    __device__ __forceinline__ Lookback(uint32_t tile, uint32_t holder) {
         maps = -1;
         from = holder;
         if (holder == tile) return;
-        if (ready) {
-            from = Direction > 0 ? tile - 1 : tile + 1;
-            maps = 0;
-            return;
-        }
         // A state is published by the last tile of a group of kGroup in the direction of the scan.
         if (Direction > 0) {
             const uint32_t p = tile / kGroup * kGroup;
@@ -834,7 +828,7 @@ __global__ void __launch_bounds__(Shape<T, G, Shared, Backward>::kThreads, 1) sc
             drawn = draw();
             const uint32_t c = work.group * kColumns + k;
             const bool active = c < a.channels;
-            const Lookback<Direction> back(work.tile, work.holder, a.ready);
+            const Lookback<Direction> back(work.tile, work.holder);
             Slot slots[8];
             if (back.maps >= 0 && active) back.load(a.scratch.slots, a.channels, c, (int)half, slots);
             float kept = 0.0f;
@@ -955,7 +949,7 @@ __global__ void __launch_bounds__(Shape<T, G, Shared, Backward>::kThreads, 1) sc
             const float tile_A = value_of(product_of(product, other));
             const float tile_sum = far_cut ? far_sum : fmaf(far_A, near_sum, far_sum);
             const bool state_tile = Backward ? tile % kGroup == 0 : (tile + 1) % kGroup == 0;
-            const bool writes = active && work.onward && half == 0 && !a.ready;
+            const bool writes = active && work.onward && half == 0;
             Slot* mine = a.scratch.slots + (size_t)tile * a.channels + c;
             if (writes && (cuts || !state_tile)) write_slot(mine, tile_A, tile_sum);
 
@@ -1031,8 +1025,9 @@ __global__ void __launch_bounds__(Shape<T, G, Shared, Backward>::kThreads, 1) sc
 // inputs once more.
 
 // The map of a tile, the work divided as above, every row read at once.
-template <typename T, typename G, int Unit, bool Shared, bool Backward, int Length>
+template <typename T, typename G, int Unit, bool Shared, bool Backward>
 __global__ void __launch_bounds__(16 * kSegments) scan_map_kernel(const __grid_constant__ ScanArgs a) {
+    constexpr int Length = LEO_B200_TILE_TOKENS / kSegments;
     __shared__ float2 products[kSegments][kColumns];
     __shared__ float values[kSegments][kColumns];
     __shared__ uint32_t cuts[kSegments];
@@ -1180,7 +1175,172 @@ __global__ void __launch_bounds__(1024) scan_join_kernel(const __grid_constant__
         read(from, more);
         walk(from, more);
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) *a.scratch.ticket = kNone;  // the next one is 0
+}
+
+// The tiles themselves, the state before each in the slot of the tile before it.
+// Nothing is waited for, so a block a tile keeps its tokens in registers and
+// the SM's blocks hide one another's loads.
+template <typename T, typename G, int Unit, bool Shared, bool Backward>
+__global__ void __launch_bounds__(16 * kSegments, 2) scan_tile_kernel(const __grid_constant__ ScanArgs a) {
+    constexpr int Length = LEO_B200_TILE_TOKENS / kSegments;
+    __shared__ __align__(16) float products[kSegments][kColumns];
+    __shared__ __align__(16) float states[kSegments][kColumns];                     // of a segment from zero, then before it
+    __shared__ __align__(16) float values[Backward ? kSegments : 1][kColumns];  // the same from the right
+    __shared__ bool starts[kSegments], ends[kSegments];
+    const uint32_t place = blockIdx.x / a.groups, group = blockIdx.x - place * a.groups;
+    const LeoB200StoryTile tile = a.schedule[place];
+    const uint32_t segment = threadIdx.x >> 4, first = tile.first + segment * Length;
+    const int count = max(min((int)tile.count - (int)segment * Length, Length), 0);
+    const Columns<Unit> col(group, a.channels);
+    typename Columns<Unit>::template Rows<T> xs[Length], ss[Backward ? Length : 1];
+    typename Columns<Unit>::template Rows<G> gs[Shared ? 1 : Length];
+    {
+        const T* x = static_cast<const T*>(a.drive) + (int64_t)first * a.drive_stride + col.c;
+        const T* s = static_cast<const T*>(a.grad_states) + (Backward ? (int64_t)first * a.grad_states_stride + col.c : 0);
+        const G* g = static_cast<const G*>(a.decay) + (Shared ? 0 : (int64_t)first * a.decay_stride) + col.c;
+#pragma unroll
+        for (int j = 0; j < Length; ++j)
+            if (j < count) {
+                xs[j] = col.read(x + j * a.drive_stride);
+                if constexpr (Backward) ss[j] = col.read(s + j * a.grad_states_stride);
+                if constexpr (!Shared) gs[j] = col.read(g + j * a.decay_stride);
+            }
+    }
+    // Of the threads that join the segments, a channel each: 64 from the left, and 64 more from the right.
+    const uint32_t k = threadIdx.x % kColumns, c = group * kColumns + k, side = threadIdx.x / kColumns;
+    const bool joins = side < (Backward ? 2 : 1), leftward = Backward && side == 0;
+    float before = 0.0f;
+    if (joins && c < a.channels) {
+        if (Backward && !leftward)
+            before = a.carries[(size_t)tile.kept * a.channels + c];
+        else if (tile.holder != tile.tile)
+            before = __uint_as_float((uint32_t)(
+                a.scratch.slots[(size_t)(Backward ? tile.tile + 1 : tile.tile - 1) * a.channels + c] >> 32));
+    }
+    const StoryBits bits = count ? story_bits(a.tables, first) : StoryBits{};
+    const Segment s = segment_of(bits, first, count);
+    Quad h, n, gate;
+    Product4 product;
+    if constexpr (Shared) gate = col.get_row(static_cast<const G*>(a.decay));
+#pragma unroll
+    for (int j = 0; j < Length; ++j)
+        if (j < count) {
+            if (s.starts >> j & 1u) h = col.get_row(a.initial, story_starting(a.tables, s, j));
+            if constexpr (!Shared) gate = col.unpack(gs[j]);
+            const Quad v = col.unpack(xs[j]);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) h.v[q] = fma2(gate.v[q], h.v[q], v.v[q]);
+            product.times(gate);
+        }
+    if constexpr (Backward) {
+#pragma unroll
+        for (int j = Length - 1; j >= 0; --j)
+            if (j < count) {
+                if (s.ends >> j & 1u) n = col.get_row(a.grad_final, story_ending(a.tables, s, j));
+                if constexpr (!Shared) gate = col.unpack(gs[j]);
+                const Quad v = col.unpack(ss[j]);
+#pragma unroll
+                for (int q = 0; q < 2; ++q) n.v[q] = mul2(gate.v[q], add2(v.v[q], n.v[q]));
+            }
+        col.put_shared(values[segment], n);
+    }
+    col.put_shared(states[segment], h);
+    Quad A;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const float2 hi = parts(product.hi[q]), lo = parts(product.lo[q]);
+        A.v[q] = pair_of(value_of(make_float2(hi.x, lo.x)), value_of(make_float2(hi.y, lo.y)));
+    }
+    col.put_shared(products[segment], A);
+    if ((threadIdx.x & 15u) == 0) starts[segment] = s.starts != 0, ends[segment] = s.ends != 0;
+    __syncthreads();
+    if (joins && !leftward) {
+#pragma unroll
+        for (int w = 0; w < kSegments; ++w) {
+            const float v = states[w][k];
+            states[w][k] = before;
+            if constexpr (!Backward)
+                if (a.carries && c < a.channels && w % (kKept / Length) == 0 && (uint32_t)w * Length < tile.count)
+                    a.carries[(size_t)(tile.kept + w / (kKept / Length)) * a.channels + c] = before;
+            before = starts[w] ? v : fmaf(products[w][k], before, v);
+        }
+    } else if (joins) {
+#pragma unroll
+        for (int w = kSegments - 1; w >= 0; --w) {
+            const float v = values[Backward ? w : 0][k];
+            values[Backward ? w : 0][k] = before;
+            before = ends[w] ? v : fmaf(products[w][k], before, v);
+        }
+    }
+    __syncthreads();
+    const size_t row = (size_t)first * a.channels + col.c;
+    h = col.get_shared(states[segment]);
+    if constexpr (!Backward) {
+        T* out = static_cast<T*>(a.states) + row;
+#pragma unroll
+        for (int j = 0; j < Length; ++j)
+            if (j < count) {
+                if (s.starts >> j & 1u) h = col.get_row(a.initial, story_starting(a.tables, s, j));
+                if constexpr (!Shared) gate = col.unpack(gs[j]);
+                const Quad v = col.unpack(xs[j]);
+#pragma unroll
+                for (int q = 0; q < 2; ++q) h.v[q] = fma2(gate.v[q], h.v[q], v.v[q]);
+                col.put(out + (size_t)j * a.channels, h);
+                if (s.ends >> j & 1u) col.put_row(a.final_states, story_ending(a.tables, s, j), h);
+            }
+    } else {
+        // The state before each token, then the slopes from the right.
+        Quad previous[Length];
+#pragma unroll
+        for (int j = 0; j < Length; ++j)
+            if (j < count) {
+                if (s.starts >> j & 1u) h = col.get_row(a.initial, story_starting(a.tables, s, j));
+                if constexpr (!Shared) gate = col.unpack(gs[j]);
+                previous[j] = h;
+                const Quad v = col.unpack(xs[j]);
+#pragma unroll
+                for (int q = 0; q < 2; ++q) h.v[q] = fma2(gate.v[q], h.v[q], v.v[q]);
+            }
+        n = col.get_shared(values[segment]);
+        Quad sum;
+        T* out = static_cast<T*>(a.grad_drive) + row;
+        G* out_gate = static_cast<G*>(a.grad_decay) + (Shared ? 0 : row);
+#pragma unroll
+        for (int j = Length - 1; j >= 0; --j)
+            if (j < count) {
+                if (s.ends >> j & 1u) n = col.get_row(a.grad_final, story_ending(a.tables, s, j));
+                if constexpr (!Shared) gate = col.unpack(gs[j]);
+                const Quad v = col.unpack(ss[j]);
+                Quad slope, term;
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    slope.v[q] = add2(v.v[q], n.v[q]);
+                    term.v[q] = mul2(slope.v[q], previous[j].v[q]);
+                    n.v[q] = mul2(gate.v[q], slope.v[q]);
+                    if constexpr (Shared) sum.v[q] = add2(sum.v[q], term.v[q]);
+                }
+                col.put(out + (size_t)j * a.channels, slope);
+                if constexpr (!Shared) col.put(out_gate + (size_t)j * a.channels, term);
+                if (a.grad_initial && (s.starts >> j & 1u))
+                    col.put_row(a.grad_initial, story_starting(a.tables, s, j), n);
+            }
+        if constexpr (Shared) {
+            col.put_shared(states[segment], sum);  // only these threads' columns, which they have read
+            __syncthreads();
+            if (threadIdx.x < kColumns && c < a.channels) {
+                float total = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kSegments; ++w) total += states[w][k];
+                a.scratch.partials[(size_t)tile.tile * a.channels + c] = total;
+            }
+        }
+    }
+    if (tile.tile == 0 && a.tables.full < a.tables.stories && side == 0) {
+        if constexpr (!Backward)
+            copy_empty(a.tables, a.channels, c, a.initial, a.final_states);
+        else if (a.grad_initial)
+            copy_empty(a.tables, a.channels, c, a.grad_final, a.grad_initial);
+    }
 }
 
 // The gradient of a shared row of gates: the tiles' sums in double, a column of
@@ -1432,6 +1592,20 @@ void launch_scan(ScanArgs& a, void* workspace, size_t workspace_bytes, cudaStrea
         require(workspace != nullptr && workspace_bytes >= size, "the workspace is too small");
         require(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "the workspace must be aligned to 16 bytes");
     }
+    // Whole tiles that may be worked on side by side without waiting for one another, of those in the longest row.
+    const uint64_t whole = (uint64_t)a.tables.tiles[0] * a.groups;
+    if (a.tables.longest[0] > kGroup && whole / a.tables.longest[0] < kAbreast[Backward]) {
+        a.tiles = a.tables.tiles[0];
+        a.schedule = a.tables.schedule[0][Backward];
+        constexpr uint32_t threads = 16 * kSegments;
+        scan_map_kernel<T, G, Unit, Shared, Backward><<<(uint32_t)whole, threads, 0, stream>>>(a);
+        check(cudaGetLastError(), "scan_map_kernel");
+        scan_join_kernel<Backward><<<(a.channels + kJoinChannels - 1) / kJoinChannels, 1024, 0, stream>>>(a);
+        check(cudaGetLastError(), "scan_join_kernel");
+        scan_tile_kernel<T, G, Unit, Shared, Backward><<<(uint32_t)whole, threads, 0, stream>>>(a);
+        check(cudaGetLastError(), "scan_tile_kernel");
+        return;
+    }
     const int sms = sm_count();
     const auto kernel = scan_kernel<T, G, Unit, Shared, Backward>;
     static std::atomic<uint64_t> allowed{0};
@@ -1443,16 +1617,7 @@ void launch_scan(ScanArgs& a, void* workspace, size_t workspace_bytes, cudaStrea
         if constexpr (Backward)
             describe<T>(&a.grad_map, a.grad_states, a.grad_states_stride, a.tables.tokens, a.channels, rows);
     }
-    // Tiles that may be worked on side by side without waiting for one another, of those in the longest row.
-    const uint64_t abreast = total / a.tables.longest[halves];
-    a.ready = a.tables.longest[halves] > kGroup && abreast < kAbreast[Backward];
-    if (a.ready) {
-        scan_map_kernel<T, G, Unit, Shared, Backward, S::kSegment>
-            <<<(uint32_t)total, 16 * kSegments, 0, stream>>>(a);
-        check(cudaGetLastError(), "scan_map_kernel");
-        scan_join_kernel<Backward><<<(a.channels + kJoinChannels - 1) / kJoinChannels, 1024, 0, stream>>>(a);
-        check(cudaGetLastError(), "scan_join_kernel");
-    } else if (a.tiles > 1) {
+    if (a.tiles > 1) {
         check(cudaMemsetAsync(workspace, 0xff, 256 + (size_t)a.tiles * a.channels * sizeof(Slot), stream), "clear scan slots");
     }
     const uint32_t blocks = a.tiles == 1 || total <= 2u * (uint32_t)sms ? (uint32_t)total : (uint32_t)sms;
@@ -1470,10 +1635,10 @@ void dispatch_shape(int unit, bool shared, Body&& body) {
 }
 
 // Tiled loads and rows of neighbours need every tensor of the call to allow
-// them; a stride of zero has no tiled form.
+// them; rows that overlap have no tiled form.
 int unit_of_call(uint32_t channels, uint32_t tokens, int64_t stride0, int64_t stride1, int64_t stride2, int least) {
     int unit = std::min(least, channels % 4 == 0 ? 4 : channels % 2 == 0 ? 2 : 1);
-    const bool strided = stride0 > 0 && stride1 > 0 && stride2 > 0;
+    const bool strided = stride0 >= channels && stride1 >= channels && stride2 >= channels;
     if (unit == 4 && (!strided || tokens == 0)) unit = 2;
     return unit;
 }
@@ -1605,7 +1770,7 @@ int leo_b200_gated_scan(int device, const LeoB200StoryTables* tables, uint32_t c
             const bool shared = decay_shared != 0 && tables->tokens > 0;
             int unit = std::min(unit_of(drive, drive_stride, sizeof(T)), unit_of(states, channels, sizeof(T)));
             if (!shared) unit = std::min(unit, unit_of(decay, decay_stride, sizeof(G)));
-            unit = unit_of_call(channels, tables->tokens, drive_stride, shared ? 1 : decay_stride, 1, unit);
+            unit = unit_of_call(channels, tables->tokens, drive_stride, shared ? channels : decay_stride, channels, unit);
             DeviceScope scope(device);
             dispatch_shape(unit, shared, [&](auto u, auto is_shared) {
                 launch_scan<T, G, u(), is_shared(), false>(a, workspace, workspace_bytes, (cudaStream_t)stream);
@@ -1649,7 +1814,7 @@ int leo_b200_gated_scan_backward(int device, const LeoB200StoryTables* tables, u
             unit = std::min(unit, unit_of(grad_drive, channels, sizeof(T)));
             if (!shared)
                 unit = std::min({unit, unit_of(decay, decay_stride, sizeof(G)), unit_of(grad_decay, channels, sizeof(G))});
-            unit = unit_of_call(channels, tables->tokens, drive_stride, shared ? 1 : decay_stride, grad_states_stride, unit);
+            unit = unit_of_call(channels, tables->tokens, drive_stride, shared ? channels : decay_stride, grad_states_stride, unit);
             DeviceScope scope(device);
             dispatch_shape(unit, shared, [&](auto u, auto is_shared) {
                 launch_scan<T, G, u(), is_shared(), true>(a, workspace, workspace_bytes, (cudaStream_t)stream);
