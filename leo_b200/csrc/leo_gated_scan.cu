@@ -8,28 +8,39 @@
 // h -> A h + H (A the product of the gates, H the state from zero), or as
 // h -> H if a story starts inside, and such maps compose.  The batch is cut into
 // tiles of 128 tokens or fewer (leo_b200_story_table): a block takes a tile of
-// 64 channels, each thread a segment of 8 tokens of four channels.  The
-// segments' maps give the tile's, the tiles' maps the state before a tile, and
-// each thread then runs its tokens again and writes them.  The backward pass is
-// the same from the right, with m -> A m + M for m[t] = a[t] slope[t]; h is
-// formed anew from the states that the forward pass keeps every 64 tokens.
+// 64 channels, each thread a segment of 8 tokens of four channels (4 tokens in
+// tiles of 64, where a stage of 128 would not fit).  The segments' maps give the
+// tile's, the tiles' maps the state before a tile, and each thread then runs its
+// tokens again and writes them.  The backward pass is the same from the right,
+// with m -> A m + M for m[t] = a[t] slope[t]; h is formed anew from the states
+// that the forward pass keeps every 64 tokens.
 //
-// Pipeline.  One block an SM works through tiles dealt by a ticket.  While the
-// loads of tile i + 2 are in flight into its own third of shared memory (each
-// warp loads what it will use itself, so they need no barrier), eight warps map
-// tile i + 1 and write tile i, and four more compose tile i + 1.  Every input
-// is read once and the loads never pause.
+// Pipeline.  One block an SM works through tiles dealt by a ticket, every input
+// read once.  Two teams of eight warps take tiles in turn: a team loads the tile
+// after its next into shared memory (tiled loads where rows keep 16 bytes, each
+// warp what it will use itself, so they need no barrier), maps its tile and
+// writes it, and the other team's work fills its waits.  Four warps compose a
+// tile's segments; four more scout, that is they do all the reading between
+// tiles (slots, kept states, tickets, the schedule), since a warp with a load in
+// flight waits for it with every read of shared memory.  Where four stages do
+// not fit, one team with three maps tile i + 1 between the map and the writing
+// of tile i.  81,920 tokens x 1,024 channels (bfloat16, float gates) in 64 stories:
+// 141 us with one team and 129 us with two, 103 us at the rate of a copy; 20,480
+// x 4,096 in 32 stories 141 and 264 us backward, 103 and 180 us at that rate.  A
+// loop of the same loads and stores alone runs at a copy's rate, so the rest is
+// the length of a tile's chain, from its loads to its map, the composing and the writes.
 //
 // Between tiles.  Each tile publishes its map, every kGroup-th the state after
 // it instead, so a tile reads at most kGroup slots.  A slot and its mark are one
 // 8-byte word, so a slot that is there costs one trip to L2.  Tickets deal the
 // first tiles of all stories, then their second ones, and so on: a tile's
 // predecessors have lower tickets, so they have started before it and every wait
-// ends, and with many stories they are long done when it reads them.  Tiles in
+// ends, and with many stories they are long done when it reads them.  (Tiles in
 // the order of their tokens wait for neighbours that are mapped in the same
-// moment: 81,920 tokens x 1,024 channels of 64 stories took 236 us that way,
-// 127 us without any wait.  Which slots are read, and in which order they are
-// composed, depends on the layout alone: results are the same in every run.
+// moment, which took a quarter longer.)  Which slots are read, and in which
+// order they are composed, depends on the layout alone: results are the same in
+// every run.  Where a single long story leaves too few tiles side by side, the
+// maps are found in a pass of their own (scan_map_kernel and on).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -61,10 +72,12 @@ constexpr uint32_t kNone = 0xffffffffu;
 constexpr size_t kSharedLimit = 227 * 1024;
 constexpr uint32_t kKept = LEO_B200_TILE_TOKENS / 2;  // tokens between the states kept for the backward pass
 constexpr int kGroup = 16;                       // tiles between published states
-// Fewer independent tiles than these are mapped in a pass of their own.  One story
-// of 65,536 tokens: 512 channels (8 abreast) forward 108 us so and 127 us in one
-// pass, backward 137 and 143 us; 1,024 channels (16) 184 and 207 us, 248 and 229 us.
-constexpr uint32_t kAbreast[2] = {20, 12};  // forward, backward
+// Where fewer tiles than this can be worked on without waiting for one another
+// (the stories' channel groups), they are mapped ahead, which reads the inputs
+// twice.  One story of 65,536 tokens, bfloat16 with float gates, so and in one pass:
+// 64 channels forward 29 and 61 us, backward 35 and 68 us; 512 channels (8 abreast)
+// 121 and 135 us, 148 and 158 us; 1,024 channels (16) 213 and 211 us, 268 and 252 us.
+constexpr uint32_t kAbreast = 12;
 constexpr uint32_t kSpinLimit = 1u << 21;        // polls of a wait, a memory round trip and more apart
 
 __device__ uint32_t g_gave_up;
@@ -1019,10 +1032,21 @@ __global__ void __launch_bounds__(Shape<T, G, Shared, Backward>::kThreads, 1) sc
 
 // Few stories side by side: the tiles of one are then in the works at the same
 // time, and each would wait for its neighbours.  Their maps are found first, in
-// a pass over the inputs, and joined to the states after every tile; the pass
-// above then waits for nothing.  One document of 65,537 tokens x 257 channels
-// took 121 us forward and 278 us backward without these two, which read the
-// inputs once more.
+// a pass over the inputs, and joined to the states after every tile; then the
+// tiles are written by a block each, which reads the inputs once more and waits
+// for nothing.  One document of 65,537 tokens x 257 channels, float32 with one gate
+// a channel: 66 us forward and 92 us backward, 104 and 137 us in one pass (21 and 31 us
+// at the rate of a copy; rows of 257 are read and written an element at a time).
+
+// Calls body(true_type) for a segment that is whole and inside a story, as most
+// are: nothing is asked of its tokens there.  body(false_type) for the others.
+template <typename Body>
+__device__ __forceinline__ void with_plain(const Segment& s, int length, Body&& body) {
+    if (s.count == length && (s.starts | s.ends) == 0)
+        body(std::true_type{});
+    else
+        body(std::false_type{});
+}
 
 // The map of a tile, the work divided as above, every row read at once.
 template <typename T, typename G, int Unit, bool Shared, bool Backward>
@@ -1053,21 +1077,24 @@ __global__ void __launch_bounds__(16 * kSegments) scan_map_kernel(const __grid_c
     Quad value, gate;
     Product4 product;
     if constexpr (Shared) gate = col.get_row(static_cast<const G*>(a.decay));
+    with_plain(s, Length, [&](auto plain) {
+        constexpr bool kPlain = decltype(plain)::value;
 #pragma unroll
-    for (int k = 0; k < Length; ++k) {
-        const int j = Backward ? Length - 1 - k : k;
-        if (j < count) {
-            if (Backward ? s.ends >> j & 1u : s.starts >> j & 1u)
-                value = Backward ? col.get_row(a.grad_final, story_ending(a.tables, s, j))
-                                 : col.get_row(a.initial, story_starting(a.tables, s, j));
-            if constexpr (!Shared) gate = col.unpack(gs[j]);
-            const Quad v = col.unpack(xs[j]);
+        for (int k = 0; k < Length; ++k) {
+            const int j = Backward ? Length - 1 - k : k;
+            if (kPlain || j < count) {
+                if (!kPlain && ((Backward ? s.ends : s.starts) >> j & 1u))
+                    value = Backward ? col.get_row(a.grad_final, story_ending(a.tables, s, j))
+                                     : col.get_row(a.initial, story_starting(a.tables, s, j));
+                if constexpr (!Shared) gate = col.unpack(gs[j]);
+                const Quad v = col.unpack(xs[j]);
 #pragma unroll
-            for (int q = 0; q < 2; ++q)
-                value.v[q] = Backward ? mul2(gate.v[q], add2(v.v[q], value.v[q])) : fma2(gate.v[q], value.v[q], v.v[q]);
-            product.times(gate);
+                for (int q = 0; q < 2; ++q)
+                    value.v[q] = Backward ? mul2(gate.v[q], add2(v.v[q], value.v[q])) : fma2(gate.v[q], value.v[q], v.v[q]);
+                product.times(gate);
+            }
         }
-    }
+    });
     col.put_shared(values[segment], value);
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
@@ -1222,28 +1249,31 @@ __global__ void __launch_bounds__(16 * kSegments, 2) scan_tile_kernel(const __gr
     Quad h, n, gate;
     Product4 product;
     if constexpr (Shared) gate = col.get_row(static_cast<const G*>(a.decay));
+    with_plain(s, Length, [&](auto plain) {
+        constexpr bool kPlain = decltype(plain)::value;
 #pragma unroll
-    for (int j = 0; j < Length; ++j)
-        if (j < count) {
-            if (s.starts >> j & 1u) h = col.get_row(a.initial, story_starting(a.tables, s, j));
-            if constexpr (!Shared) gate = col.unpack(gs[j]);
-            const Quad v = col.unpack(xs[j]);
-#pragma unroll
-            for (int q = 0; q < 2; ++q) h.v[q] = fma2(gate.v[q], h.v[q], v.v[q]);
-            product.times(gate);
-        }
-    if constexpr (Backward) {
-#pragma unroll
-        for (int j = Length - 1; j >= 0; --j)
-            if (j < count) {
-                if (s.ends >> j & 1u) n = col.get_row(a.grad_final, story_ending(a.tables, s, j));
+        for (int j = 0; j < Length; ++j)
+            if (kPlain || j < count) {
+                if (!kPlain && (s.starts >> j & 1u)) h = col.get_row(a.initial, story_starting(a.tables, s, j));
                 if constexpr (!Shared) gate = col.unpack(gs[j]);
-                const Quad v = col.unpack(ss[j]);
+                const Quad v = col.unpack(xs[j]);
 #pragma unroll
-                for (int q = 0; q < 2; ++q) n.v[q] = mul2(gate.v[q], add2(v.v[q], n.v[q]));
+                for (int q = 0; q < 2; ++q) h.v[q] = fma2(gate.v[q], h.v[q], v.v[q]);
+                product.times(gate);
             }
-        col.put_shared(values[segment], n);
-    }
+        if constexpr (Backward) {
+#pragma unroll
+            for (int j = Length - 1; j >= 0; --j)
+                if (kPlain || j < count) {
+                    if (!kPlain && (s.ends >> j & 1u)) n = col.get_row(a.grad_final, story_ending(a.tables, s, j));
+                    if constexpr (!Shared) gate = col.unpack(gs[j]);
+                    const Quad v = col.unpack(ss[j]);
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) n.v[q] = mul2(gate.v[q], add2(v.v[q], n.v[q]));
+                }
+        }
+    });
+    if constexpr (Backward) col.put_shared(values[segment], n);
     col.put_shared(states[segment], h);
     Quad A;
 #pragma unroll
@@ -1275,64 +1305,68 @@ __global__ void __launch_bounds__(16 * kSegments, 2) scan_tile_kernel(const __gr
     __syncthreads();
     const size_t row = (size_t)first * a.channels + col.c;
     h = col.get_shared(states[segment]);
-    if constexpr (!Backward) {
-        T* out = static_cast<T*>(a.states) + row;
+    Quad sum;
+    with_plain(s, Length, [&](auto plain) {
+        constexpr bool kPlain = decltype(plain)::value;
+        if constexpr (!Backward) {
+            T* out = static_cast<T*>(a.states) + row;
 #pragma unroll
-        for (int j = 0; j < Length; ++j)
-            if (j < count) {
-                if (s.starts >> j & 1u) h = col.get_row(a.initial, story_starting(a.tables, s, j));
-                if constexpr (!Shared) gate = col.unpack(gs[j]);
-                const Quad v = col.unpack(xs[j]);
+            for (int j = 0; j < Length; ++j)
+                if (kPlain || j < count) {
+                    if (!kPlain && (s.starts >> j & 1u)) h = col.get_row(a.initial, story_starting(a.tables, s, j));
+                    if constexpr (!Shared) gate = col.unpack(gs[j]);
+                    const Quad v = col.unpack(xs[j]);
 #pragma unroll
-                for (int q = 0; q < 2; ++q) h.v[q] = fma2(gate.v[q], h.v[q], v.v[q]);
-                col.put(out + (size_t)j * a.channels, h);
-                if (s.ends >> j & 1u) col.put_row(a.final_states, story_ending(a.tables, s, j), h);
-            }
-    } else {
-        // The state before each token, then the slopes from the right.
-        Quad previous[Length];
-#pragma unroll
-        for (int j = 0; j < Length; ++j)
-            if (j < count) {
-                if (s.starts >> j & 1u) h = col.get_row(a.initial, story_starting(a.tables, s, j));
-                if constexpr (!Shared) gate = col.unpack(gs[j]);
-                previous[j] = h;
-                const Quad v = col.unpack(xs[j]);
-#pragma unroll
-                for (int q = 0; q < 2; ++q) h.v[q] = fma2(gate.v[q], h.v[q], v.v[q]);
-            }
-        n = col.get_shared(values[segment]);
-        Quad sum;
-        T* out = static_cast<T*>(a.grad_drive) + row;
-        G* out_gate = static_cast<G*>(a.grad_decay) + (Shared ? 0 : row);
-#pragma unroll
-        for (int j = Length - 1; j >= 0; --j)
-            if (j < count) {
-                if (s.ends >> j & 1u) n = col.get_row(a.grad_final, story_ending(a.tables, s, j));
-                if constexpr (!Shared) gate = col.unpack(gs[j]);
-                const Quad v = col.unpack(ss[j]);
-                Quad slope, term;
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    slope.v[q] = add2(v.v[q], n.v[q]);
-                    term.v[q] = mul2(slope.v[q], previous[j].v[q]);
-                    n.v[q] = mul2(gate.v[q], slope.v[q]);
-                    if constexpr (Shared) sum.v[q] = add2(sum.v[q], term.v[q]);
+                    for (int q = 0; q < 2; ++q) h.v[q] = fma2(gate.v[q], h.v[q], v.v[q]);
+                    col.put(out + (size_t)j * a.channels, h);
+                    if (!kPlain && (s.ends >> j & 1u)) col.put_row(a.final_states, story_ending(a.tables, s, j), h);
                 }
-                col.put(out + (size_t)j * a.channels, slope);
-                if constexpr (!Shared) col.put(out_gate + (size_t)j * a.channels, term);
-                if (a.grad_initial && (s.starts >> j & 1u))
-                    col.put_row(a.grad_initial, story_starting(a.tables, s, j), n);
-            }
-        if constexpr (Shared) {
-            col.put_shared(states[segment], sum);  // only these threads' columns, which they have read
-            __syncthreads();
-            if (threadIdx.x < kColumns && c < a.channels) {
-                float total = 0.0f;
+        } else {
+            // The state before each token, then the slopes from the right.
+            Quad previous[Length];
 #pragma unroll
-                for (int w = 0; w < kSegments; ++w) total += states[w][k];
-                a.scratch.partials[(size_t)tile.tile * a.channels + c] = total;
-            }
+            for (int j = 0; j < Length; ++j)
+                if (kPlain || j < count) {
+                    if (!kPlain && (s.starts >> j & 1u)) h = col.get_row(a.initial, story_starting(a.tables, s, j));
+                    if constexpr (!Shared) gate = col.unpack(gs[j]);
+                    previous[j] = h;
+                    const Quad v = col.unpack(xs[j]);
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) h.v[q] = fma2(gate.v[q], h.v[q], v.v[q]);
+                }
+            n = col.get_shared(values[segment]);
+            T* out = static_cast<T*>(a.grad_drive) + row;
+            G* out_gate = static_cast<G*>(a.grad_decay) + (Shared ? 0 : row);
+            (void)out_gate;
+#pragma unroll
+            for (int j = Length - 1; j >= 0; --j)
+                if (kPlain || j < count) {
+                    if (!kPlain && (s.ends >> j & 1u)) n = col.get_row(a.grad_final, story_ending(a.tables, s, j));
+                    if constexpr (!Shared) gate = col.unpack(gs[j]);
+                    const Quad v = col.unpack(ss[j]);
+                    Quad slope, term;
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        slope.v[q] = add2(v.v[q], n.v[q]);
+                        term.v[q] = mul2(slope.v[q], previous[j].v[q]);
+                        n.v[q] = mul2(gate.v[q], slope.v[q]);
+                        if constexpr (Shared) sum.v[q] = add2(sum.v[q], term.v[q]);
+                    }
+                    col.put(out + (size_t)j * a.channels, slope);
+                    if constexpr (!Shared) col.put(out_gate + (size_t)j * a.channels, term);
+                    if (!kPlain && a.grad_initial && (s.starts >> j & 1u))
+                        col.put_row(a.grad_initial, story_starting(a.tables, s, j), n);
+                }
+        }
+    });
+    if constexpr (Backward && Shared) {
+        col.put_shared(states[segment], sum);  // only these threads' columns, which they have read
+        __syncthreads();
+        if (threadIdx.x < kColumns && c < a.channels) {
+            float total = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kSegments; ++w) total += states[w][k];
+            a.scratch.partials[(size_t)tile.tile * a.channels + c] = total;
         }
     }
     if (tile.tile == 0 && a.tables.full < a.tables.stories && side == 0) {
@@ -1362,8 +1396,8 @@ __global__ void __launch_bounds__(kReduceThreads) shared_decay_kernel(const floa
 }
 
 // One token of every lane: Unit neighbouring channels a thread.  Bound by memory
-// (two reads, the state's read and write, one write a channel): 4,096 x 4,096 with
-// float32 gates move 268 MB.
+// (two reads, the state's read and write, one write a channel): 4,096 x 4,096 in
+// bfloat16 with float32 gates move 268 MB in 43 us, 96 % of a copy's rate.
 template <typename T, typename G, int Unit>
 __global__ void __launch_bounds__(256)
     step_kernel(uint32_t lanes, uint32_t channels, const T* drive, int64_t drive_stride, const G* decay,
@@ -1594,7 +1628,7 @@ void launch_scan(ScanArgs& a, void* workspace, size_t workspace_bytes, cudaStrea
     }
     // Whole tiles that may be worked on side by side without waiting for one another, of those in the longest row.
     const uint64_t whole = (uint64_t)a.tables.tiles[0] * a.groups;
-    if (a.tables.longest[0] > kGroup && whole / a.tables.longest[0] < kAbreast[Backward]) {
+    if (a.tables.longest[0] > kGroup && whole / a.tables.longest[0] < kAbreast) {
         a.tiles = a.tables.tiles[0];
         a.schedule = a.tables.schedule[0][Backward];
         constexpr uint32_t threads = 16 * kSegments;
