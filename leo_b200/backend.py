@@ -25,6 +25,7 @@ Errors raise :class:`leo_b200.native.LeoError`; there is no CPU fallback.
 from __future__ import annotations
 
 import ctypes as C
+import math
 from dataclasses import dataclass
 
 import numpy as np
@@ -516,7 +517,8 @@ class GpuBackend:
         ``history`` (bytes or symbol numbers), ``bias`` and ``allowed`` (257
         numbers and truth values, the last for the end of the document), then
         the largest at ``temperature`` 0, or the one that ``uniform`` in [0, 1)
-        falls on."""
+        falls on.  Arguments are checked before the step; if then no symbol is
+        left to pick, :class:`leo_b200.native.LeoError` is raised after it."""
         import torch
 
         from .logits import pack_allowed, pick_symbols
@@ -526,9 +528,10 @@ class GpuBackend:
             raise ValueError("uniform must lie in [0, 1)")
         if bias is not None and len(bias) != OUTPUT_CLASSES or allowed is not None and len(allowed) != OUTPUT_CLASSES:
             raise ValueError(f"bias and allowed have {OUTPUT_CLASSES} entries, one a class")
-        # A target makes the step form its probabilities; a frozen one neither learns from it nor counts it.
-        self.training_step_batch([(symbol, 0)], FROZEN)
-        p = self.lane_array(self.CANONICAL_LANE, "probabilities", capacity=4 * OUTPUT_CLASSES)
+        if not temperature >= 0.0 or not 0.0 < repetition < math.inf:
+            raise ValueError("temperature must not be negative, repetition must be positive and finite")
+        if not math.isfinite(presence) or not math.isfinite(frequency):
+            raise ValueError("presence and frequency must be finite")
         where = torch.device("cuda", self.device)
         rules = {"repetition": repetition, "presence": presence, "frequency": frequency}
         if spoken:
@@ -537,6 +540,9 @@ class GpuBackend:
             rules["bias"] = torch.as_tensor(bias, dtype=torch.float32).to(where)
         if allowed is not None:
             rules["allowed"] = pack_allowed(torch.as_tensor(allowed, dtype=torch.bool)[None]).to(where)
+        # A target makes the step form its probabilities; a frozen one neither learns from it nor counts it.
+        self.training_step_batch([(symbol, 0)], FROZEN)
+        p = self.lane_array(self.CANONICAL_LANE, "probabilities", capacity=4 * OUTPUT_CLASSES)
         logits = torch.log(torch.from_numpy(p)).to(where)[None]
         symbols, chance = pick_symbols(logits, temperature=temperature,
                                        uniforms=torch.full((1,), uniform, dtype=torch.float64, device=where), **rules)

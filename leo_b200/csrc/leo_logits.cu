@@ -243,8 +243,9 @@ __device__ __forceinline__ void read_bias(const RowRules& k, const Row<T>& row, 
 // A block takes a run of a row, of up to kAdjustRun symbols: it counts the
 // history's symbols in it once, in shared memory, then goes through it with the
 // groups of the next turn in flight.  Any vocabulary and history fit, and the runs
-// of a long row go side by side.  (256 x 50,001 with 1,000 symbols of history: 33 us
-// in runs of 4,096 symbols, whose counts then take longer than their logits.)
+// of a long row go side by side.  256 x 50,001 bfloat16 with 1,000 symbols of history
+// and a bias row each: 27 us, 31 us with nothing in L2, where a copy's rate gives 16 us;
+// 33 us in runs of 4,096 symbols, whose counts then take longer than their logits.
 constexpr uint32_t kAdjustThreads = 256;
 constexpr uint32_t kAdjustTurn = kAdjustThreads * 8;   // symbols of a turn
 constexpr uint32_t kAdjustRun = 4 * kAdjustTurn;
@@ -347,7 +348,10 @@ __device__ __forceinline__ double exp_down(double y, const double* two_to) {
     return none ? 0.0 : __hiloint2double(high, __double2loint(v));
 }
 
-// A sum of weights exp((z - top) / heat), by its own top; `cold` is 64 / ln 2 / heat.
+// 64 / ln 2 / heat.  Above 0, so that a masked place's -inf stays -inf at an infinite temperature.
+__device__ __forceinline__ double cold_of(double heat) { return fmax(kSixtyFourths / heat, 0x1p-1000); }
+
+// A sum of weights exp((z - top) / heat), by its own top; `cold` is cold_of(heat).
 struct Weights {
     double top, sum;
 };
@@ -382,8 +386,9 @@ struct Part {
 // step the running sum passes u * total, and one warp walks that step again.
 // Everything is in 64 bits: among 131,072 borders between symbols a float32 sum
 // would put one in a hundred draws on the wrong side.  What bounds it is the 64-bit
-// exponential, some 16 operations a symbol: 8.4 million symbols take 9 us at the
-// card's rate for them, their logits 3 us at its bandwidth.
+// exponential, some 16 operations a symbol in a chain: 64 rows of 131,072 take 54 us,
+// with the issue slots two fifths full; the operations take 9 us at the card's rate
+// for them, the logits 3 us at its bandwidth.
 constexpr uint32_t kStepSymbols = 256;
 constexpr uint32_t kPickWindow = 96;  // steps whose counts are in shared memory at a time
 
@@ -413,7 +418,7 @@ __global__ void __launch_bounds__(32 * Warps) pick_kernel(const __grid_constant_
     const float temperature = a.temperature ? a.temperature[at] : a.temperature_value;
     const bool greedy = temperature == 0.0f;
     const double uniform = a.uniforms ? a.uniforms[at] : 0.0;
-    const double heat = greedy ? 1.0 : (double)temperature, cold = kSixtyFourths / heat;
+    const double heat = greedy ? 1.0 : (double)temperature, cold = cold_of(heat);
     const double reciprocal = 1.0 / (double)k.repetition;
     for (uint32_t j = threadIdx.x; j < kPowers; j += 32 * Warps) two_to[j] = kTwoTo[j];
 
@@ -684,7 +689,7 @@ __global__ void __launch_bounds__(128) narrow_pick_kernel(const __grid_constant_
     else
         __syncthreads();
     const bool greedy = temperature == 0.0f;
-    const double heat = greedy ? 1.0 : (double)temperature, cold = kSixtyFourths / heat;
+    const double heat = greedy ? 1.0 : (double)temperature, cold = cold_of(heat);
     const double reciprocal = 1.0 / (double)k.repetition;
     double z[N], best_value = -CUDART_INF;
     uint32_t best = kAll, bad = !(temperature >= 0.0f);
@@ -822,7 +827,8 @@ struct RowScale {
 };
 
 // Rows of up to 32 N symbols, a warp each: symbol 32 j + lane is in register j,
-// so the mask's word j is the warp's, and the logits are read once.
+// so the mask's word j is the warp's, and the logits are read once.  81,984 rows of 257
+// float32 take 39 us (26 us at a copy's rate), with the issue slots three quarters full.
 template <typename T, int N>
 __global__ void __launch_bounds__(256) narrow_loss_kernel(const __grid_constant__ LossArgs a) {
     const uint32_t lane = threadIdx.x & 31u;
@@ -882,9 +888,10 @@ __global__ void __launch_bounds__(256) narrow_loss_kernel(const __grid_constant_
 // weights, the gradient.  The first two are a warp's own, by its own largest
 // logit, so that the warps meet once.  A row that fits is copied into shared memory first,
 // each thread the groups that it will sweep, so that it comes from memory once
-// and three blocks an SM overlap their copies with the others' sweeps (2,048 x
-// 32,001 bfloat16: 87 us with the row in registers and two blocks); a larger one
-// is read in every sweep, the last two times out of L2.
+// and three blocks an SM overlap their copies with the others' sweeps; a larger one
+// is read in every sweep, the last two times out of L2.  2,048 x 32,001 bfloat16: 63 us
+// (40 us at a copy's rate; two exponentials a symbol fill three quarters of the issue
+// slots with what goes with them), 87 us with the row in registers and two blocks.
 template <typename T, int Threads, bool Held>
 __global__ void __launch_bounds__(Threads, Held ? 3 : 2) wide_loss_kernel(const __grid_constant__ LossArgs a) {
     extern __shared__ __align__(16) unsigned char dynamic[];

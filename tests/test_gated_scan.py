@@ -321,6 +321,18 @@ def test_scan_and_gradients(native_lib, lengths, channels, dtype, decay):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("channels", [1, 66, 136])
+@pytest.mark.parametrize("dtype,decay", [("f32", "f32"), ("f32", "channel"), ("bf16", "bf16"), ("bf16", "f32"),
+                                         ("bf16", "channel"), ("f16", "f16"), ("f16", "channel")])
+def test_long_stories_of_few_channels(native_lib, channels, dtype, decay):
+    """Tiles mapped ahead, with short, empty and long stories around one another."""
+    lengths = [300, 2600, 0, 1, 5, 130, 2200, 64]
+    s = make(41, lengths, channels, DTYPES[dtype], decay, channels != 66, "cuda")
+    scan, grad = run_all(s, lengths)
+    check_all(s, lengths, scan, grad)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("lengths,channels,dtype,decay", [
     ([3000, 600], 1600, "bf16", "f32"), ([2300], 1537, "f32", "f32"), ([5000], 768, "f16", "channel"),
     ([40, 3500, 100, 2700], 648, "f32", "channel"), ([2500, 7], 1282, "bf16", "bf16")])

@@ -358,6 +358,20 @@ def test_pick_at_the_edges(native_lib, vocabulary):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("vocabulary", [70, 900, 9000])
+def test_pick_at_any_temperature(native_lib, vocabulary):
+    """From the smallest float to infinity, where every symbol that is left is as likely."""
+    g = torch.Generator().manual_seed(vocabulary)
+    temperature = torch.tensor([1e-45, 1e-30, 1e-3, 1e3, 1e30, 3e38, math.inf, math.inf])
+    x = torch.randn(8, vocabulary, generator=g)
+    x[:, ::3] = -math.inf
+    x[7] = -math.inf
+    x[7, 5::7] = torch.randn(x[7, 5::7].shape, generator=g)
+    uniforms = torch.rand(8, generator=g, dtype=torch.float64)
+    check_pick({"logits": x, "rules": {}}, x.cuda(), {}, temperature.cuda(), uniforms.cuda())
+
+
+@pytest.mark.gpu
 def test_draws_follow_the_distribution(native_lib):
     """Evenly spread uniforms hit every symbol as often as its probability says, to one draw."""
     from leo_b200.logits import pick_symbols

@@ -167,6 +167,11 @@ def test_backend_picks_the_next_symbol(native_lib):
         assert drawn == END_DOCUMENT or p[drawn] > 0
         with pytest.raises(LeoError, match="no symbol is left"):
             gpu.next_symbol(65, allowed=[False] * 257)
+        before = gpu.lane_array(gpu.CANONICAL_LANE, "probabilities", capacity=4 * 257).copy()
+        for refused in ({"temperature": -1.0}, {"repetition": 0.0}, {"presence": float("nan")}):
+            with pytest.raises(ValueError, match="must"):
+                gpu.next_symbol(66, **refused)  # no step is taken
+        assert np.array_equal(before, gpu.lane_array(gpu.CANONICAL_LANE, "probabilities", capacity=4 * 257))
         with pytest.raises(ValueError, match="uniform"):
             gpu.next_symbol(65, uniform=1.0)
         with pytest.raises(ValueError, match="257 entries"):
