@@ -15,6 +15,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -65,7 +66,7 @@ def build(verbose: bool = False) -> Path:
     BUILD.mkdir(exist_ok=True)
     headers = list(CSRC.glob("*.h")) + list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.inc")) + \
         list((ROOT / "include").glob("*.h"))
-    objects = []
+    objects, commands = [], []
     common = ["-std=c++17", "-O3", "-lineinfo", "-Xcompiler", "-fPIC", "-I", str(ROOT / "include")]
     for name in CU_SOURCES:
         src = CSRC / name
@@ -75,15 +76,17 @@ def build(verbose: bool = False) -> Path:
                    "-Xcompiler", "-ffp-contract=off", "-c", str(src), "-o", str(obj)]
             if verbose:
                 cmd.insert(1, "-Xptxas=-v")
-            _run(cmd)
+            commands.append(cmd)
         objects.append(obj)
     for name in CPP_SOURCES:
         src = CSRC / name
         obj = BUILD / (name + ".o")
         if _stale(obj, [src] + headers):
-            _run(["g++", "-std=c++17", "-O2", "-fPIC", "-ffp-contract=off", "-fno-fast-math", "-I",
-                  str(ROOT / "include"), "-c", str(src), "-o", str(obj)])
+            commands.append(["g++", "-std=c++17", "-O2", "-fPIC", "-ffp-contract=off", "-fno-fast-math", "-I",
+                             str(ROOT / "include"), "-c", str(src), "-o", str(obj)])
         objects.append(obj)
+    with ThreadPoolExecutor(max(1, min(len(commands), os.cpu_count() or 1))) as pool:
+        list(pool.map(_run, commands))
     if _stale(LIB, objects):
         _run([NVCC, *ARCH, "-shared", "-o", str(LIB), *map(str, objects), "-lcudart"])
     return LIB
@@ -91,4 +94,3 @@ def build(verbose: bool = False) -> Path:
 
 if __name__ == "__main__":
     print(build(verbose="-v" in sys.argv))
-    _ = os
