@@ -827,9 +827,11 @@ struct RowScale {
 };
 
 // Rows of up to 32 N symbols, a warp each: symbol 32 j + lane is in register j,
-// so the mask's word j is the warp's, and the logits are read once.  81,984 rows of 257
-// float32 take 39 us (26 us at a copy's rate), with the issue slots three quarters full.
-template <typename T, int N>
+// so the mask's word j is the warp's, and the logits are read once.  Full: all
+// registers but the last are, which spares their tests.  81,984 rows of 257
+// float32 take 37 us, 39 us with the tests (26 us at a copy's rate); the issue slots
+// are three quarters full.
+template <typename T, int N, bool Full>
 __global__ void __launch_bounds__(256) narrow_loss_kernel(const __grid_constant__ LossArgs a) {
     const uint32_t lane = threadIdx.x & 31u;
     const uint64_t at = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -837,25 +839,28 @@ __global__ void __launch_bounds__(256) narrow_loss_kernel(const __grid_constant_
     const uint32_t row = (uint32_t)at;
     const T* in = static_cast<const T*>(a.logits) + (int64_t)row * a.logits_stride + lane;
     T* out = static_cast<T*>(a.gradient) + (int64_t)row * a.gradient_stride + lane;
-    const uint32_t mine = (a.vocabulary + 31 - lane) / 32;  // symbols of the lane
+    const uint32_t symbols = (a.vocabulary + 31 - lane) / 32;  // of the lane
+    const auto mine = [&](int j) { return Full && j < N - 1 ? true : j < (int)symbols; };
     float z[N];
 #pragma unroll
-    for (int j = 0; j < N; ++j) z[j] = j < mine ? load(in + 32 * j) : -CUDART_INF_F;
+    for (int j = 0; j < N; ++j) z[j] = mine(j) ? load(in + 32 * j) : -CUDART_INF_F;
     const int32_t target = a.targets[row];
     const MaskRow mask = mask_row(a.allowed, a.allowed_stride, a.states, a.state, row);
     const bool outside = target >= 0 && (uint32_t)target >= a.vocabulary;
     if (target < 0 || outside) {
 #pragma unroll
         for (int j = 0; j < N; ++j)
-            if (j < mine) store(out + 32 * j, 0.0f);
+            if (mine(j)) store(out + 32 * j, 0.0f);
         if (lane == 0) a.losses[row] = outside ? CUDART_NAN_F : 0.0f;
         return;
     }
+    const bool counts = mask.allows((uint32_t)target);
+    const float hit = counts ? load(in - lane + target) : -CUDART_INF_F;
     const uint32_t bit = 1u << lane;
     if (mask.words) {
 #pragma unroll
         for (int j = 0; j < N; ++j)
-            if (j < mine && !(__ldg(mask.words + j) & bit)) z[j] = -CUDART_INF_F;
+            if (mine(j) && !(__ldg(mask.words + j) & bit)) z[j] = -CUDART_INF_F;
     } else if (!mask.open) {
 #pragma unroll
         for (int j = 0; j < N; ++j) z[j] = -CUDART_INF_F;
@@ -874,11 +879,9 @@ __global__ void __launch_bounds__(256) narrow_loss_kernel(const __grid_constant_
     const float scale = a.weights ? a.weights[row] : 1.0f, gain = sum == 0.0f ? 0.0f : scale / sum;
 #pragma unroll
     for (int j = 0; j < N; ++j)
-        if (j < mine) store(out + 32 * j, w[j] * gain);
+        if (mine(j)) store(out + 32 * j, w[j] * gain);
     // The target's term, in place of what this lane has written there.
     if (lane == ((uint32_t)target & 31u)) {
-        const bool counts = mask.allows((uint32_t)target);
-        const float hit = counts ? load(in + (target & ~31)) : -CUDART_INF_F;
         if (counts && sum != 0.0f) store(out + (target & ~31), fmaf(by.weight(hit), gain, -scale));
         a.losses[row] = by.loss(sum, hit);
     }
@@ -1040,13 +1043,15 @@ void launch_pick(const LogitArgs& a, cudaStream_t stream) {
     check(cudaLaunchKernelEx(&config, kernel, a, steps), "pick_kernel");
 }
 
-// A warp a row while it holds the row in 32 registers a lane, a block above.
+// A warp a row while it holds the row in 32 registers a lane (rows of bytes and the
+// end, the framework's own, in full ones), a block above.
 template <typename T>
 void launch_loss(const LossArgs& a, cudaStream_t stream) {
     const uint32_t v = a.vocabulary, warps = (a.rows + 7) / 8;
-    if (v <= 288) narrow_loss_kernel<T, 9><<<warps, 256, 0, stream>>>(a);
-    else if (v <= 512) narrow_loss_kernel<T, 16><<<warps, 256, 0, stream>>>(a);
-    else if (v <= 1024) narrow_loss_kernel<T, 32><<<warps, 256, 0, stream>>>(a);
+    if (v <= 256) narrow_loss_kernel<T, 8, false><<<warps, 256, 0, stream>>>(a);
+    else if (v <= 288) narrow_loss_kernel<T, 9, true><<<warps, 256, 0, stream>>>(a);
+    else if (v <= 512) narrow_loss_kernel<T, 16, false><<<warps, 256, 0, stream>>>(a);
+    else if (v <= 1024) narrow_loss_kernel<T, 32, false><<<warps, 256, 0, stream>>>(a);
     else if (const size_t held = ((size_t)v + 14) / 8 * sizeof(Eight<T>); held <= 110 * 1024) {
         // three blocks an SM up to 75 KB a row, two up to 110 KB
         const bool small = v <= 8192;
