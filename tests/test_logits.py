@@ -439,6 +439,18 @@ def test_loss(native_lib, rows, vocabulary, states, pad, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("vocabulary", [1, 32, 255, 256, 257, 288, 289, 512, 513, 1024, 1025, 8192, 8193])
+def test_loss_at_every_width(native_lib, vocabulary):
+    """Both sides of every border between forms of the kernel."""
+    s = make(vocabulary, 11, vocabulary, torch.float32, 0, 3, None)
+    logits, rules = to_gpu(s, 2)
+    g = torch.Generator().manual_seed(vocabulary)
+    targets = torch.randint(-1, vocabulary, (11,), generator=g, dtype=torch.int32)
+    targets[0], targets[1] = vocabulary - 1, vocabulary
+    check_loss(s, logits, rules, targets, torch.rand(11, generator=g))
+
+
+@pytest.mark.gpu
 def test_loss_of_odd_rows(native_lib):
     """-inf logits, a certain symbol, huge and equal logits, a NaN where it counts."""
     from leo_b200.logits import masked_cross_entropy
