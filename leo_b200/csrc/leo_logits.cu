@@ -2,8 +2,8 @@
 // grammar masks; the pick of the next symbol; the cross entropy over the
 // allowed symbols with its gradient.
 //
-// All three are bound by reading the logits once (and writing as much, except
-// the pick).  Rows start anywhere, so they are read in groups of eight symbols
+// Each has to read the logits once (and write as much, except the pick); what it
+// is bound by stands at its kernel.  Rows start anywhere, so they are read in groups of eight symbols
 // laid so that the addresses are multiples of 16 bytes, the ends of a row one by
 // one; a row of 257 classes and the like is one warp's in the loss.
 #include <cooperative_groups.h>
