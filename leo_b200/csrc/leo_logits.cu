@@ -420,6 +420,10 @@ __global__ void __launch_bounds__(32 * Warps) pick_kernel(const __grid_constant_
     const double uniform = a.uniforms ? a.uniforms[at] : 0.0;
     const double heat = greedy ? 1.0 : (double)temperature, cold = cold_of(heat);
     const double reciprocal = 1.0 / (double)k.repetition;
+    // A step's weights are taken by the float of its largest logit.  The two are 2^-24 of it
+    // apart, which times `cold`, as weights see it, is at most a 64th of a power of two up to
+    // here; beyond, where a small temperature makes more of it, the largest itself is found.
+    const float near = (float)fmin(1e38, 0x1p24 / cold);
     for (uint32_t j = threadIdx.x; j < kPowers; j += 32 * Warps) two_to[j] = kTwoTo[j];
 
     // Bit i: symbol v + i is in the row and allowed.
@@ -502,8 +506,9 @@ __global__ void __launch_bounds__(32 * Warps) pick_kernel(const __grid_constant_
                     if (z[i] > best_value) best_value = z[i], best = (uint32_t)(v + i);
                 best_rough = fmaxf(best_rough, most);
             }
-            double top = (double)warp_max(most);
-            if (!(fabs(top) < 1e38)) {  // what float calls infinite may not be
+            most = warp_max(most);
+            double top = (double)most;
+            if (!(fabsf(most) < near)) {  // and what float calls infinite may not be
                 top = z[0];
 #pragma unroll
                 for (int i = 1; i < 8; ++i) top = fmax(top, z[i]);
@@ -581,7 +586,7 @@ __global__ void __launch_bounds__(32 * Warps) pick_kernel(const __grid_constant_
                 if (owner == kAll) owner = last;  // u is nearly 1, and the sums were rounded
                 if (rank == owner) {
                     double running = sum_before, step_before = sum_before;
-                    uint32_t found = kAll, last_step = 0;
+                    uint32_t found = kAll, last_step = (mine.best - (uint32_t)block_first) / kStepSymbols;
                     for (uint32_t base = 0; base < steps && found == kAll; base += 32) {
                         const uint32_t j = base + lane;
                         const double s = j < steps ? by(weights[j], best_value) : 0.0;
@@ -652,8 +657,18 @@ __global__ void __launch_bounds__(32 * Warps) pick_kernel(const __grid_constant_
             if (hit == kAll && running > goal) hit = last, hit_z = z[i];
         }
     }
+    const uint32_t hits = __ballot_sync(kAll, hit != kAll);
+    uint32_t some = __ballot_sync(kAll, last != kAll);
+    if (some == 0) {  // the step had a weight by the float of its largest logit only: that symbol
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (last == kAll || z[i] > last_z) last = (uint32_t)(v + i), last_z = z[i];
+        double most = last_z;
+        for (int off = 16; off > 0; off >>= 1) most = fmax(most, __shfl_xor_sync(kAll, most, off));
+        some = __ballot_sync(kAll, last_z == most);
+        some &= -some;  // the lowest of equal ones
+    }
     // The first lane with a hit, or, the sums having been rounded, the last with any weight.
-    const uint32_t hits = __ballot_sync(kAll, hit != kAll), some = __ballot_sync(kAll, last != kAll);
     if (hits ? lane == (uint32_t)__ffs(hits) - 1u : lane == 31u - __clz(some)) {
         const double logit = hits ? hit_z : last_z;
         a.symbols[at] = (int32_t)(hits ? hit : last);
