@@ -819,7 +819,7 @@ __device__ __forceinline__ float exp2_of(float x) {
 struct RowScale {
     float top, c, shift, off;  // weights are 2^off times too large
     __device__ __forceinline__ explicit RowScale(float top_) : top(top_) {
-        c = fabsf(top) < 1e37f ? 1.44269504f : 0x1p-20f;
+        c = fabsf(top) <= 0x1p30f ? 1.44269504f : 1.0f;
         shift = top == -CUDART_INF_F ? 0.0f : top * c;
         off = top == -CUDART_INF_F ? 0.0f : fmaf(top, c, -shift);
     }
@@ -837,7 +837,9 @@ struct RowScale {
     __device__ __forceinline__ float loss(float sum, float z) const {
         if (sum != sum) return sum;
         if (sum == 0.0f || z == -CUDART_INF_F) return CUDART_INF_F;
-        return fmaf(off, -0.693147181f, logf(sum)) + (top - z);
+        // The whole part of `off` comes out of the sum exactly.
+        const float whole = rintf(off);
+        return fmaf(off - whole, -0.693147181f, logf(sum * __int_as_float((127 - (int)whole) << 23))) + (top - z);
     }
 };
 
