@@ -26,6 +26,7 @@ from typing import NamedTuple, Sequence
 
 import numpy as np
 import torch
+from torch.autograd.graph import increment_version
 
 from . import native
 from .ctypes_types import LeoB200StoryTables
@@ -232,4 +233,5 @@ def gated_step(drive, decay, state, stream=None):
         native.check(native.lib().leo_b200_gated_step(
             device, lanes, channels, code, drive.data_ptr(), stride, decay_code, decay.data_ptr(), decay_stride, shared,
             state.data_ptr(), state_stride, output.data_ptr(), raw))
+    increment_version(state)  # a backward pass that saved it fails instead of using the new values
     return output

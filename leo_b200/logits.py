@@ -23,6 +23,7 @@ import ctypes as C
 import struct
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import native
 from .ctypes_types import LeoB200LogitRules
@@ -147,12 +148,15 @@ def adjust_logits(logits, *, history=None, lengths=None, repetition=1.0, presenc
         check_tensor("out", out, device, logits.dtype, logits.shape)
         if row_stride("out", out) < vocabulary and rows > 1:
             raise ValueError("the rows of out overlap")
+    given = out
     with on_stream(device, stream, rules.tensors + (out,)) as raw:
         if out is None:
             out = logits.new_empty((rows, vocabulary))
         native.check(native.lib().leo_b200_adjust_logits(
             device, code, logits.data_ptr(), stride, rows, vocabulary, rules.packed, out.data_ptr(),
             out.stride(0), raw))
+    if given is not None:
+        increment_version(given)  # a backward pass that saved it fails instead of using the new values
     return out
 
 
