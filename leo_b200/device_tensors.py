@@ -6,6 +6,7 @@ from __future__ import annotations
 import contextlib
 
 import torch
+from torch.autograd import forward_ad
 
 from .ctypes_types import BF16, F16, F32
 
@@ -17,8 +18,8 @@ def device_of(name: str, tensor) -> int:
     index = tensor.get_device() if isinstance(tensor, torch.Tensor) else -1
     if index < 0 or not tensor.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
-    if tensor.requires_grad:
-        _refuse_gradient(name)
+    if tensor.requires_grad or forward_ad._current_level >= 0:
+        _refuse_gradient(name, tensor)
     return index
 
 
@@ -29,16 +30,19 @@ def dtype_code(name: str, tensor) -> int:
     return code
 
 
-def _refuse_gradient(name: str) -> None:
-    if torch.is_grad_enabled():
+def _refuse_gradient(name: str, tensor) -> None:
+    if tensor.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} asks for a gradient, which this call does not record: detach it and use the "
                          "gradients that the operators return")
+    if forward_ad.unpack_dual(tensor).tangent is not None:
+        raise ValueError(f"{name} has a tangent, which this call does not carry on")
 
 
 def check_tensor(name: str, tensor, device: int, dtype=None, shape=None) -> None:
     """A tensor of the call: on CUDA device ``device``, asking for no gradient."""
     if (isinstance(tensor, torch.Tensor) and tensor.get_device() == device and (dtype is None or tensor.dtype == dtype)
-            and (shape is None or tensor.shape == shape) and not tensor.requires_grad):
+            and (shape is None or tensor.shape == shape) and not tensor.requires_grad
+            and forward_ad._current_level < 0):
         return
     if not isinstance(tensor, torch.Tensor) or not tensor.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
@@ -48,7 +52,7 @@ def check_tensor(name: str, tensor, device: int, dtype=None, shape=None) -> None
         raise ValueError(f"{name} must be {dtype}, not {tensor.dtype}")
     if shape is not None and tensor.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(tensor.shape)}")
-    _refuse_gradient(name)
+    _refuse_gradient(name, tensor)
 
 
 def row_stride(name: str, tensor) -> int:
