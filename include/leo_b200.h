@@ -355,7 +355,9 @@ size_t leo_b200_gated_scan_carry_count(const LeoB200StoryTables* tables, uint32_
    once.  `decay` is one row per token (decay_shared 0; of `dtype` or float)
    or one row for all tokens (decay_shared 1).  Gates are meant to lie in
    [-1, 1]; a larger one is taken as it is, as long as the product of the
-   gates of any span of a story stays finite.  final_states[story] (float,
+   gates of any span of a story stays finite.  An infinite state stays infinite
+   as the recurrence keeps it, but may be NaN after eight gates in a row whose
+   product is 0 in float, as after a gate of 0.  final_states[story] (float,
    [stories][channels]) receives the state after the last token, initial[story]
    for a story without one.  `carries` (NULL: not kept) receives
    leo_b200_gated_scan_carry_count floats for the backward pass. */

@@ -195,6 +195,20 @@ __device__ __forceinline__ float value_of(float2 x) {
     return x.y == x.y ? x.x + x.y : x.x;  // an infinite product has no error term
 }
 
+// A product of segments' products that underflows has to leave an infinite state
+// infinite: it becomes the smallest float of its sign.  (It adds at most 2^-149 of a
+// finite state, as a rounding among the subnormals does.)  A segment's own product may
+// be 0, by a gate of 0 or by gates below 2^-18, and makes an infinite state NaN.
+__device__ __forceinline__ float smallest(float zero) { return __uint_as_float(__float_as_uint(zero) | 1u); }
+__device__ __forceinline__ float times(float x, float y) {
+    const float p = x * y;
+    return p == 0.0f && x != 0.0f && y != 0.0f ? smallest(p) : p;
+}
+__device__ __forceinline__ float2 times(float2 x, float2 y) {
+    const float2 p = product_of(x, y);
+    return p.x == 0.0f ? make_float2(times(x.x, y.x), 0.0f) : p;
+}
+
 // The state before a tile, out of the slots between it and the tile that holds
 // the near end of the story that crosses into it, or the nearest one that
 // published a state.  Direction +1: from the left; -1: from the right.
@@ -227,7 +241,7 @@ struct Lookback {
         for (int j = 0; j < 8; ++j)
             if (j < count) s[j] = read_slot(p + j * step);
     }
-    // Composes them as (A, H); false if one of them was not there yet.
+    // From the left: composes them as (A, H); false if one of them was not there yet.
     __device__ __forceinline__ bool compose(const Slot (&s)[8], int half, float& A, float& H) const {
         const int count = maps + 1 - half * 8;
         bool there = true;
@@ -242,6 +256,32 @@ struct Lookback {
                 A *= __uint_as_float(low);
             }
         return there;
+    }
+    // The product of half 1 again, kept from 0.
+    __device__ __forceinline__ float product(const Slot (&s)[8]) const {
+        float A = 1.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < maps - 7) A = times(A, __uint_as_float((uint32_t)s[j]));
+        return A;
+    }
+    // From the right: whether all are there.
+    __device__ __forceinline__ bool there(const Slot (&s)[8], int half) const {
+        bool all = true;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < maps + 1 - half * 8) all = all && (uint32_t)s[j] != kNone;
+        return all;
+    }
+    // The state after them; for half 1 from that after half 0.
+    __device__ __forceinline__ float run(const Slot (&s)[8], int half, float state) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < maps + 1 - half * 8) {
+                const float value = __uint_as_float((uint32_t)(s[j] >> 32));
+                state = j == 0 && half == 0 ? value : fmaf(__uint_as_float((uint32_t)s[j]), state, value);
+            }
+        return state;
     }
 };
 
@@ -849,31 +889,53 @@ __global__ void __launch_bounds__(Shape<T, G, Shared, Backward>::kThreads, 1) sc
                 kept = __ldcs(a.carries + (size_t)work.kept * a.channels + c);
             float carry = 0.0f;
             if (back.maps >= 0) {
+                // Forward, the halves are composed at the same time, since tiles wait for the state; backward, with
+                // more to do elsewhere, one after the other, which needs no product (20,480 tokens x 4,096: 144 and
+                // 266 us; 146 and 271 us the other way round).
                 float A = 1.0f, H = 0.0f;
-                bool there = !active || back.compose(slots, (int)half, A, H);
+                const auto look = [&] {
+                    if constexpr (Direction > 0)
+                        return back.compose(slots, (int)half, A, H);
+                    else
+                        return back.there(slots, (int)half);
+                };
+                bool there = !active || look(), gave_up = false;
                 for (uint32_t n = 0; !__all_sync(kNone, there); ++n) {
                     if (n >= kSpinLimit) {
                         if (lane == 0) atomicExch(&g_gave_up, 1u);
-                        A = H = CUDART_NAN_F;
+                        gave_up = true;
                         break;
                     }
                     if (active) {
                         back.load(a.scratch.slots, a.channels, c, (int)half, slots);
-                        there = back.compose(slots, (int)half, A, H);
+                        there = look();
                     }
                 }
-                const float other_A = __shfl_xor_sync(kNone, A, 16), other_H = __shfl_xor_sync(kNone, H, 16);
-                // the far half's map of the near half's state; one slot is the state itself
-                if (back.maps < 8)
-                    carry = half ? other_H : H;
-                else
-                    carry = half ? fmaf(A, other_H, H) : fmaf(other_A, H, other_H);
+                if constexpr (Direction > 0) {
+                    const float other_A = __shfl_xor_sync(kNone, A, 16), other_H = __shfl_xor_sync(kNone, H, 16);
+                    // the far half's map of the near half's state; one slot is the state itself
+                    if (back.maps < 8) {
+                        carry = half ? other_H : H;
+                    } else {
+                        carry = half ? fmaf(A, other_H, H) : fmaf(other_A, H, other_H);
+                        if (__any_sync(kNone, carry != carry)) {  // an infinite state, perhaps, times 0
+                            if (half) A = back.product(slots);
+                            const float kept_A = __shfl_xor_sync(kNone, A, 16);
+                            carry = half ? fmaf(A, other_H, H) : fmaf(kept_A, H, other_H);
+                        }
+                    }
+                } else {
+                    if (active && half == 0) carry = back.run(slots, 0, 0.0f);
+                    carry = __shfl_xor_sync(kNone, carry, 16);
+                    if (active && half) carry = back.run(slots, 1, carry);
+                }
+                if (gave_up) carry = CUDART_NAN_F;
             }
             if (i >= 2) sync_of<kTaken>(i & 1u);
-            if (half == 0) {
+            if (half)
                 control.scouted[i & 1u][0][k] = carry;
-                if constexpr (Backward) control.scouted[i & 1u][1][k] = kept;
-            }
+            else if constexpr (Backward)
+                control.scouted[i & 1u][1][k] = kept;
             if (leader)
                 control.ring[(i + S::kAhead) & 7u] =
                     Work{x.x, !one_each && ticket < total ? x.y : kNone, x.z, ticket - place * a.groups, y.x, x.w, y.y, 0};
@@ -941,6 +1003,7 @@ __global__ void __launch_bounds__(Shape<T, G, Shared, Backward>::kThreads, 1) sc
             };
             float2 product = make_float2(1.0f, 0.0f);
             float sum = 0.0f, A[kHalf], v[kHalf];
+            bool zero = false;
 #pragma unroll
             for (int j = 0; j < kHalf; ++j) {
                 const int w = segment(j);
@@ -949,7 +1012,9 @@ __global__ void __launch_bounds__(Shape<T, G, Shared, Backward>::kThreads, 1) sc
                 v[j] = Backward ? m.M[Backward ? w : 0][k] : m.H[w][k];
                 sum = cut_at(j) ? v[j] : fmaf(A[j], sum, v[j]);
                 product = product_of(product, p);
+                zero |= A[j] == 0.0f;
             }
+            if (product.x == 0.0f && !zero) product.x = smallest(product.x);
             const bool cut = (cut_bytes.x | cut_bytes.y) != 0;
             const bool other_cut = __shfl_xor_sync(kNone, cut, 16);
             const float other_sum = __shfl_xor_sync(kNone, sum, 16);
@@ -959,7 +1024,9 @@ __global__ void __launch_bounds__(Shape<T, G, Shared, Backward>::kThreads, 1) sc
             const float near_A = value_of(half ? other : product), near_sum = half ? other_sum : sum;
             const bool near_cut = half ? other_cut : cut, far_cut = half ? cut : other_cut;
             const float far_A = value_of(half ? product : other), far_sum = half ? sum : other_sum;
-            const float tile_A = value_of(product_of(product, other));
+            const float both = near_A * far_A;
+            const float tile_A =
+                both == 0.0f && near_A != 0.0f && far_A != 0.0f ? smallest(both) : value_of(product_of(product, other));
             const float tile_sum = far_cut ? far_sum : fmaf(far_A, near_sum, far_sum);
             const bool state_tile = Backward ? tile % kGroup == 0 : (tile + 1) % kGroup == 0;
             const bool writes = active && work.onward && half == 0;
@@ -990,19 +1057,15 @@ __global__ void __launch_bounds__(Shape<T, G, Shared, Backward>::kThreads, 1) sc
                 // The state before each segment: this lane's half from the right is the other one from the left.
                 const uint2 starts = reinterpret_cast<const uint2*>(m.starts)[1 - half];
                 float h[kHalf];
-                float2 P = make_float2(1.0f, 0.0f);
                 float state = 0.0f;
 #pragma unroll
                 for (int j = 0; j < kHalf; ++j) h[j] = m.H[segment(kHalf - 1 - j)][k];
                 const auto start_at = [&](int j) { return ((j < 4 ? starts.x : starts.y) >> (j & 3) * 8 & 1u) != 0; };
 #pragma unroll
-                for (int j = 0; j < kHalf; ++j) {
-                    state = start_at(j) ? h[j] : fmaf(A[kHalf - 1 - j], state, h[j]);
-                    P.x *= A[kHalf - 1 - j];
-                }
+                for (int j = 0; j < kHalf; ++j) state = start_at(j) ? h[j] : fmaf(A[kHalf - 1 - j], state, h[j]);
                 // Lanes of half 1 hold the segments on the left, and pass the state after them on.
                 const bool left_cut = (starts.x | starts.y) != 0;
-                const float after = half ? (left_cut ? state : fmaf(P.x, kept, state)) : 0.0f;
+                const float after = half ? (left_cut ? state : fmaf(far_A, kept, state)) : 0.0f;
                 const float from_left = __shfl_xor_sync(kNone, after, 16);
                 float at = half ? kept : from_left;
 #pragma unroll
@@ -1117,6 +1180,11 @@ __global__ void __launch_bounds__(16 * kSegments) scan_map_kernel(const __grid_c
         all = product_of(all, A);
         cut |= cuts[w] != 0;
     }
+    if (all.x == 0.0f) {
+        all = make_float2(1.0f, 0.0f);
+#pragma unroll 1
+        for (int w = 0; w < kSegments; ++w) all = times(all, products[w][threadIdx.x]);
+    }
     // A map that a story starts in has no product; all bits set say so.
     uint32_t low = __float_as_uint(value_of(all));
     if (low == kNone) low = 0x7fffffffu;
@@ -1138,7 +1206,7 @@ __global__ void __launch_bounds__(1024) scan_join_kernel(const __grid_constant__
             const float value = __uint_as_float((uint32_t)(s >> 32)), product = __uint_as_float((uint32_t)s);
             const bool here = (uint32_t)s == kNone;
             H = here ? value : fmaf(product, H, value);
-            A *= product;
+            A = times(A, product);
             cut |= here;
         }
         __device__ __forceinline__ float of(float state) const { return cut ? H : fmaf(A, state, H); }
@@ -1178,7 +1246,7 @@ __global__ void __launch_bounds__(1024) scan_join_kernel(const __grid_constant__
         const bool cut = __shfl_sync(kNone, mine.cut, from);
         if (r == sub) before = all;
         all.H = cut ? H : fmaf(A, all.H, H);
-        all.A *= A;
+        all.A = times(all.A, A);
         all.cut |= cut;
     }
     if (sub == 0) products[warp][k] = all.A, values[warp][k] = all.H, cuts[warp][k] = all.cut;

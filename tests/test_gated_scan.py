@@ -562,3 +562,64 @@ def test_refusals(native_lib):
     refused(lambda: gated_step(x, x, h0), "state must have shape")
     with torch.no_grad():
         gated_scan(x.clone().requires_grad_(), x, layout)
+
+
+# ---------------------------------------------------------------- infinite states
+
+
+def token_by_token(lengths, s):
+    """States and gradients in 64 bits, a token at a time; infinities and NaN as the recurrence makes them."""
+    x, a, g, h0, gf = (s[k].cpu().double() for k in ("x", "a", "g", "h0", "gf"))
+    a = a.expand_as(x)
+    h, dx, da = torch.zeros_like(x), torch.zeros_like(x), torch.zeros_like(x)
+    final, dh0 = h0.clone(), gf.clone()
+    for i, begin in enumerate(offsets_of(lengths)[:-1]):
+        for t in range(begin, begin + lengths[i]):
+            final[i] = h[t] = a[t] * (h[t - 1] if t > begin else h0[i]) + x[t]
+        for t in reversed(range(begin, begin + lengths[i])):
+            dx[t] = g[t] + dh0[i]
+            da[t] = dx[t] * (h[t - 1] if t > begin else h0[i])
+            dh0[i] = a[t] * dx[t]
+    return h, final, dx, da, dh0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,decay", [("f32", "f32"), ("f32", "channel"), ("bf16", "f32")])
+@pytest.mark.parametrize("lengths,channels", [([1500, 700], 72), ([5000], 10), ([3000, 0, 90, 40], 71),
+                                              ([2500, 130, 2100], 1540)],
+                         ids=["tiles", "runs", "unaligned", "one pass"])
+def test_infinite_states_stay_infinite(native_lib, lengths, channels, dtype, decay):
+    """Products of many gates that underflow: an infinite state times one is infinite, with the sign that
+    the gates give it, and NaN only after a gate of 0; on the way back as well.  Finite channels keep to
+    their bounds, however small their products of gates.  (Eight gates in a row of product 0 in float
+    may do what one of 0 does, which 1e-4 does not reach.)"""
+    s = make(3, lengths, channels, DTYPES[dtype], decay, True)
+    fast = torch.tensor([0.3, 0.05, -0.4, 1e-4, 0.9, -0.01])[torch.arange(channels) % 6]
+    s["a"] = (fast if decay == "channel" else fast.expand(sum(lengths), channels)).clone()
+    bad = torch.arange(channels) // 6 % 2 == 0  # channels with infinities
+    s["h0"][0, bad] = float("inf")
+    s["gf"][0, bad] = -float("inf")
+    if decay != "channel":  # a gate of 0 far behind the infinity, in some of them
+        s["a"][lengths[0] - 2, bad & (torch.arange(channels) % 4 == 0)] = 0.0
+        if len(lengths) == 3:  # and an infinite drive in the middle of the last story
+            s["x"][sum(lengths) - lengths[-1] // 2, bad] = -float("inf")
+    s = {k: v.cuda() for k, v in s.items()}
+    scan, grad = run_all(s, lengths)
+    h, final, dx, da, dh0 = token_by_token(lengths, s)
+    assert bool(torch.isinf(h[:, bad]).any())
+    if decay == "channel":
+        da = da.sum(0)
+    for got, want, what in ((scan.states, h, "states"), (scan.final, final, "final"), (grad.drive, dx, "drive"),
+                            (grad.decay, da, "decay"), (grad.initial, dh0, "initial")):
+        want = want.to(torch.float32)
+        rest = torch.isfinite(want)
+        assert torch.equal(torch.isnan(got.cpu()), torch.isnan(want)), what
+        assert torch.equal(torch.isfinite(got.cpu()), rest), what
+        there = ~rest & ~torch.isnan(want)
+        assert torch.equal(got.cpu().float()[there], want[there]), what
+    clean = {k: v[..., ~bad.cuda()].contiguous() for k, v in s.items()}
+    part = lambda t: t[..., ~bad.cuda()]  # noqa: E731
+    r = oracle(lengths, clean["x"], clean["a"], clean["g"], clean["h0"], clean["gf"])
+    close(part(scan.states), r["h"], r["eh"], "states")
+    close(part(grad.drive), r["dx"], r["edx"], "grad_drive")
+    close(part(grad.decay), r["da"], r["eda"], "grad_decay")
