@@ -526,8 +526,14 @@ class GpuBackend:
         spoken = [OUTPUT_CLASSES - 1 if s == END_DOCUMENT else s if s < OUTPUT_CLASSES - 1 else -1 for s in history]
         if not 0.0 <= uniform < 1.0:
             raise ValueError("uniform must lie in [0, 1)")
-        if bias is not None and len(bias) != OUTPUT_CLASSES or allowed is not None and len(allowed) != OUTPUT_CLASSES:
+        if bias is not None:
+            bias = torch.as_tensor(bias, dtype=torch.float32).detach()
+        if allowed is not None:
+            allowed = torch.as_tensor(allowed, dtype=torch.bool)
+        if any(v is not None and v.shape != (OUTPUT_CLASSES,) for v in (bias, allowed)):
             raise ValueError(f"bias and allowed have {OUTPUT_CLASSES} entries, one a class")
+        # as the pick takes them, in 32 bits
+        repetition, presence, frequency = (C.c_float(v).value for v in (repetition, presence, frequency))
         if not temperature >= 0.0 or not 0.0 < repetition < math.inf:
             raise ValueError("temperature must not be negative, repetition must be positive and finite")
         if not math.isfinite(presence) or not math.isfinite(frequency):
@@ -537,9 +543,9 @@ class GpuBackend:
         if spoken:
             rules["history"] = torch.tensor([spoken], dtype=torch.int32, device=where)
         if bias is not None:
-            rules["bias"] = torch.as_tensor(bias, dtype=torch.float32).to(where)
+            rules["bias"] = bias.to(where)
         if allowed is not None:
-            rules["allowed"] = pack_allowed(torch.as_tensor(allowed, dtype=torch.bool)[None]).to(where)
+            rules["allowed"] = pack_allowed(allowed[None]).to(where)
         # A target makes the step form its probabilities; a frozen one neither learns from it nor counts it.
         self.training_step_batch([(symbol, 0)], FROZEN)
         p = self.lane_array(self.CANONICAL_LANE, "probabilities", capacity=4 * OUTPUT_CLASSES)

@@ -178,3 +178,23 @@ def test_backend_picks_the_next_symbol(native_lib):
             gpu.next_symbol(65, bias=[0.0])
         assert gpu.state_digest() == digest
         assert bytes(gpu.synchronize_model().statistics) == statistics
+
+
+REFUSED = [{"repetition": 1e-50}, {"repetition": 1e300}, {"presence": 1e300}, {"presence": -1e39}, {"frequency": 1e39},
+           {"frequency": float("inf")}, {"bias": np.zeros((257, 1))}, {"bias": [0.0] * 256}, {"bias": 1.0},
+           {"allowed": np.ones((257, 2), bool)}, {"temperature": float("nan")}, {"uniform": float("nan")}]
+
+
+@pytest.mark.parametrize("arguments", REFUSED, ids=[next(iter(r)) for r in REFUSED])
+def test_next_symbol_refuses_before_the_step(arguments):
+    """What 32 bits make 0 or infinite, and what has another shape, is refused while the document stands."""
+    from leo_b200.backend import GpuBackend
+
+    class Standing:
+        device, CANONICAL_LANE = 0, 0
+
+        def training_step_batch(self, *_):
+            pytest.fail("the step was taken")
+
+    with pytest.raises(ValueError):
+        GpuBackend.next_symbol(Standing(), 65, **arguments)
