@@ -302,15 +302,16 @@ template <typename T, typename G, bool Shared, bool Backward>
 struct Shape {
     // A token of a tile takes this much of a stage.
     static constexpr int kRow = kColumns * (int)((Backward ? 2 : 1) * sizeof(T) + (Shared ? 0 : sizeof(G)));
-    struct Maps {
-        float2 A[Shared ? 1 : kSegments][kColumns];   // hi, lo; a shared gate's follow from the tokens
-        float H[kSegments][kColumns];                 // then the state before each segment
-        float M[Backward ? kSegments : 1][kColumns];  // then the value before each segment from the right
-        uint8_t starts[kSegments], ends[kSegments];   // whether a story does in the segment
+    struct Maps {  // read and written up to 16 bytes at a time
+        alignas(16) float2 A[Shared ? 1 : kSegments][kColumns];   // hi, lo; a shared gate's follow from the tokens
+        alignas(16) float H[kSegments][kColumns];     // then the state before each segment
+        alignas(16) float M[Backward ? kSegments : 1][kColumns];  // then the value before each segment from the right
+        alignas(16) uint8_t starts[kSegments];
+        alignas(16) uint8_t ends[kSegments];  // whether a story does in the segment
     };
     struct Control {
         Maps maps[2];
-        float sums[Backward && Shared ? 2 : 1][Backward && Shared ? kSegments : 1][kColumns];
+        alignas(16) float sums[Backward && Shared ? 2 : 1][Backward && Shared ? kSegments : 1][kColumns];
         Work ring[8];  // the block's work; an entry is rewritten when no warp reads it any more
         float scouted[2][Backward ? 2 : 1][kColumns];  // the value before the tile; the kept state before it
         uint64_t landed[4][kWarps];  // barriers of the tiled loads
@@ -1115,8 +1116,8 @@ __device__ __forceinline__ void with_plain(const Segment& s, int length, Body&& 
 template <typename T, typename G, int Unit, bool Shared, bool Backward>
 __global__ void __launch_bounds__(16 * kSegments) scan_map_kernel(const __grid_constant__ ScanArgs a) {
     constexpr int Length = LEO_B200_TILE_TOKENS / kSegments;
-    __shared__ float2 products[kSegments][kColumns];
-    __shared__ float values[kSegments][kColumns];
+    __shared__ __align__(16) float2 products[kSegments][kColumns];
+    __shared__ __align__(16) float values[kSegments][kColumns];
     __shared__ uint32_t cuts[kSegments];
     const uint32_t place = blockIdx.x / a.groups, group = blockIdx.x - place * a.groups;
     const LeoB200StoryTile tile = a.schedule[place];
