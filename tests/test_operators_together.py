@@ -198,3 +198,26 @@ def test_next_symbol_refuses_before_the_step(arguments):
 
     with pytest.raises(ValueError):
         GpuBackend.next_symbol(Standing(), 65, **arguments)
+
+
+@pytest.mark.gpu
+def test_the_greedy_pick_is_the_most_likely_class(native_lib):
+    """Without rules next_symbol gives the arg-max of the step's probabilities, the end only where it is that."""
+    from leo_b200.backend import GpuBackend
+    from leo_b200.configs import WORKLOADS
+    from leo_b200.ctypes_types import BEGIN_DOCUMENT, END_DOCUMENT, TRAINING
+    from leo_b200.model import HostModel
+    from leo_b200.synthetic import story_stream
+
+    wl = WORKLOADS["test"]
+    with GpuBackend(HostModel.initialize(wl.config, wl.topology), device=0, max_lanes=4) as gpu:
+        gpu.train_story_batch(story_stream(1, 4, 16, 48), TRAINING)
+        gpu.begin_document()
+        gpu.advance_frozen_batch([(BEGIN_DOCUMENT, None)])
+        for byte in b"once upon a time, ":
+            symbol, chance = gpu.next_symbol(byte)
+            p = gpu.lane_array(gpu.CANONICAL_LANE, "probabilities", capacity=4 * 257).astype(np.float64)
+            # the logarithms are floats: classes a rounding of theirs apart may be taken for equal
+            taken = 256 if symbol == END_DOCUMENT else symbol
+            assert np.log(p[taken]) >= np.log(p.max()) * (1 + 2 * U)
+            assert abs(chance - np.log(p[taken] / p.sum())) <= 1e-5
