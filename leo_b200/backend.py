@@ -517,8 +517,11 @@ class GpuBackend:
         ``history`` (bytes or symbol numbers), ``bias`` and ``allowed`` (257
         numbers and truth values, the last for the end of the document), then
         the largest at ``temperature`` 0, or the one that ``uniform`` in [0, 1)
-        falls on.  Arguments are checked before the step; if then no symbol is
-        left to pick, :class:`leo_b200.native.LeoError` is raised after it."""
+        falls on.  (A log-probability is never positive, so ``repetition``
+        multiplies it; the step keeps its probabilities in 32 bits, and a class
+        whose one is 0 there is out at every temperature.)  Arguments are
+        checked before the step; if then no symbol is left to pick,
+        :class:`leo_b200.native.LeoError` is raised after it."""
         import torch
 
         from .logits import pack_allowed, pick_symbols

@@ -25,8 +25,8 @@
 // flight waits for it with every read of shared memory.  Where four stages do
 // not fit, one team with three maps tile i + 1 between the map and the writing
 // of tile i.  81,920 tokens x 1,024 channels (bfloat16, float gates) in 64 stories:
-// 141 us with one team and 129 us with two, 103 us at the rate of a copy; 20,480
-// x 4,096 in 32 stories 141 and 264 us backward, 103 and 180 us at that rate.  A
+// 141 us with one team and 127 us with two, 103 us at the rate of a copy; 20,480
+// x 4,096 in 32 stories 141 and 260 us backward, 103 and 180 us at that rate.  A
 // loop of the same loads and stores alone runs at a copy's rate, so the rest is
 // the length of a tile's chain, from its loads to its map, the composing and the writes.
 //
@@ -1099,7 +1099,7 @@ __global__ void __launch_bounds__(Shape<T, G, Shared, Backward>::kThreads, 1) sc
 // a pass over the inputs, and joined to the states after every tile; then the
 // tiles are written by a block each, which reads the inputs once more and waits
 // for nothing.  One document of 65,537 tokens x 257 channels, float32 with one gate
-// a channel: 66 us forward and 92 us backward, 104 and 137 us in one pass (21 and 31 us
+// a channel: 66 us forward and 90 us backward, 104 and 137 us in one pass (21 and 31 us
 // at the rate of a copy; rows of 257 are read and written an element at a time).
 
 // Calls body(true_type) for a segment that is whole and inside a story, as most

@@ -908,10 +908,12 @@ __global__ void __launch_bounds__(256) narrow_loss_kernel(const __grid_constant_
 // weights, the gradient.  The first two are a warp's own, by its own largest
 // logit, so that the warps meet once.  A row that fits is copied into shared memory first,
 // each thread the groups that it will sweep, so that it comes from memory once
-// and three blocks an SM overlap their copies with the others' sweeps; a larger one
-// is read in every sweep, the last two times out of L2.  2,048 x 32,001 bfloat16: 63 us
-// (40 us at a copy's rate; two exponentials a symbol fill three quarters of the issue
-// slots with what goes with them), 87 us with the row in registers and two blocks.
+// and three blocks an SM overlap their copies with the others' sweeps.  2,048 x 32,001
+// bfloat16: 63 us (40 us at a copy's rate; two exponentials a symbol fill three quarters
+// of the issue slots with what goes with them), 87 us with the row in registers and two
+// blocks.  A larger row is read in every sweep, in part out of L2: 400 x 131,072 float32
+// come from memory 2.2 times, and 1,024 of them take 377 us (165 us at a copy's rate).
+// The float32 form of 512 threads spills 28 bytes a thread at its 40 registers.
 template <typename T, int Threads, bool Held>
 __global__ void __launch_bounds__(Threads, Held ? 3 : 2) wide_loss_kernel(const __grid_constant__ LossArgs a) {
     extern __shared__ __align__(16) unsigned char dynamic[];
@@ -1035,7 +1037,7 @@ template <typename T, int Warps>
 void launch_pick(const LogitArgs& a, cudaStream_t stream) {
     const uint32_t all = (a.vocabulary + 7 + kStepSymbols - 1) / kStepSymbols;
     uint32_t blocks = 1;
-    // two blocks an SM and no second wave of them: 64 rows of 131,072 take 70 us in 512 blocks, 61 us in 256
+    // two blocks on each of 148 SMs and no second wave: 64 rows of 131,072 take 59 us in 512 blocks, 54 us in 256
     while (blocks < 8 && blocks * 2 * Warps <= all && (uint64_t)a.rows * blocks * 2 <= 296) blocks *= 2;
     if (all > 2048) blocks = 8;
     const uint32_t steps = (all + blocks - 1) / blocks;

@@ -16,7 +16,8 @@ Types: float32, bfloat16 or float16 drives; gates of the same type or float32
 (slow decays such as 0.999 are 1 in bfloat16); states between tokens, initial
 and final states are float32.  The calls run asynchronously on the current
 stream of the tensors' device, or on ``stream``, and can be captured into a
-CUDA graph.  PyTorch only owns the memory; no gradient is recorded for autograd.
+CUDA graph.  PyTorch only owns the memory; no gradient is recorded for autograd,
+and a tensor that asks for one, or carries a forward-mode tangent, is refused.
 """
 
 from __future__ import annotations
@@ -216,7 +217,8 @@ def gated_scan_gave_up(device: int = 0) -> bool:
 
 def gated_step(drive, decay, state, stream=None):
     """One token for each lane: ``state`` (float32 [lanes, channels]) becomes
-    ``decay * state + drive`` in place; returns it in the drive's type.
+    ``decay * state + drive`` in place (for autograd too: a backward pass that
+    saved ``state`` before fails); returns it in the drive's type.
     ``drive``: [lanes, channels]; ``decay``: the same shape, or [channels]."""
     device = device_of("drive", drive)
     code, stride = dtype_code("drive", drive), row_stride("drive", drive)

@@ -140,7 +140,8 @@ def adjust_logits(logits, *, history=None, lengths=None, repetition=1.0, presenc
     and another one multiplied by it, then ``presence + frequency * c`` is
     taken off.  ``bias`` (float32 ``[vocabulary]`` or ``[rows, vocabulary]``)
     is added, and what the mask forbids becomes -inf.  ``out`` may be
-    ``logits`` itself; another one must not overlap it."""
+    ``logits`` itself; another one must not overlap it.  (A backward pass that
+    saved ``out`` before fails, as after any operation in place.)"""
     device, code, stride = _check_logits(logits)
     rules = _Rules(logits, device, history, lengths, repetition, presence, frequency, bias, allowed, state)
     rows, vocabulary = logits.shape
