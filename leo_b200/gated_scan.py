@@ -151,9 +151,12 @@ def gated_scan(drive, decay, layout: StoryLayout, initial=None, keep_carries: bo
 
     ``drive``: [tokens, channels]; ``decay``: the same shape, or [channels] for
     one fixed decay a channel (the elements of a row adjacent, rows at any
-    distance, so a slice of a wider projection will do).  ``initial``: float32
-    [stories, channels], zero if ``None``.  ``keep_carries``: keep what
-    :func:`gated_scan_backward` needs."""
+    distance, so a slice of a wider projection will do).  Gates are meant to lie
+    in [-1, 1]; larger ones do as long as the product of those of any span of a
+    story stays finite (float32).  An infinite state stays infinite, but may be
+    NaN after eight gates in a row whose product is 0 in float32, as after a gate
+    of 0.  ``initial``: float32 [stories, channels], zero if ``None``.
+    ``keep_carries``: keep what :func:`gated_scan_backward` needs."""
     device, code, stride, (decay_code, decay_stride, shared) = _check_scan(drive, decay, layout, initial)
     tokens, channels = drive.shape
     L = native.lib()
